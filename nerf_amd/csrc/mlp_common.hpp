@@ -291,5 +291,12 @@ template <> struct Prec<NERF_PREC_FP16> {
     }
 };
 
+// x^2 + y^2 + z^2 with each rounding fixed, whichever instructions the compiler has: the square of y is added without one
+// of its own, the others are rounded first
+__device__ __forceinline__ float square_sum(float x, float y, float z) {
+#pragma clang fp contract(off)
+    return __builtin_fmaf(y, y, x * x) + z * z;
+}
+
 }  // namespace mlp
 }  // namespace nerf

@@ -240,7 +240,7 @@ __global__ __launch_bounds__(CHAIN_THREADS, 2) void mlp_fwd_kernel(const FwdArgs
             px = __fadd_rn(r.ox, __fmul_rn(r.dx, r.z));        // nerf.py:409
             py = __fadd_rn(r.oy, __fmul_rn(r.dy, r.z));
             pz = __fadd_rn(r.oz, __fmul_rn(r.dz, r.z));
-            const float n = sqrtf(__fadd_rn(__fadd_rn(__fmul_rn(r.dx, r.dx), __fmul_rn(r.dy, r.dy)), __fmul_rn(r.dz, r.dz)));
+            const float n = sqrtf(square_sum(r.dx, r.dy, r.dz));
             vx = r.dx / n; vy = r.dy / n; vz = r.dz / n;       // nerf.py:417
         }
         encode<PREC, 10, PE_KS>(px, py, pz, h, pe);

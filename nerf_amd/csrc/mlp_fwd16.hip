@@ -165,7 +165,7 @@ __global__ __launch_bounds__(CHAIN_THREADS, 2) void mlp_fwd16_kernel(const Fwd16
         for (int ct = 0; ct < 2; ++ct) {
             const float* f = reinterpret_cast<const float*>(lds + in_base + ct * 7 * 256) + lane;
             const float dx = f[256], dy = f[320], dz = f[384];
-            const float nrm = sqrtf(__fadd_rn(__fadd_rn(__fmul_rn(dx, dx), __fmul_rn(dy, dy)), __fmul_rn(dz, dz)));
+            const float nrm = sqrtf(square_sum(dx, dy, dz));
             encode16<PREC, 4, 1>(dx / nrm, dy / nrm, dz / nrm, g, &vpe[0][ct], 2);          // nerf.py:417
         }
     };
