@@ -48,6 +48,9 @@ enum {
 
 /* precision selector of the MLP kernels (operand type; accumulation is fp32) */
 enum { NERF_PREC_BF16 = 0, NERF_PREC_FP16 = 1 };
+/* element type of the operators on tensors of any of the three types (nerf_embed_*, nerf_grouped_*, nerf_scan_*): the
+ * two above or this */
+enum { NERF_PREC_FP32 = 2 };
 
 int nerf_version(void);
 const char *nerf_error_string(int code);
@@ -364,6 +367,81 @@ int nerf_mlp_bwd_data(int64_t M, const float *d_raw, const void *packed, int pre
 int nerf_mlp_bwd_weights(int64_t M, const void *packed, const void *saved, const void *dz, int precision,
                          const float *grad_scale, void *partial, int64_t partial_bytes, float *d_params,
                          void *stream);
+
+/* ------------------------------------------------------------------------
+ * Rows grouped by an id: sub-networks chosen per point, per-image codes, feature tables.  The reference has one network
+ * for all points (models/nerf.py:155-209) and feeds it encoded positions only (:68-76); these calls stand beside those.
+ * `precision`: NERF_PREC_BF16, NERF_PREC_FP16 or NERF_PREC_FP32, the type of every tensor named void* below.
+ *
+ * Grouping.  ids [n] of id_bytes 4 (int32) or 8 (int64).  order [n]: the rows 0 .. n-1 sorted by id, rows of one id in
+ * their own order; offsets [n_groups + 1]: group g is order[offsets[g]] .. order[offsets[g+1] - 1].  An id outside
+ * [0, n_groups) belongs to no group; such rows come last.  tile_base (nullable) [n_groups + 2]: the number of 128-row
+ * tiles of the groups before each (the rows of no group count as one more group), as nerf_grouped_* read it.  keys
+ * (nullable) [n]: the sorted ids, n_groups for rows of no group, as nerf_embed_bwd reads them.  workspace:
+ * nerf_group_rows_workspace_bytes bytes, 256-byte aligned.  n = 0 writes nothing.  Limits: n <= 2^31 - 129,
+ * 1 <= n_groups <= 2^24.
+ */
+int64_t nerf_group_rows_workspace_bytes(int64_t n, int64_t n_groups);
+int nerf_group_rows(int64_t n, const void *ids, int id_bytes, int64_t n_groups, int32_t *order, int32_t *offsets,
+                    int32_t *tile_base, int32_t *keys, void *workspace, int64_t workspace_bytes, void *stream);
+/* Rows that are in group order already: offsets_in [n_groups + 1] made safe to index with (offsets[0] = 0, never below
+ * the one before, never above n), and their tile_base.  offsets must not alias offsets_in. */
+int nerf_group_offsets(int64_t n, int64_t n_groups, const int32_t *offsets_in, int32_t *offsets, int32_t *tile_base,
+                       void *stream);
+
+/* out [n, dim] = scale * table[ids], an id outside [0, rows) gives zeros; table rows are table_ld elements apart. */
+int nerf_embed_fwd(int64_t n, const void *ids, int id_bytes, int64_t rows, int64_t dim, const void *table, int64_t table_ld,
+                   float scale, int precision, void *out, void *stream);
+/* d_table [rows, dim] (written, not accumulated) = scale * the sum of d_out's rows by id, from order, offsets and keys of
+ * nerf_group_rows(ids, rows).  fp32 sums in a fixed order, no atomics.  dim <= 2^20. */
+int64_t nerf_embed_bwd_workspace_bytes(int64_t n, int64_t rows, int64_t dim);
+int nerf_embed_bwd(int64_t n, int64_t rows, int64_t dim, const int32_t *order, const int32_t *offsets, const int32_t *keys,
+                   const void *d_out, int64_t d_out_ld, float scale, int precision, void *d_table, void *workspace,
+                   int64_t workspace_bytes, void *stream);
+
+/* Linear layers of n_groups sub-networks, weight [n_groups, N, K], bias (nullable) [n_groups, N]:
+ *   y[i] = act(weight[g(i)] x[i] + bias[g(i)]), act = ReLU when relu (keeps a NaN), zeros for rows of no group.
+ * order (nullable: rows are in group order), offsets and tile_base from nerf_group_rows or nerf_group_offsets for the same
+ * n and n_groups; rows are read and written where they are (row order[p] of x [n, K], y [n, N]).  order must not name a
+ * row twice (nerf_group_rows never does).
+ * The backward calls take the layer's output y when it had a ReLU, else NULL: dZ = d_y [y > 0].
+ *   nerf_grouped_bwd_data:    d_x[i] = weight[g(i)]^T dZ[i] [n, K], zeros for rows of no group
+ *   nerf_grouped_bwd_weights: d_weight[g] = sum dZ[i] x[i]^T, d_bias[g] (nullable) = sum dZ[i] over the rows of g; written,
+ *                             zeros for a group without rows; fixed order of summation, no atomics
+ * Products are summed in fp32 (fp32 operands: exact products).  n_groups <= 65535, K and N <= 65536.  *_ld: elements
+ * between rows.  workspace 256-byte aligned. */
+int nerf_grouped_fwd(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets, const int32_t *tile_base,
+                     int K, int N, const void *x, int64_t x_ld, const void *weight, const void *bias, int relu,
+                     int precision, void *y, void *stream);
+int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets, const int32_t *tile_base,
+                          int K, int N, const void *d_y, int64_t d_y_ld, const void *y, const void *weight, int precision,
+                          void *d_x, void *stream);
+int64_t nerf_grouped_bwd_weights_workspace_bytes(int64_t n, int64_t n_groups, int K, int N);
+int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets,
+                             const int32_t *tile_base, int K, int N, const void *d_y, int64_t d_y_ld, const void *y,
+                             const void *x, int64_t x_ld, int precision, void *d_weight, void *d_bias, void *workspace,
+                             int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Gated linear recurrence along the samples of a ray: h[t] = gate[t] h[t-1] + value[t] from `state` (nullable = 0), for B
+ * sequences of T samples and D channels; with gate = 1 - alpha and value = alpha c, back to front, the compositing of
+ * models/nerf.py:430-456 for features of any width.  gate_shared: one gate per sample, else one per channel.
+ * *_sb, *_st: elements between sequences and between samples (0 to repeat); channels are contiguous.  reverse: from the
+ * last sample to the first.  state, last, d_last, d_state: fp32 [B, D]; h, d_h, d_value [B, T, D], d_gate [B, T, D or 1]
+ * contiguous.  Where D is a multiple of 16 bytes, value, h, d_h and d_value (and a gate per channel) are 16-byte aligned
+ * and their strides multiples of it (NERF_E_ALIGN).
+ * states (nullable in the forward): nerf_scan_states_floats floats, the fp32 states the backward starts from.
+ * Backward: d_h, d_last nullable = 0; d_gate, d_value, d_state nullable = not wanted.  T = 0 writes nothing.
+ * The product of consecutive gates has to stay in the range of fp32 wherever the state in front of them is not zero. */
+int64_t nerf_scan_states_floats(int64_t B, int64_t T, int64_t D, int precision);
+int64_t nerf_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, int gate_shared, int backward, int precision);
+int nerf_scan_fwd(int64_t B, int64_t T, int64_t D, const void *gate, int64_t gate_sb, int64_t gate_st, int gate_shared,
+                  const void *value, int64_t value_sb, int64_t value_st, const float *state, int reverse, int precision,
+                  void *h, float *last, float *states, void *workspace, int64_t workspace_bytes, void *stream);
+int nerf_scan_bwd(int64_t B, int64_t T, int64_t D, const void *gate, int64_t gate_sb, int64_t gate_st, int gate_shared,
+                  const void *value, int64_t value_sb, int64_t value_st, const float *state, const float *states,
+                  const void *d_h, const float *d_last, int reverse, int precision, void *d_gate, void *d_value,
+                  float *d_state, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Adam on a flat fp32 buffer -- the optimizer.step() of scripts/train_nerf.py:336
  * (torch.optim.Adam, no weight decay, no amsgrad).  step is 1-based. */

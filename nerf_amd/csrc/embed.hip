@@ -1,0 +1,369 @@
+// Rows of a table by id, scaled, and the table's gradient: per-image codes and feature tables beside the positional
+// encoding.  (The reference feeds its networks encoded positions only, models/nerf.py:68-76.)
+//
+//   out[i] = scale * table[ids[i]]          an id outside [0, rows) gives a row of zeros
+//   d_table[v] = scale * sum of d_out[i] over the i with ids[i] = v
+//
+// Forward: bound by memory, one 16-byte piece of a row per lane, four rows in flight per lane group.
+//
+// Gradient: the positions come sorted by id (nerf_group_rows).  A lane group of LPR lanes sums R consecutive sorted
+// positions, a lane holding VEC columns in fp32; a run of equal ids that begins and ends inside is finished at once.
+// The ragged ends of a workgroup's lane groups meet in LDS, those of the workgroups in the workspace, where a second
+// kernel adds them up in order of position and writes zeros for the rows that nothing reads.  No atomics: the result
+// does not depend on timing, and an id that holds all positions is spread over all workgroups like any other.
+#include "elems.hpp"
+#include "groups.hpp"
+
+namespace nerf {
+namespace emb {
+
+constexpr int THREADS = 256;
+constexpr int FWD_ROWS = 4;      // rows a lane group has in flight
+constexpr int LONG_RUN = 16;     // workgroup partials of one row above which a whole workgroup adds them up
+
+// LPR lanes share a row; columns beyond LPR * VEC are walked by the same lanes
+template <typename T, int VEC, typename ID>
+__global__ __launch_bounds__(THREADS) void fwd_kernel(int64_t n, const ID* __restrict__ ids, int64_t rows, int dim, int lpr,
+                                                      const T* __restrict__ table, int64_t ld, float scale, T* __restrict__ out) {
+    const int groups = THREADS / lpr;
+    const int sub = (int)threadIdx.x / lpr, l = (int)threadIdx.x % lpr;
+    const int64_t step = (int64_t)gridDim.x * groups * FWD_ROWS;
+    for (int64_t i0 = ((int64_t)blockIdx.x * groups + sub) * FWD_ROWS; i0 < n; i0 += step) {
+        int64_t id[FWD_ROWS];
+#pragma unroll
+        for (int j = 0; j < FWD_ROWS; ++j) id[j] = i0 + j < n ? (int64_t)ids[i0 + j] : -1;
+        for (int c = l * VEC; c < dim; c += lpr * VEC) {
+            Pack<T, VEC> x[FWD_ROWS];
+#pragma unroll
+            for (int j = 0; j < FWD_ROWS; ++j) {
+                const bool ok = id[j] >= 0 && id[j] < rows;
+                if (ok) x[j] = load_pack<T, VEC>(table + id[j] * ld + c);
+                else
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) x[j].v[v] = (T)0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < FWD_ROWS; ++j) {
+                if (i0 + j >= n) break;
+                const bool ok = id[j] >= 0 && id[j] < rows;
+                Pack<T, VEC> y;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) y.v[v] = ok ? (T)((float)x[j].v[v] * scale) : (T)0.0f;
+                store_pack<T, VEC>(out + (i0 + j) * dim + c, y);
+            }
+        }
+    }
+}
+
+struct BwdArgs {
+    int64_t n, rows;
+    int dim, lpr, per;             // per: sorted positions of one lane group
+    const int32_t *order, *offsets, *keys;
+    float scale;
+    float* part;                   // [2 * workgroups][dim]: slot 2w a run that came in from the left of workgroup w,
+};                                 // slot 2w + 1 one that began in it and goes on to the right
+
+template <typename T, int VEC>
+__device__ __forceinline__ void write_row(T* d_table, int64_t row, int dim, int col, const float (&acc)[VEC], float scale) {
+    Pack<T, VEC> y;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) y.v[v] = (T)(acc[v] * scale);
+    store_pack<T, VEC>(d_table + row * dim + col, y);
+}
+
+template <int VEC>
+__device__ __forceinline__ void write_part(float* part, int64_t slot, int dim, int col, const float (&acc)[VEC]) {
+    Pack<float, VEC> y;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) y.v[v] = acc[v];
+    if constexpr (VEC == 8) {
+        Pack<float, 4> a, b;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) { a.v[v] = acc[v]; b.v[v] = acc[4 + v]; }
+        store_pack<float, 4>(part + slot * dim + col, a);
+        store_pack<float, 4>(part + slot * dim + col + 4, b);
+    } else {
+        store_pack<float, VEC>(part + slot * dim + col, y);
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void add_part(float (&acc)[VEC], const float* p) {
+    if constexpr (VEC == 8) {
+        const Pack<float, 4> a = load_pack<float, 4>(p), b = load_pack<float, 4>(p + 4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) { acc[v] += a.v[v]; acc[4 + v] += b.v[v]; }
+    } else {
+        const Pack<float, VEC> a = load_pack<float, VEC>(p);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[v] += a.v[v];
+    }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(THREADS) void bwd_sum_kernel(BwdArgs a, const T* __restrict__ d_out, int64_t ld, T* __restrict__ d_table) {
+    constexpr int BATCH = 8;
+    __shared__ float head[THREADS * VEC], tail[THREADS * VEC];
+    __shared__ int head_state[THREADS], tail_key[THREADS];         // head: 0 none, 1 ends in its lane group, 2 goes on
+    const int lpr = a.lpr, groups = THREADS / lpr;
+    const int sub = (int)threadIdx.x / lpr, l = (int)threadIdx.x % lpr;
+    const int col = ((int)blockIdx.y * lpr + l) * VEC;
+    const bool on = col < a.dim;
+    const int64_t nv = a.offsets[a.rows];                          // positions behind it belong to no row
+    const int64_t p0 = ((int64_t)blockIdx.x * groups + sub) * a.per;
+    const int64_t p1 = p0 + a.per < nv ? p0 + a.per : nv;
+    int hstate = 0, tkey = -1;
+    if (p0 < p1) {
+        float acc[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+        int key = a.keys[p0];
+        bool from_left = p0 > 0 && a.keys[p0 - 1] == key;
+        for (int64_t p = p0; p < p1; p += BATCH) {
+            int k[BATCH];
+            Pack<T, VEC> x[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                const int64_t q = p + j < p1 ? p + j : p1 - 1;
+                k[j] = a.keys[q];
+                const int64_t row = a.order[q];
+                if (on) x[j] = load_pack<T, VEC>(d_out + row * ld + col);
+            }
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                if (p + j >= p1) break;
+                if (k[j] != key) {                                 // the run of `key` ends here
+                    if (from_left) {
+                        hstate = 1;
+                        if (on)
+#pragma unroll
+                            for (int v = 0; v < VEC; ++v) head[threadIdx.x * VEC + v] = acc[v];
+                    } else if (on) {
+                        write_row<T, VEC>(d_table, key, a.dim, col, acc, a.scale);
+                    }
+                    from_left = false;
+                    key = k[j];
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+                }
+                if (on)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) acc[v] += (float)x[j].v[v];
+            }
+        }
+        const bool goes_on = p1 < nv && a.keys[p1] == key;
+        if (from_left) {
+            hstate = goes_on ? 2 : 1;
+            if (on)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) head[threadIdx.x * VEC + v] = acc[v];
+        } else if (goes_on) {
+            tkey = key;
+            if (on)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) tail[threadIdx.x * VEC + v] = acc[v];
+        } else if (on) {
+            write_row<T, VEC>(d_table, key, a.dim, col, acc, a.scale);
+        }
+    }
+    if (l == 0) { head_state[sub] = hstate; tail_key[sub] = tkey; }
+    __syncthreads();
+    if (sub != 0 || !on) return;
+    float acc[VEC];
+    bool open = false, from_left = false;
+    int key = -1;
+    for (int g = 0; g < groups; ++g) {
+        const int at = (g * lpr + l) * VEC;
+        const int hs = head_state[g], tk = tail_key[g];
+        if (hs) {
+            if (!open) {                                           // g == 0: the run comes from an earlier workgroup
+                from_left = open = true;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+            }
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) acc[v] += head[at + v];
+            if (hs == 1) {
+                if (from_left) write_part<VEC>(a.part, 2 * (int64_t)blockIdx.x, a.dim, col, acc);
+                else write_row<T, VEC>(d_table, key, a.dim, col, acc, a.scale);
+                open = false;
+            }
+        }
+        if (tk >= 0) {
+            open = true;
+            from_left = false;
+            key = tk;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) acc[v] = tail[at + v];
+        }
+    }
+    if (open) write_part<VEC>(a.part, 2 * (int64_t)blockIdx.x + (from_left ? 0 : 1), a.dim, col, acc);
+}
+
+// Rows whose positions span several workgroups of bwd_sum_kernel, and rows that hold none.
+template <typename T, int VEC>
+__global__ __launch_bounds__(THREADS) void bwd_join_kernel(BwdArgs a, T* __restrict__ d_table) {
+    __shared__ float red[THREADS * VEC];
+    const int lpr = a.lpr, groups = THREADS / lpr;
+    const int sub = (int)threadIdx.x / lpr, l = (int)threadIdx.x % lpr;
+    const int col = ((int)blockIdx.y * lpr + l) * VEC;
+    const bool on = col < a.dim;
+    const int64_t span = (int64_t)groups * a.per;
+    const int64_t row0 = (int64_t)blockIdx.x * groups;
+    const int64_t row = row0 + sub;
+    bool any_long = false;
+    if (row < a.rows) {
+        const int64_t s = a.offsets[row], e = a.offsets[row + 1];
+        float acc[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+        if (s == e) {
+            if (on) {
+                Pack<T, VEC> zero;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) zero.v[v] = (T)0.0f;
+                store_pack<T, VEC>(d_table + row * a.dim + col, zero);
+            }
+        } else {
+            const int64_t w0 = s / span, w1 = (e - 1) / span;
+            any_long = w1 - w0 >= LONG_RUN;
+            if (w1 > w0 && !any_long && on) {
+                add_part<VEC>(acc, a.part + (2 * w0 + 1) * a.dim + col);
+                for (int64_t w = w0 + 1; w <= w1; ++w) add_part<VEC>(acc, a.part + 2 * w * a.dim + col);
+                write_row<T, VEC>(d_table, row, a.dim, col, acc, a.scale);
+            }
+        }
+    }
+    if (!__syncthreads_or(any_long)) return;
+    for (int g = 0; g < groups; ++g) {
+        if (row0 + g >= a.rows) break;
+        const int64_t s = a.offsets[row0 + g], e = a.offsets[row0 + g + 1];
+        if (s == e) continue;
+        const int64_t w0 = s / span, w1 = (e - 1) / span;
+        if (w1 - w0 < LONG_RUN) continue;
+        float acc[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+        if (on) {
+            // lane group `sub` takes a run of consecutive workgroups, so the order of the sum is that of the positions
+            const int64_t cnt = (w1 - w0 + 1 + groups - 1) / groups;
+            const int64_t from = w0 + sub * cnt, to = from + cnt < w1 + 1 ? from + cnt : w1 + 1;
+#pragma unroll 8
+            for (int64_t w = from; w < to; ++w) add_part<VEC>(acc, a.part + (2 * w + (w == w0 ? 1 : 0)) * a.dim + col);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) red[threadIdx.x * VEC + v] = acc[v];
+        __syncthreads();
+        if (sub == 0 && on) {
+            for (int k = 1; k < groups; ++k)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) acc[v] += red[(k * lpr + l) * VEC + v];
+            write_row<T, VEC>(d_table, row0 + g, a.dim, col, acc, a.scale);
+        }
+        __syncthreads();
+    }
+}
+
+static inline int lanes_per_row(int64_t dim, int vec) {
+    int l = 4;
+    while (l < 64 && (int64_t)l * vec < dim) l <<= 1;
+    return l;
+}
+
+// sorted positions of a lane group: enough workgroups to fill the chip (1024), few enough partial sums
+static inline int positions_per_group(int64_t n, int groups) {
+    int64_t per = (n / ((int64_t)groups * 1024) + 7) / 8 * 8;
+    if (per < 8) per = 8;
+    if (per > 64) per = 64;
+    return (int)per;
+}
+
+static inline bool sizes_ok(int64_t n, int64_t rows, int64_t dim) {
+    return n >= 0 && n <= grp::MAX_ROWS && rows >= 1 && rows <= grp::MAX_GROUPS && dim >= 1 && dim <= (1 << 20);
+}
+
+}  // namespace emb
+}  // namespace nerf
+
+extern "C" int nerf_embed_fwd(int64_t n, const void* ids, int id_bytes, int64_t rows, int64_t dim, const void* table, int64_t table_ld,
+                              float scale, int precision, void* out, void* stream) {
+    using namespace nerf;
+    NERF_REQUIRE(emb::sizes_ok(n, rows, dim) && table_ld >= dim, NERF_E_SHAPE);
+    NERF_REQUIRE(elem_ok(precision) && (id_bytes == 4 || id_bytes == 8), NERF_E_DTYPE);
+    if (n == 0) return NERF_OK;
+    NERF_REQUIRE(ids && table && out, NERF_E_NULL);
+    const int es = elem_bytes(precision), full = 16 / es;
+    NERF_REQUIRE(nerf_aligned(ids, (uintptr_t)id_bytes) && nerf_aligned(table, (uintptr_t)es) && nerf_aligned(out, (uintptr_t)es), NERF_E_ALIGN);
+    const bool wide = dim % full == 0 && table_ld % full == 0 && nerf_aligned(table, 16) && nerf_aligned(out, 16);
+    const int lpr = emb::lanes_per_row(dim, wide ? full : 1);
+    const int64_t per_block = (int64_t)(emb::THREADS / lpr) * emb::FWD_ROWS;
+    int64_t blocks = (n + per_block - 1) / per_block;
+    if (blocks > 16384) blocks = 16384;
+    hipStream_t st = (hipStream_t)stream;
+#define NERF_FWD(T, V, ID)                                                                                                      \
+    hipLaunchKernelGGL((emb::fwd_kernel<T, V, ID>), dim3((unsigned)blocks), dim3(emb::THREADS), 0, st, n, (const ID*)ids, rows, (int)dim, \
+                       lpr, (const T*)table, table_ld, scale, (T*)out)
+#define NERF_CALL(T)                                                                      \
+    do {                                                                                  \
+        if (wide && id_bytes == 8) NERF_FWD(T, full_vec<T>(), int64_t);                   \
+        else if (wide) NERF_FWD(T, full_vec<T>(), int32_t);                               \
+        else if (id_bytes == 8) NERF_FWD(T, 1, int64_t);                                  \
+        else NERF_FWD(T, 1, int32_t);                                                     \
+    } while (0)
+    NERF_ELEM_DISPATCH(precision, NERF_CALL);
+#undef NERF_CALL
+#undef NERF_FWD
+    return nerf_launch_status();
+}
+
+extern "C" int64_t nerf_embed_bwd_workspace_bytes(int64_t n, int64_t rows, int64_t dim) {
+    using namespace nerf;
+    if (!emb::sizes_ok(n, rows, dim)) return NERF_E_SHAPE;
+    int64_t most = 0;                       // over the two access widths, which the pointers decide
+    for (int vec : {1, 4, 8}) {
+        const int groups = emb::THREADS / emb::lanes_per_row(dim, vec);
+        const int64_t span = (int64_t)groups * emb::positions_per_group(n, groups);
+        const int64_t b = 2 * ((n + span - 1) / span) * dim * 4;
+        if (b > most) most = b;
+    }
+    return most < 256 ? 256 : most;
+}
+
+extern "C" int nerf_embed_bwd(int64_t n, int64_t rows, int64_t dim, const int32_t* order, const int32_t* offsets, const int32_t* keys,
+                              const void* d_out, int64_t d_out_ld, float scale, int precision, void* d_table, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+    using namespace nerf;
+    NERF_REQUIRE(emb::sizes_ok(n, rows, dim) && d_out_ld >= dim, NERF_E_SHAPE);
+    NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
+    if (n == 0) return NERF_OK;
+    NERF_REQUIRE(order && offsets && keys && d_out && d_table && workspace, NERF_E_NULL);
+    const int es = elem_bytes(precision), full = 16 / es;
+    NERF_REQUIRE(nerf_aligned(d_out, (uintptr_t)es) && nerf_aligned(d_table, (uintptr_t)es) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
+    NERF_REQUIRE(workspace_bytes >= nerf_embed_bwd_workspace_bytes(n, rows, dim), NERF_E_WORKSPACE);
+    const bool wide = dim % full == 0 && d_out_ld % full == 0 && nerf_aligned(d_out, 16) && nerf_aligned(d_table, 16);
+    const int vec = wide ? full : 1;
+    emb::BwdArgs a = {};
+    a.n = n; a.rows = rows; a.dim = (int)dim;
+    a.lpr = emb::lanes_per_row(dim, vec);
+    const int groups = emb::THREADS / a.lpr;
+    a.per = emb::positions_per_group(n, groups);
+    a.order = order; a.offsets = offsets; a.keys = keys; a.scale = scale; a.part = (float*)workspace;
+    const int64_t span = (int64_t)groups * a.per;
+    const unsigned cols = (unsigned)((dim + (int64_t)a.lpr * vec - 1) / ((int64_t)a.lpr * vec));
+    const dim3 g1((unsigned)((n + span - 1) / span), cols), g2((unsigned)((rows + groups - 1) / groups), cols), block(emb::THREADS);
+    hipStream_t st = (hipStream_t)stream;
+#define NERF_BWD(T, V)                                                                                                        \
+    do {                                                                                                                      \
+        hipLaunchKernelGGL((emb::bwd_sum_kernel<T, V>), g1, block, 0, st, a, (const T*)d_out, d_out_ld, (T*)d_table);          \
+        hipLaunchKernelGGL((emb::bwd_join_kernel<T, V>), g2, block, 0, st, a, (T*)d_table);                                    \
+    } while (0)
+#define NERF_CALL(T)                            \
+    do {                                        \
+        if (wide) NERF_BWD(T, full_vec<T>());   \
+        else NERF_BWD(T, 1);                    \
+    } while (0)
+    NERF_ELEM_DISPATCH(precision, NERF_CALL);
+#undef NERF_CALL
+#undef NERF_BWD
+    return nerf_launch_status();
+}

@@ -1,0 +1,606 @@
+// Gated linear recurrence along the samples of a ray, with its backward pass:
+//   h[t] = a[t] h[t-1] + v[t],   h[-1] = state,   per channel; a is one gate per sample or one per channel.
+// With a = 1 - alpha and v = alpha c, back to front, this is alpha compositing (models/nerf.py:430-456) of a feature of
+// any width; it also carries a ray's state on by one sample (T = 1) and serves sequences far longer than a ray.
+// Backward, with G[t] = dL/dh[t] in full:  u[t] = a[t] (g[t] + u[t+1]),  G[t] = g[t] + u[t+1],  u[T] = d_last,
+//   d_v[t] = G[t],   d_a[t] = G[t] h[t-1] (summed over the channels when they share the gate),   d_state = u[0].
+//
+// Both recurrences are affine maps of the state, x -> A x + H, and maps compose, so time is cut: a thread holds V channels
+// of L consecutive samples in registers and reduces them to one map, the threads of a tile compose theirs (shuffles within
+// a wave, LDS across waves), and each thread then walks its samples once more from its true state.  Every input is read
+// once and every output written once.  States, maps and sums are fp32; outputs are rounded once at the store.
+//
+// The backward recomputes h in registers from a and v instead of reading the rounded h: it reads as much either way, and
+// d_a then has the fp32 state in it.  The forward leaves the fp32 state at each tile boundary for that (4 / tile bytes per
+// element).
+//
+// When the sequences alone do not fill the chip, a sequence is cut into segments: a first pass over a and v (or g) leaves
+// each segment's map, a small kernel composes them, and the main pass starts every segment from its state.  That reads
+// the inputs twice; the second time they come from the last-level cache as far as they fit.
+#include "elems.hpp"
+
+namespace nerf {
+namespace scan {
+
+constexpr int THREADS = 256;
+constexpr int WAVES = THREADS / 64;
+
+template <int V> constexpr int max_len() { return V == 8 ? 4 : 8; }      // samples of a thread
+
+struct Geo {
+    int64_t B, T;
+    int D;
+    int cgl;                // log2 of the lanes that share a row of channels
+    int tg;                 // threads along time of one tile (power of two)
+    int len;                // samples of a thread
+    int seqs;               // sequences of a workgroup
+    int64_t tiles, per_seg, segs;
+    int col_blocks;
+};
+
+struct In {
+    const void* p;
+    int64_t sb, st;         // elements between sequences, between samples
+};
+
+struct Args {
+    Geo g;
+    In gate, value;
+    const float* state;     // [B][D] or NULL
+    int reverse;
+    void* h;
+    float* last;
+    float* states;          // [B][tiles - 1][D] or NULL: state in front of tiles 1 ..
+    const float* seg_in;    // [B][segs][D]: state in front of each segment (segs > 1)
+    float *agg_a, *agg_h;   // [B][segs][D]: maps of the segments
+    // backward
+    const void* d_h;        // [B][T][D] or NULL
+    const float* d_last;    // [B][D] or NULL
+    void *d_gate, *d_value;
+    float* d_state;         // [B][D] or NULL
+    float* gate_part;       // [col_blocks][B * T] when several workgroups share a gate
+};
+
+struct Place {
+    int lane, wave, cg, unit, seq_in, tgi, wd, u, ch;
+    int64_t b;
+    bool on;
+};
+
+template <int V>
+__device__ __forceinline__ Place place(const Geo& g) {
+    Place p;
+    p.lane = threadIdx.x & 63;
+    p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    p.cg = p.lane & ((1 << g.cgl) - 1);
+    const int in_wave = 64 >> g.cgl;
+    p.unit = p.wave * in_wave + (p.lane >> g.cgl);
+    p.seq_in = p.unit / g.tg;
+    p.tgi = p.unit % g.tg;
+    p.wd = g.tg < in_wave ? g.tg : in_wave;       // threads of the tile in this wave
+    p.u = p.tgi & (p.wd - 1);
+    p.b = (int64_t)blockIdx.x * g.seqs + p.seq_in;
+    p.ch = ((int)blockIdx.y << g.cgl) * V + p.cg * V;
+    p.on = p.b < g.B && p.ch < g.D;
+    return p;
+}
+
+// A x + H; H alone from a zero state, where the product of the gates may have left the range of the type
+__device__ __forceinline__ float apply(float A, float x, float H) { return x == 0.0f ? H : fmaf(A, x, H); }
+
+// Composes the maps (A, H) of a tile's threads, first to last sample (DOWN: last to first).  carry: the state in front of
+// the tile, replaced by the one behind it; in: the state in front of this thread; A becomes the map of the whole tile.
+// sm: LDS, WAVES * 64 * (V + VA) floats.
+template <int V, int VA, bool DOWN>
+__device__ __forceinline__ void compose(const Geo& g, const Place& p, float (&A)[VA], float (&H)[V], float (&carry)[V], float (&in)[V],
+                                        float* sm) {
+    const int cgn = 1 << g.cgl;
+    const int u = DOWN ? p.wd - 1 - p.u : p.u;
+    const int dir = DOWN ? cgn : -cgn;
+    for (int off = 1; off < p.wd; off <<= 1) {
+        float a2[VA], h2[V];
+        const int src = p.lane + dir * off;
+#pragma unroll
+        for (int v = 0; v < VA; ++v) a2[v] = __shfl(A[v], src, 64);
+#pragma unroll
+        for (int v = 0; v < V; ++v) h2[v] = __shfl(H[v], src, 64);
+        if (u >= off) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) H[v] = apply(A[VA == 1 ? 0 : v], h2[v], H[v]);
+#pragma unroll
+            for (int v = 0; v < VA; ++v) A[v] *= a2[v];
+        }
+    }
+    float ea[VA], eh[V], ta[VA], th[V];                 // the threads before this one; all of the wave
+    const int prev = p.lane + dir;
+    const int top = ((p.lane >> g.cgl) - p.u + (DOWN ? 0 : p.wd - 1)) * cgn + p.cg;
+#pragma unroll
+    for (int v = 0; v < VA; ++v) {
+        const float e = __shfl(A[v], prev, 64);
+        ea[v] = u == 0 ? 1.0f : e;
+        ta[v] = __shfl(A[v], top, 64);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const float e = __shfl(H[v], prev, 64);
+        eh[v] = u == 0 ? 0.0f : e;
+        th[v] = __shfl(H[v], top, 64);
+    }
+    if (g.tg > p.wd) {                                  // the tile spans several waves (block-uniform)
+        const int waves = g.tg / p.wd, first = p.wave & ~(waves - 1);
+        float* mine = sm + p.wave * 64 * (V + VA);
+        __syncthreads();                                // the last tile's values have been read
+        if (u == 0) {
+#pragma unroll
+            for (int v = 0; v < VA; ++v) mine[v * 64 + p.cg] = ta[v];
+#pragma unroll
+            for (int v = 0; v < V; ++v) mine[(VA + v) * 64 + p.cg] = th[v];
+        }
+        __syncthreads();
+        float x[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = carry[v];
+#pragma unroll
+        for (int v = 0; v < VA; ++v) A[v] = 1.0f;
+        for (int k = 0; k < waves; ++k) {
+            const int w = first + (DOWN ? waves - 1 - k : k);
+            const float* s = sm + w * 64 * (V + VA);
+            if (w == p.wave) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) in[v] = x[v];
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = apply(s[(VA == 1 ? 0 : v) * 64 + p.cg], x[v], s[(VA + v) * 64 + p.cg]);
+#pragma unroll
+            for (int v = 0; v < VA; ++v) A[v] *= s[v * 64 + p.cg];
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = x[v];
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) { in[v] = carry[v]; carry[v] = apply(ta[VA == 1 ? 0 : v], carry[v], th[v]); }
+#pragma unroll
+        for (int v = 0; v < VA; ++v) A[v] = ta[v];
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) in[v] = apply(ea[VA == 1 ? 0 : v], in[v], eh[v]);
+}
+
+template <typename T, int V>
+struct Raw { Pack<T, V> x[max_len<V>()]; };
+
+// samples t0 .. t0 + len - 1 of one input, `fill` where there is none
+template <typename T, int V>
+__device__ __forceinline__ void fetch(Raw<T, V>& r, const In& in, const Geo& g, int reverse, int64_t b, int64_t t0, int ch, bool on, float fill) {
+    const T* base = (const T*)in.p + b * in.sb + ch;
+#pragma unroll
+    for (int j = 0; j < max_len<V>(); ++j) {
+        const int64_t t = t0 + j;
+        if (on && j < g.len && t < g.T) r.x[j] = load_pack<T, V>(base + (reverse ? g.T - 1 - t : t) * in.st);
+        else
+#pragma unroll
+            for (int v = 0; v < V; ++v) r.x[j].v[v] = (T)fill;
+    }
+}
+
+// gates of the thread's samples; a shared gate is one value that all lanes of a row read from the same address
+template <typename T, int V, bool SHARED>
+struct Gates {
+    static constexpr int VA = SHARED ? 1 : V;
+    Pack<T, VA> x[max_len<V>()];
+    __device__ __forceinline__ float at(int j, int v) const { return (float)x[j].v[SHARED ? 0 : v]; }
+};
+template <typename T, int V, bool SHARED>
+__device__ __forceinline__ void fetch_gates(Gates<T, V, SHARED>& r, const Args& a, int64_t b, int64_t t0, int ch, bool on) {
+    constexpr int VA = SHARED ? 1 : V;
+    const T* base = (const T*)a.gate.p + b * a.gate.sb + (SHARED ? 0 : ch);
+#pragma unroll
+    for (int j = 0; j < max_len<V>(); ++j) {
+        const int64_t t = t0 + j;
+        if (on && j < a.g.len && t < a.g.T) r.x[j] = load_pack<T, VA>(base + (a.reverse ? a.g.T - 1 - t : t) * a.gate.st);
+        else
+#pragma unroll
+            for (int v = 0; v < VA; ++v) r.x[j].v[v] = (T)1.0f;
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void load_floats(float (&x)[V], const float* p, bool on) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = on && p ? p[v] : 0.0f;
+}
+template <int V>
+__device__ __forceinline__ void store_floats(float* p, const float (&x)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] = x[v];
+}
+
+// AGG: only the map of each segment (agg_a, agg_h); otherwise the outputs.
+template <typename T, int V, bool SHARED, bool AGG>
+__global__ __launch_bounds__(THREADS) void fwd_kernel(Args a) {
+    constexpr int VA = SHARED ? 1 : V, L = max_len<V>();
+    __shared__ float sm[WAVES * 64 * (V + VA)];
+    const Geo& g = a.g;
+    const Place p = place<V>(g);
+    const int64_t seg = blockIdx.z;
+    const int64_t first = seg * g.per_seg, stop = first + g.per_seg < g.tiles ? first + g.per_seg : g.tiles;
+    const int64_t row = p.b * g.D + p.ch;
+    float carry[V], allA[VA];
+    if (AGG) load_floats<V>(carry, nullptr, false);
+    else if (g.segs > 1) load_floats<V>(carry, a.seg_in + (p.b * g.segs + seg) * g.D + p.ch, p.on);
+    else load_floats<V>(carry, a.state ? a.state + row : nullptr, p.on);
+#pragma unroll
+    for (int v = 0; v < VA; ++v) allA[v] = 1.0f;
+    const int steps = g.tg * g.len;
+    T* h_out = (T*)a.h + p.b * g.T * g.D + p.ch;
+    for (int64_t i = first; i < stop; ++i) {
+        const int64_t t0 = i * steps + p.tgi * g.len;
+        Gates<T, V, SHARED> ga;
+        Raw<T, V> va;
+        fetch_gates<T, V, SHARED>(ga, a, p.b, t0, p.ch, p.on);
+        fetch<T, V>(va, a.value, g, a.reverse, p.b, t0, p.ch, p.on, 0.0f);
+        if (!AGG && a.states && i > 0 && p.on && p.tgi == 0)
+            store_floats<V>(a.states + (p.b * (g.tiles - 1) + i - 1) * g.D + p.ch, carry);
+        float A[VA], H[V], x[V];
+#pragma unroll
+        for (int v = 0; v < VA; ++v) A[v] = 1.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) H[v] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) H[v] = fmaf(ga.at(j, v), H[v], (float)va.x[j].v[v]);
+#pragma unroll
+            for (int v = 0; v < VA; ++v) A[v] *= ga.at(j, v);
+        }
+        compose<V, VA, false>(g, p, A, H, carry, x, sm);
+        if (AGG) {
+#pragma unroll
+            for (int v = 0; v < VA; ++v) allA[v] *= A[v];
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            Pack<T, V> y;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                x[v] = fmaf(ga.at(j, v), x[v], (float)va.x[j].v[v]);
+                y.v[v] = (T)x[v];
+            }
+            const int64_t t = t0 + j;
+            if (p.on && j < g.len && t < g.T) store_pack<T, V>(h_out + (a.reverse ? g.T - 1 - t : t) * g.D, y);
+        }
+    }
+    if (!p.on || p.tgi != 0) return;
+    if (AGG) {
+        const int64_t at = (p.b * g.segs + seg) * g.D + p.ch;
+        store_floats<V>(a.agg_h + at, carry);
+#pragma unroll
+        for (int v = 0; v < V; ++v) a.agg_a[at + v] = allA[VA == 1 ? 0 : v];
+    } else if (stop == g.tiles) {
+        store_floats<V>(a.last + row, carry);
+    }
+}
+
+// The same backwards in time.  AGG: the map of u over each segment.
+template <typename T, int V, bool SHARED, bool AGG>
+__global__ __launch_bounds__(THREADS) void bwd_kernel(Args a) {
+    constexpr int VA = SHARED ? 1 : V, L = max_len<V>();
+    __shared__ float sm[WAVES * 64 * (V + VA)];
+    const Geo& g = a.g;
+    const Place p = place<V>(g);
+    const int64_t seg = blockIdx.z;
+    const int64_t first = seg * g.per_seg, stop = first + g.per_seg < g.tiles ? first + g.per_seg : g.tiles;
+    const int64_t row = p.b * g.D + p.ch;
+    float carry[V], allA[VA];                            // u behind the tile
+    if (AGG) load_floats<V>(carry, nullptr, false);
+    else if (g.segs > 1) load_floats<V>(carry, a.seg_in + (p.b * g.segs + seg) * g.D + p.ch, p.on);
+    else load_floats<V>(carry, a.d_last ? a.d_last + row : nullptr, p.on);
+#pragma unroll
+    for (int v = 0; v < VA; ++v) allA[v] = 1.0f;
+    const int steps = g.tg * g.len;
+    const In gin = {a.d_h, g.T * g.D, g.D};
+    for (int64_t i = stop - 1; i >= first; --i) {
+        const int64_t t0 = i * steps + p.tgi * g.len;
+        Gates<T, V, SHARED> ga;
+        Raw<T, V> va, gr;
+        fetch_gates<T, V, SHARED>(ga, a, p.b, t0, p.ch, p.on);
+        fetch<T, V>(gr, gin, g, a.reverse, p.b, t0, p.ch, p.on && a.d_h, 0.0f);
+        if (!AGG) fetch<T, V>(va, a.value, g, a.reverse, p.b, t0, p.ch, p.on, 0.0f);
+        float A[VA], U[V], u[V];
+#pragma unroll
+        for (int v = 0; v < VA; ++v) A[v] = 1.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) U[v] = 0.0f;
+#pragma unroll
+        for (int j = L - 1; j >= 0; --j) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) U[v] = ga.at(j, v) * ((float)gr.x[j].v[v] + U[v]);
+#pragma unroll
+            for (int v = 0; v < VA; ++v) A[v] *= ga.at(j, v);
+        }
+        if (AGG) {
+            compose<V, VA, true>(g, p, A, U, carry, u, sm);
+#pragma unroll
+            for (int v = 0; v < VA; ++v) allA[v] *= A[v];
+            continue;
+        }
+        float A2[VA], H[V], hs[V], h[V];
+#pragma unroll
+        for (int v = 0; v < VA; ++v) A2[v] = A[v];
+#pragma unroll
+        for (int v = 0; v < V; ++v) H[v] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < L; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) H[v] = fmaf(ga.at(j, v), H[v], (float)va.x[j].v[v]);
+        if (i == 0) load_floats<V>(hs, a.state ? a.state + row : nullptr, p.on);
+        else load_floats<V>(hs, a.states + (p.b * (g.tiles - 1) + i - 1) * g.D + p.ch, p.on);
+        compose<V, VA, true>(g, p, A, U, carry, u, sm);
+        compose<V, VA, false>(g, p, A2, H, hs, h, sm);
+        float G[L][V];
+#pragma unroll
+        for (int j = L - 1; j >= 0; --j) {
+            Pack<T, V> y;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                G[j][v] = (float)gr.x[j].v[v] + u[v];
+                u[v] = ga.at(j, v) * G[j][v];
+                y.v[v] = (T)G[j][v];
+            }
+            const int64_t t = t0 + j;
+            if (a.d_value && p.on && j < g.len && t < g.T)
+                store_pack<T, V>((T*)a.d_value + (p.b * g.T + (a.reverse ? g.T - 1 - t : t)) * g.D + p.ch, y);
+        }
+        if (i == 0 && p.tgi == 0 && p.on && a.d_state) store_floats<V>(a.d_state + row, u);
+        if (!a.d_gate) continue;
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            const int64_t t = t0 + j;
+            const int64_t at = p.b * g.T + (a.reverse ? g.T - 1 - t : t);
+            const bool ok = p.on && j < g.len && t < g.T;
+            if constexpr (SHARED) {
+                float s = 0.0f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) s += p.on ? G[j][v] * h[v] : 0.0f;
+                for (int off = 1; off < (1 << g.cgl); off <<= 1) s += __shfl_xor(s, off, 64);
+                if (ok && p.cg == 0) {
+                    if (g.col_blocks == 1) ((T*)a.d_gate)[at] = (T)s;
+                    else a.gate_part[(int64_t)blockIdx.y * g.B * g.T + at] = s;
+                }
+            } else if (ok) {
+                Pack<T, V> y;
+#pragma unroll
+                for (int v = 0; v < V; ++v) y.v[v] = (T)(G[j][v] * h[v]);
+                store_pack<T, V>((T*)a.d_gate + at * g.D + p.ch, y);
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[v] = fmaf(ga.at(j, v), h[v], (float)va.x[j].v[v]);
+        }
+    }
+    if (AGG && p.on && p.tgi == 0) {
+        const int64_t at = (p.b * g.segs + seg) * g.D + p.ch;
+        store_floats<V>(a.agg_h + at, carry);
+#pragma unroll
+        for (int v = 0; v < V; ++v) a.agg_a[at + v] = allA[VA == 1 ? 0 : v];
+    }
+}
+
+// State in front of every segment (DOWN: u behind it) from the segments' maps: one wave per sequence and channel, a lane
+// per run of consecutive segments.
+template <bool DOWN>
+__global__ __launch_bounds__(THREADS) void segments_kernel(int64_t B, int64_t segs, int D, const float* __restrict__ start,
+                                                           const float* __restrict__ agg_a, const float* __restrict__ agg_h,
+                                                           float* __restrict__ seg_in) {
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+    if (at >= B * D) return;
+    const int64_t b = at / D, d = at % D;
+    const int64_t per = (segs + 63) / 64;
+    const int64_t k0 = lane * per, k1 = k0 + per < segs ? k0 + per : segs;
+    const float *pa = agg_a + b * segs * D + d, *ph = agg_h + b * segs * D + d;
+    float A = 1.0f, H = 0.0f;
+    for (int64_t k = k0; k < k1; ++k) {
+        const int64_t s = (DOWN ? segs - 1 - k : k) * D;
+        const float m = pa[s];
+        H = apply(m, H, ph[s]);
+        A *= m;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const float a2 = __shfl_up(A, off, 64), h2 = __shfl_up(H, off, 64);
+        if (lane >= off) { H = apply(A, h2, H); A *= a2; }
+    }
+    float ea = __shfl_up(A, 1, 64), eh = __shfl_up(H, 1, 64);
+    if (lane == 0) { ea = 1.0f; eh = 0.0f; }
+    float x = apply(ea, start ? start[at] : 0.0f, eh);
+    for (int64_t k = k0; k < k1; ++k) {
+        const int64_t s = (DOWN ? segs - 1 - k : k) * D;
+        seg_in[b * segs * D + d + s] = x;
+        x = apply(pa[s], x, ph[s]);
+    }
+}
+
+// shared gate over more channels than one workgroup holds: the workgroups' sums in order
+template <typename T>
+__global__ __launch_bounds__(THREADS) void gate_join_kernel(int64_t n, int parts, const float* __restrict__ part, T* __restrict__ d_gate) {
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * THREADS) {
+        float s = 0.0f;
+        for (int k = 0; k < parts; ++k) s += part[(int64_t)k * n + i];
+        d_gate[i] = (T)s;
+    }
+}
+
+static inline bool sizes_ok(int64_t B, int64_t T, int64_t D) {
+    return B >= 0 && T >= 0 && D >= 1 && D <= 65536 && B <= ((int64_t)1 << 31) && T <= ((int64_t)1 << 40) && B * D <= ((int64_t)1 << 40) &&
+           (B == 0 || T <= ((int64_t)1 << 46) / (B * D));
+}
+static inline int vec_of(int64_t D, int precision) {
+    const int full = 16 / elem_bytes(precision);
+    return D % full == 0 ? full : 1;
+}
+
+static Geo geometry(int64_t B, int64_t T, int64_t D, int precision) {
+    Geo g = {};
+    g.B = B; g.T = T; g.D = (int)D;
+    const int v = vec_of(D, precision), max_l = v == 8 ? 4 : 8;
+    while (g.cgl < 6 && ((int64_t)v << g.cgl) < D) ++g.cgl;
+    const int units = THREADS >> g.cgl;
+    g.col_blocks = (int)((D + ((int64_t)v << g.cgl) - 1) / ((int64_t)v << g.cgl));
+    g.tg = 1;
+    while (g.tg < units && (int64_t)g.tg * max_l < T) g.tg <<= 1;
+    g.tiles = (T + (int64_t)g.tg * max_l - 1) / ((int64_t)g.tg * max_l);
+    if (g.tiles < 1) g.tiles = 1;
+    g.len = (int)((T + g.tiles * g.tg - 1) / (g.tiles * g.tg));
+    if (g.len < 1) g.len = 1;
+    g.tiles = (T + (int64_t)g.tg * g.len - 1) / ((int64_t)g.tg * g.len);
+    if (g.tiles < 1) g.tiles = 1;
+    g.seqs = units / g.tg;
+    // segments: about four workgroups per compute unit where the sequences alone give fewer than two
+    const int64_t blocks = (B + g.seqs - 1) / g.seqs * g.col_blocks;
+    g.per_seg = g.tiles;
+    if (blocks > 0 && blocks < 512 && g.tiles >= 4) {
+        const int64_t want = (1024 + blocks - 1) / blocks;
+        g.per_seg = (g.tiles + want - 1) / want;
+        if (g.per_seg < 2) g.per_seg = 2;
+    }
+    g.segs = (g.tiles + g.per_seg - 1) / g.per_seg;
+    return g;
+}
+
+struct Workspace { int64_t agg_a, agg_h, seg_in, gate_part, bytes; };
+static Workspace workspace(const Geo& g, bool shared_gate, bool backward) {
+    Workspace w = {};
+    int64_t at = 0;
+    auto take = [&](int64_t floats) {
+        const int64_t here = at;
+        at += (floats * 4 + 255) / 256 * 256;
+        return here;
+    };
+    if (g.segs > 1) {
+        const int64_t n = g.B * g.segs * g.D;
+        w.agg_a = take(n); w.agg_h = take(n); w.seg_in = take(n);
+    }
+    if (backward && shared_gate && g.col_blocks > 1) w.gate_part = take((int64_t)g.col_blocks * g.B * g.T);
+    w.bytes = at < 256 ? 256 : at;
+    return w;
+}
+
+static inline bool input_ok(const void* p, int64_t sb, int64_t st, int vec, int es) {
+    return nerf_aligned(p, (uintptr_t)(vec * es)) && sb % vec == 0 && st % vec == 0;
+}
+
+static int launch(Args& a, const Workspace& w, void* workspace, bool shared, bool backward, int precision, void* stream) {
+    const Geo& g = a.g;
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)workspace;
+    const int64_t seq_blocks = (g.B + g.seqs - 1) / g.seqs;
+    NERF_REQUIRE(seq_blocks < ((int64_t)1 << 31) && g.segs <= 65535, NERF_E_SHAPE);
+    const dim3 grid((unsigned)seq_blocks, (unsigned)g.col_blocks, (unsigned)g.segs), block(THREADS);
+    const int vec = vec_of(g.D, precision);
+    if (g.segs > 1) {
+        a.agg_a = (float*)(ws + w.agg_a); a.agg_h = (float*)(ws + w.agg_h); a.seg_in = (const float*)(ws + w.seg_in);
+    }
+    a.gate_part = (float*)(ws + w.gate_part);
+#define NERF_K(KERN, E, V, S, AGG) hipLaunchKernelGGL((KERN<E, V, S, AGG>), grid, block, 0, st, a)
+#define NERF_VS(KERN, E, AGG)                                                      \
+    do {                                                                           \
+        if (vec > 1 && shared) NERF_K(KERN, E, full_vec<E>(), true, AGG);           \
+        else if (vec > 1) NERF_K(KERN, E, full_vec<E>(), false, AGG);               \
+        else if (shared) NERF_K(KERN, E, 1, true, AGG);                             \
+        else NERF_K(KERN, E, 1, false, AGG);                                        \
+    } while (0)
+#define NERF_CALL(E)                                                                                                      \
+    do {                                                                                                                  \
+        const dim3 gs((unsigned)((g.B * g.D + WAVES - 1) / WAVES));                                                        \
+        if (!backward) {                                                                                                  \
+            if (g.segs > 1) {                                                                                             \
+                NERF_VS(fwd_kernel, E, true);                                                                             \
+                hipLaunchKernelGGL(segments_kernel<false>, gs, block, 0, st, g.B, g.segs, g.D, a.state, a.agg_a, a.agg_h, \
+                                   (float*)a.seg_in);                                                                     \
+            }                                                                                                             \
+            NERF_VS(fwd_kernel, E, false);                                                                                \
+        } else {                                                                                                          \
+            if (g.segs > 1) {                                                                                             \
+                NERF_VS(bwd_kernel, E, true);                                                                             \
+                hipLaunchKernelGGL(segments_kernel<true>, gs, block, 0, st, g.B, g.segs, g.D, a.d_last, a.agg_a, a.agg_h, \
+                                   (float*)a.seg_in);                                                                     \
+            }                                                                                                             \
+            NERF_VS(bwd_kernel, E, false);                                                                                \
+            if (shared && a.d_gate && g.col_blocks > 1) {                                                                             \
+                int64_t jb = (g.B * g.T + THREADS - 1) / THREADS;                                                          \
+                if (jb > 8192) jb = 8192;                                                                                 \
+                hipLaunchKernelGGL(gate_join_kernel<E>, dim3((unsigned)jb), block, 0, st, g.B * g.T, g.col_blocks,         \
+                                   a.gate_part, (E*)a.d_gate);                                                            \
+            }                                                                                                             \
+        }                                                                                                                 \
+    } while (0)
+    NERF_ELEM_DISPATCH(precision, NERF_CALL);
+#undef NERF_CALL
+#undef NERF_VS
+#undef NERF_K
+    return nerf_launch_status();
+}
+
+}  // namespace scan
+}  // namespace nerf
+
+extern "C" int64_t nerf_scan_states_floats(int64_t B, int64_t T, int64_t D, int precision) {
+    if (!nerf::scan::sizes_ok(B, T, D)) return NERF_E_SHAPE;
+    if (!nerf::elem_ok(precision)) return NERF_E_DTYPE;
+    const nerf::scan::Geo g = nerf::scan::geometry(B, T, D, precision);
+    return B * (g.tiles - 1) * D;
+}
+
+extern "C" int64_t nerf_scan_workspace_bytes(int64_t B, int64_t T, int64_t D, int gate_shared, int backward, int precision) {
+    if (!nerf::scan::sizes_ok(B, T, D)) return NERF_E_SHAPE;
+    if (!nerf::elem_ok(precision)) return NERF_E_DTYPE;
+    return nerf::scan::workspace(nerf::scan::geometry(B, T, D, precision), gate_shared != 0, backward != 0).bytes;
+}
+
+extern "C" int nerf_scan_fwd(int64_t B, int64_t T, int64_t D, const void* gate, int64_t gate_sb, int64_t gate_st, int gate_shared,
+                             const void* value, int64_t value_sb, int64_t value_st, const float* state, int reverse, int precision,
+                             void* h, float* last, float* states, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace nerf;
+    NERF_REQUIRE(scan::sizes_ok(B, T, D) && gate_sb >= 0 && gate_st >= 0 && value_sb >= 0 && value_st >= 0, NERF_E_SHAPE);
+    NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
+    if (B == 0 || T == 0) return NERF_OK;
+    NERF_REQUIRE(gate && value && h && last && workspace, NERF_E_NULL);
+    const int vec = scan::vec_of(D, precision), es = elem_bytes(precision);
+    NERF_REQUIRE(scan::input_ok(value, value_sb, value_st, vec, es) && scan::input_ok(gate, gate_sb, gate_st, gate_shared ? 1 : vec, es) &&
+                 nerf_aligned(h, (uintptr_t)(vec * es)) && nerf_aligned(state, 4) && nerf_aligned(last, 4) && nerf_aligned(states, 4) &&
+                 nerf_aligned(workspace, 256), NERF_E_ALIGN);
+    scan::Args a = {};
+    a.g = scan::geometry(B, T, D, precision);
+    const scan::Workspace w = scan::workspace(a.g, gate_shared != 0, false);
+    NERF_REQUIRE(workspace_bytes >= w.bytes, NERF_E_WORKSPACE);
+    a.gate = {gate, gate_sb, gate_st};
+    a.value = {value, value_sb, value_st};
+    a.state = state; a.reverse = reverse ? 1 : 0; a.h = h; a.last = last; a.states = a.g.tiles > 1 ? states : nullptr;
+    return scan::launch(a, w, workspace, gate_shared != 0, false, precision, stream);
+}
+
+extern "C" int nerf_scan_bwd(int64_t B, int64_t T, int64_t D, const void* gate, int64_t gate_sb, int64_t gate_st, int gate_shared,
+                             const void* value, int64_t value_sb, int64_t value_st, const float* state, const float* states,
+                             const void* d_h, const float* d_last, int reverse, int precision, void* d_gate, void* d_value,
+                             float* d_state, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace nerf;
+    NERF_REQUIRE(scan::sizes_ok(B, T, D) && gate_sb >= 0 && gate_st >= 0 && value_sb >= 0 && value_st >= 0, NERF_E_SHAPE);
+    NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
+    if (B == 0 || T == 0) return NERF_OK;
+    scan::Args a = {};
+    a.g = scan::geometry(B, T, D, precision);
+    NERF_REQUIRE(gate && value && workspace && (states || a.g.tiles == 1), NERF_E_NULL);
+    const int vec = scan::vec_of(D, precision), es = elem_bytes(precision);
+    NERF_REQUIRE(scan::input_ok(value, value_sb, value_st, vec, es) && scan::input_ok(gate, gate_sb, gate_st, gate_shared ? 1 : vec, es) &&
+                 nerf_aligned(d_h, (uintptr_t)(vec * es)) && nerf_aligned(d_value, (uintptr_t)(vec * es)) &&
+                 nerf_aligned(d_gate, (uintptr_t)((gate_shared ? 1 : vec) * es)) && nerf_aligned(state, 4) && nerf_aligned(states, 4) &&
+                 nerf_aligned(d_last, 4) && nerf_aligned(d_state, 4) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
+    const scan::Workspace w = scan::workspace(a.g, gate_shared != 0, true);
+    NERF_REQUIRE(workspace_bytes >= w.bytes, NERF_E_WORKSPACE);
+    a.gate = {gate, gate_sb, gate_st};
+    a.value = {value, value_sb, value_st};
+    a.state = state; a.states = (float*)states; a.reverse = reverse ? 1 : 0;
+    a.d_h = d_h; a.d_last = d_last; a.d_gate = d_gate; a.d_value = d_value; a.d_state = d_state;
+    return scan::launch(a, w, workspace, gate_shared != 0, true, precision, stream);
+}

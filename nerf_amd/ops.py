@@ -9,6 +9,7 @@ import ctypes
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _C
 from ._C import check, lib
@@ -708,6 +709,352 @@ def p16_mlp_backward(M: int, cp: int, cv: int, layers, grads, d_raw: torch.Tenso
     with torch.cuda.device(dev), _timed("mlp_bwd_p16", dev, M):
         check(lib.nerf_mlp_p16_bwd(M, cp, cv, lp, gp, len(layers), _C.PREC[precision], _p(d_raw), _p(saved), _p(scale),
                                    _p(work), work.numel(), _stream(dev)), "nerf_mlp_p16_bwd")
+
+
+# ---------------------------------------------------------------------------
+# rows grouped by an id: grouping, rows of a table, linear layers of sub-networks
+# ---------------------------------------------------------------------------
+
+_ELEM = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _gpu_elem(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A bf16 / fp16 / fp32 GPU tensor, of the type and on the device of ``like`` when given."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU (got device {t.device}); nerf_amd has no CPU path")
+    if t.dtype not in _ELEM:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} is {t.dtype}, expected {like.dtype} as the other operands")
+        if t.device != like.device:
+            raise RuntimeError(f"{name} is on {t.device}, the other operands on {like.device}")
+    return t
+
+
+def _gpu_ids(t: torch.Tensor, name: str) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU (got device {t.device}); nerf_amd has no CPU path")
+    if t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+    return t.contiguous()
+
+
+def _row_major(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(tensor, elements between rows) of a 2-D tensor whose rows are contiguous; copied when they are not."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+class RowGroups:
+    """Rows dealt out to groups: what ``group_rows`` and ``row_groups`` return and ``grouped_linear`` takes.
+
+    ``offsets`` [n_groups + 1] int32: positions offsets[g] .. offsets[g+1] - 1 hold the rows of group g.  ``order`` [n] int32:
+    the row at each position (None: the rows are in group order already).  Rows behind offsets[n_groups] belong to no group.
+    All on the GPU; nothing is read back to the host.  Treat the tensors as read-only.
+    """
+    __slots__ = ("order", "offsets", "tile_base", "n_rows", "n_groups")
+
+    def __init__(self, order, offsets, tile_base, n_rows, n_groups):
+        self.order, self.offsets, self.tile_base = order, offsets, tile_base
+        self.n_rows, self.n_groups = n_rows, n_groups
+
+
+_MAX_GROUPED_ROWS = 2 ** 31 - 1 - 128
+_MAX_GROUPS = 2 ** 24
+
+
+def _group_sizes(n: int, n_groups: int) -> None:
+    if not 1 <= n_groups <= _MAX_GROUPS:
+        raise ValueError(f"the number of groups must be between 1 and {_MAX_GROUPS}, got {n_groups}")
+    if n > _MAX_GROUPED_ROWS:
+        raise ValueError(f"at most {_MAX_GROUPED_ROWS} rows, got {n}")
+
+
+def _group(ids: torch.Tensor, n_groups: int, tiles: bool, keys: bool):
+    n, dev = ids.numel(), ids.device
+    _group_sizes(n, n_groups)
+    new = torch.zeros if n == 0 else torch.empty
+    order = torch.empty((n,), dtype=torch.int32, device=dev)
+    offsets = new((n_groups + 1,), dtype=torch.int32, device=dev)
+    base = new((n_groups + 2,), dtype=torch.int32, device=dev) if tiles else None
+    sorted_ids = torch.empty((n,), dtype=torch.int32, device=dev) if keys else None
+    nbytes = int(lib.nerf_group_rows_workspace_bytes(n, n_groups))
+    work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev), _timed("group_rows", dev, n):
+        check(lib.nerf_group_rows(n, _p(ids), ids.element_size(), n_groups, _p(order), _p(offsets), _p(base), _p(sorted_ids),
+                                  _p(work), nbytes, _stream(dev)), "nerf_group_rows")
+    return order, offsets, base, sorted_ids
+
+
+def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
+    """The rows 0 .. n-1 in order of their group ``ids`` [n] (int32 or int64), rows of one group in their own order.
+    An id outside [0, n_groups) belongs to no group; such rows come last."""
+    ids = _gpu_ids(ids, "ids")
+    if ids.dim() != 1:
+        raise ValueError(f"ids must be 1-D, got {tuple(ids.shape)}")
+    n_groups = int(n_groups)
+    order, offsets, base, _ = _group(ids, n_groups, True, False)
+    return RowGroups(order, offsets, base, ids.numel(), n_groups)
+
+
+def row_groups(offsets: torch.Tensor, n_rows: int) -> RowGroups:
+    """Groups of rows that are in group order already: group g is rows offsets[g] .. offsets[g+1] - 1, ``offsets``
+    [n_groups + 1] (int32 or int64).  Values are taken from 0 (offsets[0] counts as 0), never below the one before and
+    never above ``n_rows``."""
+    offsets = _gpu_ids(offsets, "offsets")
+    if offsets.dim() != 1 or offsets.numel() < 2:
+        raise ValueError(f"offsets must be 1-D with one entry more than there are groups, got {tuple(offsets.shape)}")
+    n_rows, n_groups, dev = int(n_rows), offsets.numel() - 1, offsets.device
+    if n_rows < 0:
+        raise ValueError(f"n_rows must not be negative, got {n_rows}")
+    _group_sizes(n_rows, n_groups)
+    given = offsets.clamp(0, n_rows).to(torch.int32)
+    new = torch.zeros if n_rows == 0 else torch.empty
+    clean = new((n_groups + 1,), dtype=torch.int32, device=dev)
+    base = new((n_groups + 2,), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        check(lib.nerf_group_offsets(n_rows, n_groups, _p(given), _p(clean), _p(base), _stream(dev)), "nerf_group_offsets")
+    return RowGroups(None, clean, base, n_rows, n_groups)
+
+
+class _EmbedRows(torch.autograd.Function):
+    """scale * table[ids] and the table's gradient."""
+
+    @staticmethod
+    def forward(ctx, ids, table, scale):
+        n, (rows, dim), dev = ids.numel(), table.shape, table.device
+        table, ld = _row_major(table)
+        out = torch.empty(tuple(ids.shape) + (dim,), dtype=table.dtype, device=dev)
+        with torch.cuda.device(dev), _timed("embed_fwd", dev, n):
+            check(lib.nerf_embed_fwd(n, _p(ids), ids.element_size(), rows, dim, _p(table), ld, scale, _ELEM[table.dtype], _p(out),
+                                     _stream(dev)), "nerf_embed_fwd")
+        ctx.save_for_backward(ids)
+        ctx.sizes, ctx.scale = (rows, dim), scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        (ids,) = ctx.saved_tensors
+        rows, dim = ctx.sizes
+        n, dev = ids.numel(), d_out.device
+        if n == 0:
+            return None, torch.zeros((rows, dim), dtype=d_out.dtype, device=dev), None
+        order, offsets, _, keys = _group(ids.reshape(-1), rows, False, True)
+        g, ld = _row_major(d_out.reshape(n, dim))
+        d_table = torch.empty((rows, dim), dtype=g.dtype, device=dev)
+        nbytes = int(lib.nerf_embed_bwd_workspace_bytes(n, rows, dim))
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev), _timed("embed_bwd", dev, n):
+            check(lib.nerf_embed_bwd(n, rows, dim, _p(order), _p(offsets), _p(keys), _p(g), ld, ctx.scale, _ELEM[g.dtype],
+                                     _p(d_table), _p(work), nbytes, _stream(dev)), "nerf_embed_bwd")
+        return None, d_table, None
+
+
+def embed_rows(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[ids]: ``ids`` of any shape (int32 or int64), ``table`` [rows, dim] in bf16, fp16 or fp32; the result
+    [*ids.shape, dim] has the table's type.  An id outside [0, rows) gives a row of zeros and takes no part in the gradient.
+    Products and the gradient's sums are fp32, rounded once; the gradient is bitwise reproducible."""
+    ids = _gpu_ids(ids, "ids")
+    table = _gpu_elem(table, "table")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"table must be [rows, dim] with at least one row and column, got {tuple(table.shape)}")
+    if ids.device != table.device:
+        raise RuntimeError(f"ids are on {ids.device}, the table on {table.device}")
+    if isinstance(scale, torch.Tensor):
+        raise TypeError("scale must be a number")
+    if table.shape[1] > 2 ** 20:
+        raise ValueError(f"at most {2 ** 20} columns, got {table.shape[1]}")
+    _group_sizes(ids.numel(), table.shape[0])
+    return _EmbedRows.apply(ids, table, float(scale))
+
+
+class _GroupedLinear(torch.autograd.Function):
+    """act(W[group] x + b[group]) for rows dealt out to groups, and its three gradients."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, relu):
+        n, dev = groups.n_rows, x.device
+        G, N, K = weight.shape
+        xr, ld = _row_major(x)
+        weight = weight.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        y = torch.empty((n, N), dtype=x.dtype, device=dev)
+        with torch.cuda.device(dev), _timed("grouped_fwd", dev, n):
+            check(lib.nerf_grouped_fwd(n, G, _p(groups.order), _p(groups.offsets), _p(groups.tile_base), K, N, _p(xr), ld, _p(weight),
+                                       _p(bias), int(relu), _ELEM[x.dtype], _p(y), _stream(dev)), "nerf_grouped_fwd")
+        ctx.save_for_backward(xr, weight, y if relu else None)
+        ctx.groups, ctx.has_bias = groups, bias is not None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_y):
+        x, weight, y = ctx.saved_tensors
+        groups, dev = ctx.groups, d_y.device
+        n, (G, N, K), prec = groups.n_rows, weight.shape, _ELEM[d_y.dtype]
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        if n == 0:
+            return (torch.zeros((0, K), dtype=d_y.dtype, device=dev) if need_x else None, torch.zeros_like(weight) if need_w else None,
+                    torch.zeros((G, N), dtype=d_y.dtype, device=dev) if need_b else None, None, None)
+        g, ld = _row_major(d_y)
+        at = (n, G, _p(groups.order), _p(groups.offsets), _p(groups.tile_base), K, N, _p(g), ld, _p(y))
+        with torch.cuda.device(dev):
+            if need_x:
+                dx = torch.empty((n, K), dtype=g.dtype, device=dev)
+                with _timed("grouped_bwd_data", dev, n):
+                    check(lib.nerf_grouped_bwd_data(*at, _p(weight), prec, _p(dx), _stream(dev)), "nerf_grouped_bwd_data")
+            if need_w or need_b:
+                dw = torch.empty_like(weight)
+                db = torch.empty((G, N), dtype=g.dtype, device=dev) if need_b else None
+                xr, x_ld = _row_major(x)
+                nbytes = int(lib.nerf_grouped_bwd_weights_workspace_bytes(n, G, K, N))
+                work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+                with _timed("grouped_bwd_weights", dev, n):
+                    check(lib.nerf_grouped_bwd_weights(*at, _p(xr), x_ld, prec, _p(dw), _p(db), _p(work), nbytes, _stream(dev)),
+                          "nerf_grouped_bwd_weights")
+        return dx, dw if need_w else None, db, None, None
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bias: Optional[torch.Tensor] = None,
+                   relu: bool = False) -> torch.Tensor:
+    """One linear layer of many sub-networks: row i of ``x`` [..., K] times the weights of its group, ``weight`` [G, N, K]
+    (each [N, K] as ``torch.nn.Linear`` keeps it), plus ``bias`` [G, N], through a ReLU when ``relu``.  ``groups`` (of
+    ``group_rows`` or ``row_groups``) says which row belongs where; x and the result [..., N] stay in their own row order.
+    Rows of no group give zeros.  x, weight and bias share one of bf16, fp16, fp32; products are summed in fp32 and rounded
+    once.  Gradients flow to x, weight and bias, and are bitwise reproducible."""
+    if not isinstance(groups, RowGroups):
+        raise TypeError(f"groups must come from group_rows or row_groups, got {type(groups).__name__}")
+    x = _gpu_elem(x, "x")
+    weight = _gpu_elem(weight, "weight", x)
+    if weight.dim() != 3 or min(weight.shape) < 1:
+        raise ValueError(f"weight must be [groups, out_features, in_features], got {tuple(weight.shape)}")
+    G, N, K = weight.shape
+    if G != groups.n_groups:
+        raise ValueError(f"weight holds {G} groups, the rows are dealt out to {groups.n_groups}")
+    if G > 65535 or N > 65536 or K > 65536:
+        raise ValueError(f"at most 65535 groups and 65536 features, got {tuple(weight.shape)}")
+    if x.dim() < 2 or x.shape[-1] != K:
+        raise ValueError(f"x must be [..., {K}], got {tuple(x.shape)}")
+    if x.numel() // K != groups.n_rows:
+        raise ValueError(f"x has {x.numel() // K} rows, the groups were made of {groups.n_rows}")
+    if groups.offsets.device != x.device:
+        raise RuntimeError(f"the groups are on {groups.offsets.device}, the operands on {x.device}")
+    if bias is not None:
+        bias = _gpu_elem(bias, "bias", x)
+        if tuple(bias.shape) != (G, N):
+            raise ValueError(f"bias must be [{G}, {N}], got {tuple(bias.shape)}")
+    y = _GroupedLinear.apply(x.reshape(-1, K), weight, bias, groups, bool(relu))
+    return y.view(tuple(x.shape[:-1]) + (N,))
+
+
+# ---------------------------------------------------------------------------
+# gated linear recurrence along a ray
+# ---------------------------------------------------------------------------
+
+def _scan_input(t: torch.Tensor, vec: int) -> Tuple[torch.Tensor, int, int]:
+    """(tensor, elements between sequences, between samples) as the kernels read it: channels contiguous, pieces of ``vec``
+    elements aligned; copied when it is not."""
+    def strides(u):
+        return tuple(u.stride(i) if u.shape[i] > 1 else 0 for i in (0, 1))
+    sb, st = strides(t)
+    if t.shape[2] > 1 and t.stride(2) != 1 or sb % vec or st % vec or t.data_ptr() % (vec * t.element_size()):
+        t = t.clone(memory_format=torch.contiguous_format)
+        sb, st = strides(t)
+    return t, sb, st
+
+
+class _GatedScan(torch.autograd.Function):
+    """h[t] = gate[t] h[t-1] + value[t] and its gradients."""
+
+    @staticmethod
+    def forward(ctx, gate, value, state, reverse):
+        (B, T, D), dev, prec = value.shape, value.device, _ELEM[value.dtype]
+        full = 16 // value.element_size()
+        shared = gate.shape[2] == 1 and D > 1
+        vec = full if D % full == 0 else 1
+        va, vsb, vst = _scan_input(value, vec)
+        ga, gsb, gst = _scan_input(gate, 1 if shared else vec)
+        st = None if state is None else state.contiguous()
+        h = torch.empty((B, T, D), dtype=value.dtype, device=dev)
+        last = torch.empty((B, D), dtype=torch.float32, device=dev)
+        need = any(ctx.needs_input_grad[:3])
+        states = torch.empty((int(lib.nerf_scan_states_floats(B, T, D, prec)),), dtype=torch.float32, device=dev) if need else None
+        nbytes = int(lib.nerf_scan_workspace_bytes(B, T, D, int(shared), 0, prec))
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev), _timed("scan_fwd", dev, B * T):
+            check(lib.nerf_scan_fwd(B, T, D, _p(ga), gsb, gst, int(shared), _p(va), vsb, vst, _p(st), int(reverse), prec, _p(h), _p(last),
+                                    _p(states), _p(work), nbytes, _stream(dev)), "nerf_scan_fwd")
+        ctx.save_for_backward(ga, va, st, states)
+        ctx.how = (shared, vec, bool(reverse))
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_h, d_last):
+        if d_h is None and d_last is None:
+            return None, None, None, None
+        gate, value, state, states = ctx.saved_tensors
+        shared, vec, reverse = ctx.how
+        (B, T, D), dev, prec = value.shape, value.device, _ELEM[value.dtype]
+        need_gate, need_value, need_state = ctx.needs_input_grad[:3]
+        ga, gsb, gst = _scan_input(gate, 1 if shared else vec)
+        va, vsb, vst = _scan_input(value, vec)
+        if d_h is not None:
+            d_h = d_h.contiguous()
+            if d_h.data_ptr() % (vec * d_h.element_size()):
+                d_h = d_h.clone()
+        d_last = None if d_last is None else _gpu_f32(d_last, "d_last")
+        d_gate = torch.empty((B, T, 1 if shared else D), dtype=value.dtype, device=dev) if need_gate else None
+        d_value = torch.empty((B, T, D), dtype=value.dtype, device=dev) if need_value else None
+        d_state = torch.empty((B, D), dtype=torch.float32, device=dev) if need_state else None
+        nbytes = int(lib.nerf_scan_workspace_bytes(B, T, D, int(shared), 1, prec))
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev), _timed("scan_bwd", dev, B * T):
+            check(lib.nerf_scan_bwd(B, T, D, _p(ga), gsb, gst, int(shared), _p(va), vsb, vst, _p(state), _p(states), _p(d_h), _p(d_last),
+                                    int(reverse), prec, _p(d_gate), _p(d_value), _p(d_state), _p(work), nbytes, _stream(dev)),
+                  "nerf_scan_bwd")
+        return d_gate, d_value, d_state, None
+
+
+def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: Optional[torch.Tensor] = None,
+               reverse: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """h[:, t] = gate[:, t] * h[:, t-1] + value[:, t] along the samples of each ray, from ``state`` (zeros when None):
+    ``value`` [B, T, D]; ``gate`` [B, T, D], or [B, T, 1] for one gate per sample; size-1 batch and sample axes of the gate are
+    expanded.  ``reverse`` runs from the last sample to the first.  Returns (h [B, T, D] in the value's type, the state behind
+    the last step [B, D] in fp32), so that ``gated_scan(..., state=last)`` goes on with the next samples.
+
+    gate and value share one of bf16, fp16, fp32; ``state`` is fp32.  States are fp32 throughout, also in the backward pass,
+    which recomputes them.  Time is cut into pieces that are composed, so the product of consecutive gates has to stay in the
+    range of fp32 wherever the state in front of them is not zero."""
+    value = _gpu_elem(value, "value")
+    gate = _gpu_elem(gate, "gate", value)
+    if value.dim() != 3 or not 1 <= value.shape[2] <= 65536:
+        raise ValueError(f"value must be [sequences, samples, channels] with 1 to 65536 channels, got {tuple(value.shape)}")
+    B, T, D = value.shape
+    if gate.dim() != 3 or gate.shape[2] not in (1, D) or gate.shape[0] not in (1, B) or gate.shape[1] not in (1, T):
+        raise ValueError(f"gate must be [{B}, {T}, {D}] or [{B}, {T}, 1], got {tuple(gate.shape)}")
+    if state is not None:
+        if not isinstance(state, torch.Tensor):
+            raise TypeError(f"state must be a torch.Tensor, got {type(state).__name__}")
+        if state.device != value.device:
+            raise RuntimeError(f"state is on {state.device}, the other operands on {value.device}")
+        if state.dtype != torch.float32:
+            raise TypeError(f"state must be float32, got {state.dtype}")
+        if tuple(state.shape) != (B, D):
+            raise ValueError(f"state must be [{B}, {D}], got {tuple(state.shape)}")
+    if B == 0 or T == 0:
+        last = value.new_zeros((B, D), dtype=torch.float32) if state is None else state.clone()
+        return value.clone(), last
+    return _GatedScan.apply(gate.expand(B, T, gate.shape[2]), value, state, bool(reverse))
 
 
 # ---------------------------------------------------------------------------
