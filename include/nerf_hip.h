@@ -376,14 +376,13 @@ int nerf_mlp_bwd_weights(int64_t M, const void *packed, const void *saved, const
  * Grouping.  ids [n] of id_bytes 4 (int32) or 8 (int64).  order [n]: the rows 0 .. n-1 sorted by id, rows of one id in
  * their own order; offsets [n_groups + 1]: group g is order[offsets[g]] .. order[offsets[g+1] - 1].  An id outside
  * [0, n_groups) belongs to no group; such rows come last.  tile_base (nullable) [n_groups + 2]: the number of 128-row
- * tiles of the groups before each (the rows of no group count as one more group), as nerf_grouped_* read it.  keys
- * (nullable) [n]: the sorted ids, n_groups for rows of no group, as nerf_embed_bwd reads them.  workspace:
+ * tiles of the groups before each (the rows of no group count as one more group), as nerf_grouped_* read it.  workspace:
  * nerf_group_rows_workspace_bytes bytes, 256-byte aligned.  n = 0 writes nothing.  Limits: n <= 2^31 - 129,
  * 1 <= n_groups <= 2^24.
  */
 int64_t nerf_group_rows_workspace_bytes(int64_t n, int64_t n_groups);
 int nerf_group_rows(int64_t n, const void *ids, int id_bytes, int64_t n_groups, int32_t *order, int32_t *offsets,
-                    int32_t *tile_base, int32_t *keys, void *workspace, int64_t workspace_bytes, void *stream);
+                    int32_t *tile_base, void *workspace, int64_t workspace_bytes, void *stream);
 /* Rows that are in group order already: offsets_in [n_groups + 1] made safe to index with (offsets[0] = 0, never below
  * the one before, never above n), and their tile_base.  offsets must not alias offsets_in. */
 int nerf_group_offsets(int64_t n, int64_t n_groups, const int32_t *offsets_in, int32_t *offsets, int32_t *tile_base,
@@ -392,12 +391,11 @@ int nerf_group_offsets(int64_t n, int64_t n_groups, const int32_t *offsets_in, i
 /* out [n, dim] = scale * table[ids], an id outside [0, rows) gives zeros; table rows are table_ld elements apart. */
 int nerf_embed_fwd(int64_t n, const void *ids, int id_bytes, int64_t rows, int64_t dim, const void *table, int64_t table_ld,
                    float scale, int precision, void *out, void *stream);
-/* d_table [rows, dim] (written, not accumulated) = scale * the sum of d_out's rows by id, from order, offsets and keys of
- * nerf_group_rows(ids, rows).  fp32 sums in a fixed order, no atomics.  dim <= 2^20. */
+/* d_table [rows, dim] (written, not accumulated) = scale * the sum of d_out's rows by id.  fp32 sums in a fixed order (the
+ * rows are grouped by id first), no atomics.  dim <= 2^20; rows, n as for nerf_group_rows; workspace 256-byte aligned. */
 int64_t nerf_embed_bwd_workspace_bytes(int64_t n, int64_t rows, int64_t dim);
-int nerf_embed_bwd(int64_t n, int64_t rows, int64_t dim, const int32_t *order, const int32_t *offsets, const int32_t *keys,
-                   const void *d_out, int64_t d_out_ld, float scale, int precision, void *d_table, void *workspace,
-                   int64_t workspace_bytes, void *stream);
+int nerf_embed_bwd(int64_t n, const void *ids, int id_bytes, int64_t rows, int64_t dim, const void *d_out, int64_t d_out_ld,
+                   float scale, int precision, void *d_table, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Linear layers of n_groups sub-networks, weight [n_groups, N, K], bias (nullable) [n_groups, N]:
  *   y[i] = act(weight[g(i)] x[i] + bias[g(i)]), act = ReLU when relu (keeps a NaN), zeros for rows of no group.

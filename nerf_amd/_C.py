@@ -68,11 +68,11 @@ _SIGS = {
     "nerf_adam_step_dev": (c_int, [c_int64, P, P, P, P, P, P]),
     "nerf_mse_pair": (c_int, [c_int64, P, P, P, P, P, P, P]),
     "nerf_group_rows_workspace_bytes": (c_int64, [c_int64, c_int64]),
-    "nerf_group_rows": (c_int, [c_int64, P, c_int, c_int64, P, P, P, P, P, c_int64, P]),
+    "nerf_group_rows": (c_int, [c_int64, P, c_int, c_int64, P, P, P, P, c_int64, P]),
     "nerf_group_offsets": (c_int, [c_int64, c_int64, P, P, P, P]),
     "nerf_embed_fwd": (c_int, [c_int64, P, c_int, c_int64, c_int64, P, c_int64, c_float, c_int, P, P]),
     "nerf_embed_bwd_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
-    "nerf_embed_bwd": (c_int, [c_int64, c_int64, c_int64, P, P, P, P, c_int64, c_float, c_int, P, P, c_int64, P]),
+    "nerf_embed_bwd": (c_int, [c_int64, P, c_int, c_int64, c_int64, P, c_int64, c_float, c_int, P, P, c_int64, P]),
     "nerf_grouped_fwd": (c_int, [c_int64, c_int64, P, P, P, c_int, c_int, P, c_int64, P, P, c_int, c_int, P, P]),
     "nerf_grouped_bwd_data": (c_int, [c_int64, c_int64, P, P, P, c_int, c_int, P, c_int64, P, P, c_int, P, P]),
     "nerf_grouped_bwd_weights_workspace_bytes": (c_int64, [c_int64, c_int64, c_int, c_int]),

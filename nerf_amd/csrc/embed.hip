@@ -316,30 +316,59 @@ extern "C" int nerf_embed_fwd(int64_t n, const void* ids, int id_bytes, int64_t 
     return nerf_launch_status();
 }
 
-extern "C" int64_t nerf_embed_bwd_workspace_bytes(int64_t n, int64_t rows, int64_t dim) {
-    using namespace nerf;
-    if (!emb::sizes_ok(n, rows, dim)) return NERF_E_SHAPE;
-    int64_t most = 0;                       // over the two access widths, which the pointers decide
+namespace nerf {
+namespace emb {
+
+struct BwdPlan { int64_t order, offsets, keys, part, group, bytes; };     // byte offsets in the workspace
+static BwdPlan bwd_plan(int64_t n, int64_t rows, int64_t dim) {
+    BwdPlan p = {};
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    int64_t part = 0;                       // over the access widths, which the pointers decide
     for (int vec : {1, 4, 8}) {
-        const int groups = emb::THREADS / emb::lanes_per_row(dim, vec);
-        const int64_t span = (int64_t)groups * emb::positions_per_group(n, groups);
+        const int groups = THREADS / lanes_per_row(dim, vec);
+        const int64_t span = (int64_t)groups * positions_per_group(n, groups);
         const int64_t b = 2 * ((n + span - 1) / span) * dim * 4;
-        if (b > most) most = b;
+        if (b > part) part = b;
     }
-    return most < 256 ? 256 : most;
+    p.order = take(4 * n);
+    p.offsets = take(4 * (rows + 1));
+    p.keys = take(4 * n);
+    p.part = take(part);
+    p.group = take(grp::workspace_bytes(n, rows));
+    p.bytes = at;
+    return p;
 }
 
-extern "C" int nerf_embed_bwd(int64_t n, int64_t rows, int64_t dim, const int32_t* order, const int32_t* offsets, const int32_t* keys,
-                              const void* d_out, int64_t d_out_ld, float scale, int precision, void* d_table, void* workspace,
-                              int64_t workspace_bytes, void* stream) {
+}  // namespace emb
+}  // namespace nerf
+
+extern "C" int64_t nerf_embed_bwd_workspace_bytes(int64_t n, int64_t rows, int64_t dim) {
+    if (!nerf::emb::sizes_ok(n, rows, dim)) return NERF_E_SHAPE;
+    return nerf::emb::bwd_plan(n, rows, dim).bytes;
+}
+
+extern "C" int nerf_embed_bwd(int64_t n, const void* ids, int id_bytes, int64_t rows, int64_t dim, const void* d_out, int64_t d_out_ld,
+                              float scale, int precision, void* d_table, void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace nerf;
     NERF_REQUIRE(emb::sizes_ok(n, rows, dim) && d_out_ld >= dim, NERF_E_SHAPE);
-    NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
+    NERF_REQUIRE(elem_ok(precision) && (id_bytes == 4 || id_bytes == 8), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(order && offsets && keys && d_out && d_table && workspace, NERF_E_NULL);
+    NERF_REQUIRE(ids && d_out && d_table && workspace, NERF_E_NULL);
     const int es = elem_bytes(precision), full = 16 / es;
-    NERF_REQUIRE(nerf_aligned(d_out, (uintptr_t)es) && nerf_aligned(d_table, (uintptr_t)es) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
-    NERF_REQUIRE(workspace_bytes >= nerf_embed_bwd_workspace_bytes(n, rows, dim), NERF_E_WORKSPACE);
+    NERF_REQUIRE(nerf_aligned(ids, (uintptr_t)id_bytes) && nerf_aligned(d_out, (uintptr_t)es) && nerf_aligned(d_table, (uintptr_t)es) &&
+                 nerf_aligned(workspace, 256), NERF_E_ALIGN);
+    const emb::BwdPlan plan = emb::bwd_plan(n, rows, dim);
+    NERF_REQUIRE(workspace_bytes >= plan.bytes, NERF_E_WORKSPACE);
+    char* ws = (char*)workspace;
+    hipStream_t st = (hipStream_t)stream;
+    int32_t *order = (int32_t*)(ws + plan.order), *offsets = (int32_t*)(ws + plan.offsets), *keys = (int32_t*)(ws + plan.keys);
+    const int rc = grp::launch_group_rows(n, ids, id_bytes, rows, order, offsets, nullptr, keys, ws + plan.group, st);
+    if (rc != NERF_OK) return rc;
     const bool wide = dim % full == 0 && d_out_ld % full == 0 && nerf_aligned(d_out, 16) && nerf_aligned(d_table, 16);
     const int vec = wide ? full : 1;
     emb::BwdArgs a = {};
@@ -347,11 +376,10 @@ extern "C" int nerf_embed_bwd(int64_t n, int64_t rows, int64_t dim, const int32_
     a.lpr = emb::lanes_per_row(dim, vec);
     const int groups = emb::THREADS / a.lpr;
     a.per = emb::positions_per_group(n, groups);
-    a.order = order; a.offsets = offsets; a.keys = keys; a.scale = scale; a.part = (float*)workspace;
+    a.order = order; a.offsets = offsets; a.keys = keys; a.scale = scale; a.part = (float*)(ws + plan.part);
     const int64_t span = (int64_t)groups * a.per;
     const unsigned cols = (unsigned)((dim + (int64_t)a.lpr * vec - 1) / ((int64_t)a.lpr * vec));
     const dim3 g1((unsigned)((n + span - 1) / span), cols), g2((unsigned)((rows + groups - 1) / groups), cols), block(emb::THREADS);
-    hipStream_t st = (hipStream_t)stream;
 #define NERF_BWD(T, V)                                                                                                        \
     do {                                                                                                                      \
         hipLaunchKernelGGL((emb::bwd_sum_kernel<T, V>), g1, block, 0, st, a, (const T*)d_out, d_out_ld, (T*)d_table);          \

@@ -2,15 +2,16 @@
 // group begins, and how many 128-row tiles the groups before it hold.  The reference has no sub-networks; this is what
 // hands sample points to them (nerf_grouped_linear) and what the gradient of a row look-up sums by (nerf_embed_bwd).
 //
-// An LSD radix sort of (id, position) in digits of at most 8 bits; ids outside [0, n_groups) take the key n_groups and
-// come last.  For a digit every wave owns a run of consecutive positions and counts its digits in LDS; an exclusive
-// sum over (digit, wave) gives each wave its first place per digit, and within a wave the lanes of one 64-element
-// round that hold the same digit find each other with one ballot per bit, so equal digits keep their order.  Only
-// integers are added, so the result does not depend on timing.
+// An LSD radix sort of (id, position); ids outside [0, n_groups) take the key n_groups and come last.  For a digit every
+// wave owns a run of consecutive positions.  The lanes of one 64-element round that hold the same digit find each other
+// with one ballot per bit, so equal digits keep their order and a digit's count is one LDS addition however many lanes
+// hold it (the samples of a ray share an id).  An exclusive sum over (digit, wave) gives each wave its first place per
+// digit.  Only integers are added, so the result does not depend on timing.
 //
-// Up to SMALL_N rows one workgroup keeps everything in LDS (one launch).  Above, three launches per digit: counts per
-// 4096-row block, an exclusive sum per digit over the blocks, and the ranked scatter.  Bound by memory: 786 432 int64
-// ids over 64 groups (one digit) read the ids twice and write the order once.
+// Up to SMALL_N rows one workgroup keeps everything in LDS (one launch, digits of at most 8 bits).  Above, three launches
+// per digit of at most 11 bits: counts per block of rows, an exclusive sum per digit over the blocks, and the ranked
+// scatter.  A wide digit costs more counters per block (8 KiB per wave at 11 bits) but saves a whole pass: ids of 256 to
+// 2047 groups take one, of up to four million two.
 #include "groups.hpp"
 
 namespace nerf {
@@ -19,8 +20,10 @@ namespace grp {
 constexpr int SMALL_N = 4096;      // rows one workgroup sorts in LDS
 constexpr int SMALL_THREADS = 1024;
 constexpr int BLOCK_THREADS = 256;
-constexpr int BLOCK_ROUNDS = 16;
-constexpr int BLOCK_ROWS = BLOCK_THREADS * BLOCK_ROUNDS;
+constexpr int MAX_BITS = 11;        // of a digit above SMALL_N rows
+// rows a thread takes: few below a million rows, where the blocks would not fill the chip otherwise
+constexpr int FEW_ROUNDS = 4, MANY_ROUNDS = 16;
+constexpr int64_t MANY_ROWS = (int64_t)1 << 20;
 
 template <typename ID>
 __device__ __forceinline__ unsigned key_of(const ID* ids, int64_t i, unsigned n_groups) {
@@ -169,26 +172,29 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(int n, const ID* _
     }
 }
 
-// digit counts of each block of BLOCK_ROWS rows: hist[digit][block]
-template <typename ID>
+// digit counts of each block of ROUNDS * BLOCK_THREADS rows: hist[digit][block]
+template <typename ID, int ROUNDS>
 __global__ __launch_bounds__(BLOCK_THREADS) void hist_kernel(int64_t n, const ID* __restrict__ ids, unsigned n_groups, int shift,
                                                              int bits, int nblk, int32_t* __restrict__ hist) {
-    __shared__ int cnt[256];
-    const int tid = threadIdx.x;
-    cnt[tid] = 0;
-    __syncthreads();
-    const int64_t p0 = (int64_t)blockIdx.x * BLOCK_ROWS;
-    unsigned k[BLOCK_ROUNDS];
+    extern __shared__ int cnt[];                                   // [1 << bits]
+    const int tid = threadIdx.x, lane = tid & 63, bins = 1 << bits;
+    const int64_t p0 = (int64_t)blockIdx.x * (ROUNDS * BLOCK_THREADS) + tid;
+    unsigned k[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < BLOCK_ROUNDS; ++r) {
-        const int64_t p = p0 + r * BLOCK_THREADS + tid;
-        k[r] = p < n ? (key_of(ids, p, n_groups) >> shift) & ((1u << bits) - 1u) : 256u;
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int64_t p = p0 + r * BLOCK_THREADS;
+        k[r] = p < n ? (key_of(ids, p, n_groups) >> shift) & (unsigned)(bins - 1) : 0u;
     }
-#pragma unroll
-    for (int r = 0; r < BLOCK_ROUNDS; ++r)
-        if (k[r] < 256u) atomicAdd(&cnt[k[r]], 1);
+    for (int d = tid; d < bins; d += BLOCK_THREADS) cnt[d] = 0;
     __syncthreads();
-    if (tid < (1 << bits)) hist[(int64_t)tid * nblk + blockIdx.x] = cnt[tid];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const bool ok = p0 + r * BLOCK_THREADS < n;
+        const unsigned long long peers = same_digit(k[r], bits, __ballot(ok));
+        if (ok && (peers >> lane) == 1ull) atomicAdd(&cnt[k[r]], __popcll(peers));
+    }
+    __syncthreads();
+    for (int d = tid; d < bins; d += BLOCK_THREADS) hist[(int64_t)d * nblk + blockIdx.x] = cnt[d];
 }
 
 // one block per digit: exclusive sum of its counts over the blocks, in place; the digit's total behind them
@@ -209,54 +215,72 @@ __global__ __launch_bounds__(BLOCK_THREADS) void rowscan_kernel(int nblk, int32_
 
 // ranked scatter of one digit.  idx_in: the positions that belong to the keys (NULL in the first pass: the row itself).
 // offsets / tile_base are written by block 0 when `single` (the digit is the whole key).
-template <typename ID>
+template <typename ID, int ROUNDS>
 __global__ __launch_bounds__(BLOCK_THREADS) void scatter_kernel(int64_t n, const ID* __restrict__ ids, const int32_t* __restrict__ idx_in,
                                                                 unsigned n_groups, int shift, int bits, int nblk,
                                                                 const int32_t* __restrict__ hist, const int32_t* __restrict__ totals,
                                                                 int32_t* __restrict__ key_out, int32_t* __restrict__ idx_out, int single,
                                                                 int32_t* __restrict__ offsets, int32_t* __restrict__ tile_base) {
     constexpr int WAVES = BLOCK_THREADS / 64;
-    __shared__ int cnt[WAVES][256];
-    __shared__ int offs[257];
+    constexpr int PER = (1 << MAX_BITS) / BLOCK_THREADS;           // digits of a thread in the exclusive sum, at most
+    extern __shared__ int cnt[];                                   // [WAVES][1 << bits], then [1 << bits] first places
     __shared__ int part[WAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const unsigned mask = (1u << bits) - 1u;
-    const int64_t p0 = (int64_t)blockIdx.x * BLOCK_ROWS + wave * (BLOCK_ROUNDS * 64) + lane;
-    unsigned k[BLOCK_ROUNDS];
-    int at[BLOCK_ROUNDS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = 1 << bits;
+    int* mine = cnt + wave * bins;
+    int* offs = cnt + WAVES * bins;
+    const int64_t p0 = (int64_t)blockIdx.x * (ROUNDS * BLOCK_THREADS) + wave * (ROUNDS * 64) + lane;
+    unsigned k[ROUNDS];
+    int at[ROUNDS];
+    unsigned long long peers[ROUNDS];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) cnt[w][tid] = 0;
-#pragma unroll
-    for (int r = 0; r < BLOCK_ROUNDS; ++r) {
+    for (int r = 0; r < ROUNDS; ++r) {
         const int64_t p = p0 + r * 64;
         k[r] = p < n ? key_of(ids, p, n_groups) : 0u;
         at[r] = p < n ? (idx_in ? idx_in[p] : (int)p) : 0;
     }
-    const int total = tid <= (int)mask ? totals[tid] : 0;
-    const int before = tid <= (int)mask ? hist[(int64_t)tid * nblk + blockIdx.x] : 0;
+    const int per = bins > BLOCK_THREADS ? bins / BLOCK_THREADS : 1;
+    int total[PER], before[PER], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int d = tid * per + j;
+        const bool on = j < per && d < bins;
+        total[j] = on ? totals[d] : 0;
+        before[j] = on ? hist[(int64_t)d * nblk + blockIdx.x] : 0;
+        sum += total[j];
+    }
+    for (int i = tid; i < WAVES * bins; i += BLOCK_THREADS) cnt[i] = 0;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < BLOCK_ROUNDS; ++r)
-        if (p0 + r * 64 < n) atomicAdd(&cnt[wave][(k[r] >> shift) & mask], 1);
-    int all;
-    const int first = block_excl_add<WAVES>(total, part, &all);      // (its barriers also publish the counts)
-    int run = first + before;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) { const int c = cnt[w][tid]; cnt[w][tid] = run; run += c; }
-    offs[tid] = first;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < BLOCK_ROUNDS; ++r) {
+    for (int r = 0; r < ROUNDS; ++r) {
         const bool ok = p0 + r * 64 < n;
-        const unsigned dig = (k[r] >> shift) & mask;
-        const unsigned long long peers = same_digit(dig, bits, __ballot(ok));
+        const unsigned dig = (k[r] >> shift) & (unsigned)(bins - 1);
+        peers[r] = same_digit(dig, bits, __ballot(ok));
+        if (ok && (peers[r] >> lane) == 1ull) atomicAdd(&mine[dig], __popcll(peers[r]));
+    }
+    int all;
+    int first = block_excl_add<WAVES>(sum, part, &all);            // (its barriers also publish the counts)
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int d = tid * per + j;
+        if (j >= per || d >= bins) continue;
+        offs[d] = first;
+        int run = first + before[j];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) { const int c = cnt[w * bins + d]; cnt[w * bins + d] = run; run += c; }
+        first += total[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const bool ok = p0 + r * 64 < n;
+        const unsigned dig = (k[r] >> shift) & (unsigned)(bins - 1);
         if (ok) {
-            const int to = cnt[wave][dig] + __popcll(peers & ((1ull << lane) - 1ull));
+            const int to = mine[dig] + __popcll(peers[r] & ((1ull << lane) - 1ull));
             idx_out[to] = at[r];
             if (key_out) key_out[to] = (int32_t)k[r];
         }
         wave_lds_sync();
-        if (ok && (peers >> lane) == 1ull) cnt[wave][dig] += __popcll(peers);
+        if (ok && (peers[r] >> lane) == 1ull) mine[dig] += __popcll(peers[r]);
         wave_lds_sync();
     }
     if (single && blockIdx.x == 0) {
@@ -316,6 +340,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void clean_offsets_kernel(int n, int
 
 struct Plan {
     int passes, bits;      // digits and bits per digit
+    int rounds;
     int64_t nblk;
     int64_t hist, totals, ka, ia, kb, ib, kout, bytes;     // byte offsets in the workspace
 };
@@ -324,9 +349,11 @@ static Plan plan_for(int64_t n, int64_t n_groups) {
     Plan p = {};
     int b = 1;
     while (b < 31 && (((int64_t)1 << b) <= n_groups)) ++b;      // keys 0 .. n_groups
-    p.passes = (b + 7) / 8;
+    const int most = n <= SMALL_N ? 8 : MAX_BITS;
+    p.passes = (b + most - 1) / most;
     p.bits = (b + p.passes - 1) / p.passes;
-    p.nblk = (n + BLOCK_ROWS - 1) / BLOCK_ROWS;
+    p.rounds = n < MANY_ROWS ? FEW_ROUNDS : MANY_ROUNDS;
+    p.nblk = (n + p.rounds * BLOCK_THREADS - 1) / (p.rounds * BLOCK_THREADS);
     int64_t at = 0;
     auto take = [&](int64_t ints) {
         const int64_t here = at;
@@ -335,7 +362,7 @@ static Plan plan_for(int64_t n, int64_t n_groups) {
     };
     if (n > SMALL_N) {
         p.hist = take(((int64_t)1 << p.bits) * p.nblk);
-        p.totals = take(256);
+        p.totals = take((int64_t)1 << p.bits);
         if (p.passes > 1) { p.ka = take(n); p.ia = take(n); }
         if (p.passes > 2) { p.kb = take(n); p.ib = take(n); }
     }
@@ -356,17 +383,11 @@ extern "C" int64_t nerf_group_rows_workspace_bytes(int64_t n, int64_t n_groups) 
     return nerf::grp::plan_for(n, n_groups).bytes;
 }
 
-extern "C" int nerf_group_rows(int64_t n, const void* ids, int id_bytes, int64_t n_groups, int32_t* order, int32_t* offsets,
-                               int32_t* tile_base, int32_t* keys, void* workspace, int64_t workspace_bytes, void* stream) {
-    using namespace nerf::grp;
-    NERF_REQUIRE(sizes_ok(n, n_groups), NERF_E_SHAPE);
-    NERF_REQUIRE(id_bytes == 4 || id_bytes == 8, NERF_E_DTYPE);
-    if (n == 0) return NERF_OK;
-    NERF_REQUIRE(ids && order && offsets && workspace, NERF_E_NULL);
-    NERF_REQUIRE(nerf_aligned(ids, (uintptr_t)id_bytes) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
+int64_t nerf::grp::workspace_bytes(int64_t n, int64_t n_groups) { return plan_for(n, n_groups).bytes; }
+
+int nerf::grp::launch_group_rows(int64_t n, const void* ids, int id_bytes, int64_t n_groups, int32_t* order, int32_t* offsets,
+                                 int32_t* tile_base, int32_t* keys, void* workspace, hipStream_t st) {
     const Plan p = plan_for(n, n_groups);
-    NERF_REQUIRE(workspace_bytes >= p.bytes, NERF_E_WORKSPACE);
-    hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     int32_t* kout = keys ? keys : (p.passes > 1 ? (int32_t*)(ws + p.kout) : nullptr);
     const int G = (int)n_groups;
@@ -382,22 +403,30 @@ extern "C" int nerf_group_rows(int64_t n, const void* ids, int id_bytes, int64_t
         int32_t *ka = (int32_t*)(ws + p.ka), *ia = (int32_t*)(ws + p.ia), *kb = (int32_t*)(ws + p.kb), *ib = (int32_t*)(ws + p.ib);
         const dim3 grid((unsigned)p.nblk), block(BLOCK_THREADS);
         const int nblk = (int)p.nblk;
+        const unsigned lds_hist = 4u << p.bits, lds_scatter = (BLOCK_THREADS / 64 + 1) * (4u << p.bits);
         const int32_t *kin = nullptr, *iin = nullptr;
         for (int pass = 0; pass < p.passes; ++pass) {
             const bool last = pass == p.passes - 1;
             int32_t* ko = last ? kout : (pass & 1 ? kb : ka);
             int32_t* io = last ? order : (pass & 1 ? ib : ia);
             const int shift = pass * p.bits;
-#define NERF_PASS(ID, SRC)                                                                                                     \
-    do {                                                                                                                       \
-        hipLaunchKernelGGL(hist_kernel<ID>, grid, block, 0, st, n, (const ID*)(SRC), (unsigned)G, shift, p.bits, nblk, hist);   \
-        hipLaunchKernelGGL(rowscan_kernel, dim3(1u << p.bits), block, 0, st, nblk, hist, totals);                               \
-        hipLaunchKernelGGL(scatter_kernel<ID>, grid, block, 0, st, n, (const ID*)(SRC), iin, (unsigned)G, shift, p.bits, nblk,  \
-                           hist, totals, ko, io, p.passes == 1 ? 1 : 0, offsets, tile_base);                                    \
+#define NERF_PASS(ID, ROUNDS, SRC)                                                                                                   \
+    do {                                                                                                                             \
+        hipLaunchKernelGGL((hist_kernel<ID, ROUNDS>), grid, block, lds_hist, st, n, (const ID*)(SRC), (unsigned)G, shift, p.bits,     \
+                           nblk, hist);                                                                                              \
+        hipLaunchKernelGGL(rowscan_kernel, dim3(1u << p.bits), block, 0, st, nblk, hist, totals);                                     \
+        hipLaunchKernelGGL((scatter_kernel<ID, ROUNDS>), grid, block, lds_scatter, st, n, (const ID*)(SRC), iin, (unsigned)G, shift,  \
+                           p.bits, nblk, hist, totals, ko, io, p.passes == 1 ? 1 : 0, offsets, tile_base);                            \
     } while (0)
-            if (pass > 0) NERF_PASS(int32_t, kin);
-            else if (id_bytes == 8) NERF_PASS(int64_t, ids);
-            else NERF_PASS(int32_t, ids);
+#define NERF_PASS_R(ID, SRC)                                        \
+    do {                                                            \
+        if (p.rounds == FEW_ROUNDS) NERF_PASS(ID, FEW_ROUNDS, SRC); \
+        else NERF_PASS(ID, MANY_ROUNDS, SRC);                       \
+    } while (0)
+            if (pass > 0) NERF_PASS_R(int32_t, kin);
+            else if (id_bytes == 8) NERF_PASS_R(int64_t, ids);
+            else NERF_PASS_R(int32_t, ids);
+#undef NERF_PASS_R
 #undef NERF_PASS
             kin = ko;
             iin = io;
@@ -409,6 +438,18 @@ extern "C" int nerf_group_rows(int64_t n, const void* ids, int id_bytes, int64_t
         if (tile_base) hipLaunchKernelGGL(tile_base_kernel, dim3(1), dim3(SMALL_THREADS), 0, st, (int)n, G, offsets, tile_base);
     }
     return nerf_launch_status();
+}
+
+extern "C" int nerf_group_rows(int64_t n, const void* ids, int id_bytes, int64_t n_groups, int32_t* order, int32_t* offsets,
+                               int32_t* tile_base, void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace nerf::grp;
+    NERF_REQUIRE(sizes_ok(n, n_groups), NERF_E_SHAPE);
+    NERF_REQUIRE(id_bytes == 4 || id_bytes == 8, NERF_E_DTYPE);
+    if (n == 0) return NERF_OK;
+    NERF_REQUIRE(ids && order && offsets && workspace, NERF_E_NULL);
+    NERF_REQUIRE(nerf_aligned(ids, (uintptr_t)id_bytes) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
+    NERF_REQUIRE(workspace_bytes >= plan_for(n, n_groups).bytes, NERF_E_WORKSPACE);
+    return launch_group_rows(n, ids, id_bytes, n_groups, order, offsets, tile_base, nullptr, workspace, (hipStream_t)stream);
 }
 
 extern "C" int nerf_group_offsets(int64_t n, int64_t n_groups, const int32_t* offsets_in, int32_t* offsets, int32_t* tile_base,

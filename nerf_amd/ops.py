@@ -6,6 +6,7 @@ falls back to PyTorch arithmetic.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -718,6 +719,31 @@ def p16_mlp_backward(M: int, cp: int, cv: int, layers, grads, d_raw: torch.Tenso
 _ELEM = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _call(name: str, timer: str, dev: torch.device, units: int, *args) -> None:
+    """lib.<name>(*args, current stream of ``dev``).  These calls are short enough for the host's side of them to count, so
+    the device is switched only when another one is current and the stream comes as a plain number."""
+    if KERNEL_TIMES is None and torch.cuda.current_device() == dev.index:
+        rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev), _timed(timer, dev, units):
+            rc = getattr(lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        check(rc, name)
+
+
+@functools.lru_cache(maxsize=4096)
+def _size(name: str, *args) -> int:
+    """A workspace size: a function of the sizes alone."""
+    n = int(getattr(lib, name)(*args))
+    if n < 0:
+        check(n, name)
+    return n
+
+
 def _gpu_elem(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A bf16 / fp16 / fp32 GPU tensor, of the type and on the device of ``like`` when given."""
     if not isinstance(t, torch.Tensor):
@@ -776,31 +802,23 @@ def _group_sizes(n: int, n_groups: int) -> None:
         raise ValueError(f"at most {_MAX_GROUPED_ROWS} rows, got {n}")
 
 
-def _group(ids: torch.Tensor, n_groups: int, tiles: bool, keys: bool):
-    n, dev = ids.numel(), ids.device
-    _group_sizes(n, n_groups)
-    new = torch.zeros if n == 0 else torch.empty
-    order = torch.empty((n,), dtype=torch.int32, device=dev)
-    offsets = new((n_groups + 1,), dtype=torch.int32, device=dev)
-    base = new((n_groups + 2,), dtype=torch.int32, device=dev) if tiles else None
-    sorted_ids = torch.empty((n,), dtype=torch.int32, device=dev) if keys else None
-    nbytes = int(lib.nerf_group_rows_workspace_bytes(n, n_groups))
-    work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev), _timed("group_rows", dev, n):
-        check(lib.nerf_group_rows(n, _p(ids), ids.element_size(), n_groups, _p(order), _p(offsets), _p(base), _p(sorted_ids),
-                                  _p(work), nbytes, _stream(dev)), "nerf_group_rows")
-    return order, offsets, base, sorted_ids
-
-
 def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
     """The rows 0 .. n-1 in order of their group ``ids`` [n] (int32 or int64), rows of one group in their own order.
     An id outside [0, n_groups) belongs to no group; such rows come last."""
     ids = _gpu_ids(ids, "ids")
     if ids.dim() != 1:
         raise ValueError(f"ids must be 1-D, got {tuple(ids.shape)}")
-    n_groups = int(n_groups)
-    order, offsets, base, _ = _group(ids, n_groups, True, False)
-    return RowGroups(order, offsets, base, ids.numel(), n_groups)
+    n, n_groups, dev = ids.numel(), int(n_groups), ids.device
+    _group_sizes(n, n_groups)
+    new = torch.zeros if n == 0 else torch.empty
+    order = torch.empty((n,), dtype=torch.int32, device=dev)
+    offsets = new((n_groups + 1,), dtype=torch.int32, device=dev)
+    base = new((n_groups + 2,), dtype=torch.int32, device=dev)
+    nbytes = _size("nerf_group_rows_workspace_bytes", n, n_groups)
+    work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    _call("nerf_group_rows", "group_rows", dev, n, n, ids.data_ptr(), ids.element_size(), n_groups, order.data_ptr(), offsets.data_ptr(),
+          base.data_ptr(), work.data_ptr(), nbytes)
+    return RowGroups(order, offsets, base, n, n_groups)
 
 
 def row_groups(offsets: torch.Tensor, n_rows: int) -> RowGroups:
@@ -818,9 +836,17 @@ def row_groups(offsets: torch.Tensor, n_rows: int) -> RowGroups:
     new = torch.zeros if n_rows == 0 else torch.empty
     clean = new((n_groups + 1,), dtype=torch.int32, device=dev)
     base = new((n_groups + 2,), dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        check(lib.nerf_group_offsets(n_rows, n_groups, _p(given), _p(clean), _p(base), _stream(dev)), "nerf_group_offsets")
+    _call("nerf_group_offsets", "group_offsets", dev, n_rows, n_rows, n_groups, given.data_ptr(), clean.data_ptr(), base.data_ptr())
     return RowGroups(None, clean, base, n_rows, n_groups)
+
+
+def _embed_fwd(ids, table, scale):
+    n, (rows, dim), dev = ids.numel(), table.shape, table.device
+    table, ld = _row_major(table)
+    out = torch.empty(ids.shape + (dim,), dtype=table.dtype, device=dev)
+    _call("nerf_embed_fwd", "embed_fwd", dev, n, n, ids.data_ptr(), ids.element_size(), rows, dim, table.data_ptr(), ld, scale,
+          _ELEM[table.dtype], out.data_ptr())
+    return out
 
 
 class _EmbedRows(torch.autograd.Function):
@@ -828,15 +854,9 @@ class _EmbedRows(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, ids, table, scale):
-        n, (rows, dim), dev = ids.numel(), table.shape, table.device
-        table, ld = _row_major(table)
-        out = torch.empty(tuple(ids.shape) + (dim,), dtype=table.dtype, device=dev)
-        with torch.cuda.device(dev), _timed("embed_fwd", dev, n):
-            check(lib.nerf_embed_fwd(n, _p(ids), ids.element_size(), rows, dim, _p(table), ld, scale, _ELEM[table.dtype], _p(out),
-                                     _stream(dev)), "nerf_embed_fwd")
         ctx.save_for_backward(ids)
-        ctx.sizes, ctx.scale = (rows, dim), scale
-        return out
+        ctx.sizes, ctx.scale = tuple(table.shape), scale
+        return _embed_fwd(ids, table, scale)
 
     @staticmethod
     @once_differentiable
@@ -846,14 +866,12 @@ class _EmbedRows(torch.autograd.Function):
         n, dev = ids.numel(), d_out.device
         if n == 0:
             return None, torch.zeros((rows, dim), dtype=d_out.dtype, device=dev), None
-        order, offsets, _, keys = _group(ids.reshape(-1), rows, False, True)
         g, ld = _row_major(d_out.reshape(n, dim))
         d_table = torch.empty((rows, dim), dtype=g.dtype, device=dev)
-        nbytes = int(lib.nerf_embed_bwd_workspace_bytes(n, rows, dim))
+        nbytes = _size("nerf_embed_bwd_workspace_bytes", n, rows, dim)
         work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev), _timed("embed_bwd", dev, n):
-            check(lib.nerf_embed_bwd(n, rows, dim, _p(order), _p(offsets), _p(keys), _p(g), ld, ctx.scale, _ELEM[g.dtype],
-                                     _p(d_table), _p(work), nbytes, _stream(dev)), "nerf_embed_bwd")
+        _call("nerf_embed_bwd", "embed_bwd", dev, n, n, ids.data_ptr(), ids.element_size(), rows, dim, g.data_ptr(), ld, ctx.scale,
+              _ELEM[g.dtype], d_table.data_ptr(), work.data_ptr(), nbytes)
         return None, d_table, None
 
 
@@ -872,7 +890,22 @@ def embed_rows(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> to
     if table.shape[1] > 2 ** 20:
         raise ValueError(f"at most {2 ** 20} columns, got {table.shape[1]}")
     _group_sizes(ids.numel(), table.shape[0])
-    return _EmbedRows.apply(ids, table, float(scale))
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _EmbedRows.apply(ids, table, float(scale))
+    return _embed_fwd(ids, table, float(scale))
+
+
+def _grouped_fwd(x, weight, bias, groups, relu):
+    """(y, x as it was read, weight as it was read)"""
+    n, dev = groups.n_rows, x.device
+    G, N, K = weight.shape
+    x, ld = _row_major(x)
+    weight = weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty((n, N), dtype=x.dtype, device=dev)
+    _call("nerf_grouped_fwd", "grouped_fwd", dev, n, n, G, _ptr(groups.order), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N,
+          x.data_ptr(), ld, weight.data_ptr(), _ptr(bias), int(relu), _ELEM[x.dtype], y.data_ptr())
+    return y, x, weight
 
 
 class _GroupedLinear(torch.autograd.Function):
@@ -880,17 +913,9 @@ class _GroupedLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, relu):
-        n, dev = groups.n_rows, x.device
-        G, N, K = weight.shape
-        xr, ld = _row_major(x)
-        weight = weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        y = torch.empty((n, N), dtype=x.dtype, device=dev)
-        with torch.cuda.device(dev), _timed("grouped_fwd", dev, n):
-            check(lib.nerf_grouped_fwd(n, G, _p(groups.order), _p(groups.offsets), _p(groups.tile_base), K, N, _p(xr), ld, _p(weight),
-                                       _p(bias), int(relu), _ELEM[x.dtype], _p(y), _stream(dev)), "nerf_grouped_fwd")
-        ctx.save_for_backward(xr, weight, y if relu else None)
-        ctx.groups, ctx.has_bias = groups, bias is not None
+        y, x, weight = _grouped_fwd(x, weight, bias, groups, relu)
+        ctx.save_for_backward(x, weight, y if relu else None)
+        ctx.groups = groups
         return y
 
     @staticmethod
@@ -905,21 +930,18 @@ class _GroupedLinear(torch.autograd.Function):
             return (torch.zeros((0, K), dtype=d_y.dtype, device=dev) if need_x else None, torch.zeros_like(weight) if need_w else None,
                     torch.zeros((G, N), dtype=d_y.dtype, device=dev) if need_b else None, None, None)
         g, ld = _row_major(d_y)
-        at = (n, G, _p(groups.order), _p(groups.offsets), _p(groups.tile_base), K, N, _p(g), ld, _p(y))
-        with torch.cuda.device(dev):
-            if need_x:
-                dx = torch.empty((n, K), dtype=g.dtype, device=dev)
-                with _timed("grouped_bwd_data", dev, n):
-                    check(lib.nerf_grouped_bwd_data(*at, _p(weight), prec, _p(dx), _stream(dev)), "nerf_grouped_bwd_data")
-            if need_w or need_b:
-                dw = torch.empty_like(weight)
-                db = torch.empty((G, N), dtype=g.dtype, device=dev) if need_b else None
-                xr, x_ld = _row_major(x)
-                nbytes = int(lib.nerf_grouped_bwd_weights_workspace_bytes(n, G, K, N))
-                work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-                with _timed("grouped_bwd_weights", dev, n):
-                    check(lib.nerf_grouped_bwd_weights(*at, _p(xr), x_ld, prec, _p(dw), _p(db), _p(work), nbytes, _stream(dev)),
-                          "nerf_grouped_bwd_weights")
+        at = (n, G, _ptr(groups.order), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N, g.data_ptr(), ld, _ptr(y))
+        if need_x:
+            dx = torch.empty((n, K), dtype=g.dtype, device=dev)
+            _call("nerf_grouped_bwd_data", "grouped_bwd_data", dev, n, *at, weight.data_ptr(), prec, dx.data_ptr())
+        if need_w or need_b:
+            dw = torch.empty((G, N, K), dtype=g.dtype, device=dev)
+            db = torch.empty((G, N), dtype=g.dtype, device=dev) if need_b else None
+            x, x_ld = _row_major(x)
+            nbytes = _size("nerf_grouped_bwd_weights_workspace_bytes", n, G, K, N)
+            work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            _call("nerf_grouped_bwd_weights", "grouped_bwd_weights", dev, n, *at, x.data_ptr(), x_ld, prec, dw.data_ptr(), _ptr(db),
+                  work.data_ptr(), nbytes)
         return dx, dw if need_w else None, db, None, None
 
 
@@ -951,8 +973,12 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
         bias = _gpu_elem(bias, "bias", x)
         if tuple(bias.shape) != (G, N):
             raise ValueError(f"bias must be [{G}, {N}], got {tuple(bias.shape)}")
-    y = _GroupedLinear.apply(x.reshape(-1, K), weight, bias, groups, bool(relu))
-    return y.view(tuple(x.shape[:-1]) + (N,))
+    rows = x if x.dim() == 2 else x.reshape(-1, K)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
+        y = _GroupedLinear.apply(rows, weight, bias, groups, bool(relu))
+    else:
+        y = _grouped_fwd(rows, weight, bias, groups, bool(relu))[0]
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))
 
 
 # ---------------------------------------------------------------------------
@@ -962,13 +988,31 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
 def _scan_input(t: torch.Tensor, vec: int) -> Tuple[torch.Tensor, int, int]:
     """(tensor, elements between sequences, between samples) as the kernels read it: channels contiguous, pieces of ``vec``
     elements aligned; copied when it is not."""
-    def strides(u):
-        return tuple(u.stride(i) if u.shape[i] > 1 else 0 for i in (0, 1))
-    sb, st = strides(t)
-    if t.shape[2] > 1 and t.stride(2) != 1 or sb % vec or st % vec or t.data_ptr() % (vec * t.element_size()):
+    (B, T, D), (sb, st, sc) = t.shape, t.stride()
+    sb, st = sb if B > 1 else 0, st if T > 1 else 0
+    if D > 1 and sc != 1 or sb % vec or st % vec or t.data_ptr() % (vec * t.element_size()):
         t = t.clone(memory_format=torch.contiguous_format)
-        sb, st = strides(t)
+        sb, st = T * D if B > 1 else 0, D if T > 1 else 0
     return t, sb, st
+
+
+def _scan_fwd(gate, value, state, reverse, need):
+    """(h, last, gate, value and state as they were read, the states the backward starts from)"""
+    (B, T, D), dev, prec = value.shape, value.device, _ELEM[value.dtype]
+    full = 16 // value.element_size()
+    shared = gate.shape[2] == 1 and D > 1
+    vec = full if D % full == 0 else 1
+    value, vsb, vst = _scan_input(value, vec)
+    gate, gsb, gst = _scan_input(gate, 1 if shared else vec)
+    state = None if state is None else state.contiguous()
+    h = torch.empty((B, T, D), dtype=value.dtype, device=dev)
+    last = torch.empty((B, D), dtype=torch.float32, device=dev)
+    states = torch.empty((_size("nerf_scan_states_floats", B, T, D, prec),), dtype=torch.float32, device=dev) if need else None
+    nbytes = _size("nerf_scan_workspace_bytes", B, T, D, int(shared), 0, prec)
+    work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    _call("nerf_scan_fwd", "scan_fwd", dev, B * T, B, T, D, gate.data_ptr(), gsb, gst, int(shared), value.data_ptr(), vsb, vst, _ptr(state),
+          int(reverse), prec, h.data_ptr(), last.data_ptr(), _ptr(states), work.data_ptr(), nbytes)
+    return h, last, gate, value, state, states
 
 
 class _GatedScan(torch.autograd.Function):
@@ -976,24 +1020,9 @@ class _GatedScan(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gate, value, state, reverse):
-        (B, T, D), dev, prec = value.shape, value.device, _ELEM[value.dtype]
-        full = 16 // value.element_size()
-        shared = gate.shape[2] == 1 and D > 1
-        vec = full if D % full == 0 else 1
-        va, vsb, vst = _scan_input(value, vec)
-        ga, gsb, gst = _scan_input(gate, 1 if shared else vec)
-        st = None if state is None else state.contiguous()
-        h = torch.empty((B, T, D), dtype=value.dtype, device=dev)
-        last = torch.empty((B, D), dtype=torch.float32, device=dev)
-        need = any(ctx.needs_input_grad[:3])
-        states = torch.empty((int(lib.nerf_scan_states_floats(B, T, D, prec)),), dtype=torch.float32, device=dev) if need else None
-        nbytes = int(lib.nerf_scan_workspace_bytes(B, T, D, int(shared), 0, prec))
-        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev), _timed("scan_fwd", dev, B * T):
-            check(lib.nerf_scan_fwd(B, T, D, _p(ga), gsb, gst, int(shared), _p(va), vsb, vst, _p(st), int(reverse), prec, _p(h), _p(last),
-                                    _p(states), _p(work), nbytes, _stream(dev)), "nerf_scan_fwd")
-        ctx.save_for_backward(ga, va, st, states)
-        ctx.how = (shared, vec, bool(reverse))
+        h, last, gate, value, state, states = _scan_fwd(gate, value, state, reverse, True)
+        ctx.save_for_backward(gate, value, state, states)
+        ctx.reverse = reverse
         ctx.set_materialize_grads(False)
         return h, last
 
@@ -1003,25 +1032,26 @@ class _GatedScan(torch.autograd.Function):
         if d_h is None and d_last is None:
             return None, None, None, None
         gate, value, state, states = ctx.saved_tensors
-        shared, vec, reverse = ctx.how
         (B, T, D), dev, prec = value.shape, value.device, _ELEM[value.dtype]
         need_gate, need_value, need_state = ctx.needs_input_grad[:3]
-        ga, gsb, gst = _scan_input(gate, 1 if shared else vec)
-        va, vsb, vst = _scan_input(value, vec)
+        shared = gate.shape[2] == 1 and D > 1
+        full = 16 // value.element_size()
+        vec = full if D % full == 0 else 1
+        gate, gsb, gst = _scan_input(gate, 1 if shared else vec)
+        value, vsb, vst = _scan_input(value, vec)
         if d_h is not None:
             d_h = d_h.contiguous()
             if d_h.data_ptr() % (vec * d_h.element_size()):
                 d_h = d_h.clone()
-        d_last = None if d_last is None else _gpu_f32(d_last, "d_last")
+        d_last = None if d_last is None else d_last.contiguous()
         d_gate = torch.empty((B, T, 1 if shared else D), dtype=value.dtype, device=dev) if need_gate else None
         d_value = torch.empty((B, T, D), dtype=value.dtype, device=dev) if need_value else None
         d_state = torch.empty((B, D), dtype=torch.float32, device=dev) if need_state else None
-        nbytes = int(lib.nerf_scan_workspace_bytes(B, T, D, int(shared), 1, prec))
+        nbytes = _size("nerf_scan_workspace_bytes", B, T, D, int(shared), 1, prec)
         work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev), _timed("scan_bwd", dev, B * T):
-            check(lib.nerf_scan_bwd(B, T, D, _p(ga), gsb, gst, int(shared), _p(va), vsb, vst, _p(state), _p(states), _p(d_h), _p(d_last),
-                                    int(reverse), prec, _p(d_gate), _p(d_value), _p(d_state), _p(work), nbytes, _stream(dev)),
-                  "nerf_scan_bwd")
+        _call("nerf_scan_bwd", "scan_bwd", dev, B * T, B, T, D, gate.data_ptr(), gsb, gst, int(shared), value.data_ptr(), vsb, vst,
+              _ptr(state), states.data_ptr(), _ptr(d_h), _ptr(d_last), int(ctx.reverse), prec, _ptr(d_gate), _ptr(d_value), _ptr(d_state),
+              work.data_ptr(), nbytes)
         return d_gate, d_value, d_state, None
 
 
@@ -1054,7 +1084,11 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: Optional[torch.Te
     if B == 0 or T == 0:
         last = value.new_zeros((B, D), dtype=torch.float32) if state is None else state.clone()
         return value.clone(), last
-    return _GatedScan.apply(gate.expand(B, T, gate.shape[2]), value, state, bool(reverse))
+    if gate.shape[0] != B or gate.shape[1] != T:
+        gate = gate.expand(B, T, gate.shape[2])
+    if torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or state is not None and state.requires_grad):
+        return _GatedScan.apply(gate, value, state, bool(reverse))
+    return _scan_fwd(gate, value, state, bool(reverse), False)[:2]
 
 
 # ---------------------------------------------------------------------------
