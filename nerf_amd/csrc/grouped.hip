@@ -6,13 +6,20 @@
 // Rows stay where they are: a tile is 128 consecutive positions of the grouped order, and the kernels read and write
 // row order[position] of the ordinary tensors (a row is one or more whole cache lines, so gathering costs nothing).  The
 // number of tiles is known on the device only: the grid is the upper bound n / 128 + groups + 1 and a workgroup finds its
-// group in tile_base, the running number of tiles, with one or two 64-wide comparisons.
+// group in tile_base, the running number of tiles, with a 64-wide comparison.
 //
-// Operands go through registers into LDS in 16-byte pieces, two buffers, one barrier per step; products run on
-// v_mfma_f32_32x32x16_{bf16,f16} or, in fp32, v_mfma_f32_32x32x2_f32 (exact products, fp32 sums).  A 16-byte piece holds
-// the values of consecutive contraction indices of one row; operands whose contraction index is the row (W in dX, both in
-// dW) are read with ds_read_b64_tr_b16, which hands a lane four rows of its column, or in fp32 with four 4-byte reads.
-// LDS pieces are permuted within a row so that the 16 (8) lanes of one LDS cycle fall on different banks.
+// A workgroup of four waves multiplies 128 rows by 128 (64) outputs.  One contraction step of both operands, 32 KiB, is
+// copied into LDS by the memory system itself (global_load_lds, 16 bytes per lane), read whole into registers, and the
+// copy of the next step runs while the products of this one are formed: v_mfma_f32_32x32x16_{bf16,f16} or, in fp32,
+// v_mfma_f32_32x32x2_f32 (exact products, fp32 sums).  One buffer is enough for that, so three workgroups share a compute
+// unit and one's reads sit beside the others' products; a persistent form with two buffers and register staging was slower
+// (its copies had to be waited for together).  Operands that are not in whole aligned 16-byte pieces, and gradients that a
+// ReLU gates, go through registers instead of the direct copy, in the same loop.
+//
+// A 16-byte piece holds the values of consecutive contraction indices of one row; operands whose contraction index is the
+// row (W in dX, both in dW) are read with ds_read_b64_tr_b16, which hands a lane four rows of its column, or in fp32 with
+// four 4-byte reads.  Pieces are permuted within a row (by the address they are copied from) so that the lanes of one LDS
+// cycle fall on different banks.
 #include "elems.hpp"
 #include "groups.hpp"
 
@@ -59,39 +66,58 @@ __device__ __forceinline__ typename El<T>::frag nt_frag(const char* tile, int ro
     return *reinterpret_cast<const typename El<T>::frag*>(tile + nt_addr(row0 + (lane & 31), 2 * s + (lane >> 5)));
 }
 
-// ---- row-major tile, contraction index = row: [step_len rows][up to 128 columns] ------------------------------
-template <typename T> constexpr int tr_pitch() { return sizeof(T) == 2 ? 256 : 544; }
-template <typename T> constexpr int tr_bytes() { return step_len<T>() * tr_pitch<T>(); }
-template <typename T>
-__device__ __forceinline__ int tr_addr(int row, int q) {
-    if constexpr (sizeof(T) == 2) return row * 256 + ((q ^ ((row & 3) << 2)) << 4);
-    else return row * 544 + (q << 4);
+// ---- row-major tile, contraction index = row: [step_len rows][COLS columns] -----------------------------------
+// 16-bit: a transposing read takes 64 bytes of four rows, which go to different 64-byte windows; fp32: lanes 0-31 read a
+// row and lanes 32-63 the fourth one after it, which go to different halves of the banks
+template <typename T, int COLS>
+__device__ __forceinline__ int tr_swap(int row) {
+    if constexpr (sizeof(T) == 2) return (row & (COLS < 128 ? 1 : 3)) << 2;
+    else return ((row >> 2) & 1) << 3;
+}
+template <typename T, int COLS>
+__device__ __forceinline__ int tr_addr(int row, int q) { return row * (COLS * (int)sizeof(T)) + ((q ^ tr_swap<T, COLS>(row)) << 4); }
+template <typename T, int COLS> constexpr int tr_bytes() { return step_len<T>() * COLS * (int)sizeof(T); }
+
+// where a lane begins to read its fragment of columns col0 .. col0 + 31 in product step s
+template <typename T, int COLS>
+__device__ __forceinline__ int tr_lane(int col0, int s, int lane) {
+    if constexpr (sizeof(T) == 2) {
+        const int row = 16 * s + 8 * (lane >> 5) + ((lane & 15) >> 2), col = col0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        return tr_addr<T, COLS>(row, col >> 3) + ((col >> 2) & 1) * 8;
+    } else {
+        const int col = col0 + (lane & 31);
+        return tr_addr<T, COLS>(8 * s + 4 * (lane >> 5), col >> 2) + (col & 3) * 4;
+    }
 }
 
-template <typename T>
+template <typename T, int COLS>
 __device__ __forceinline__ typename El<T>::frag tr_frag(const char* tile, int col0, int s, int lane) {
+    const char* at = tile + tr_lane<T, COLS>(col0, s, lane);
     if constexpr (sizeof(T) == 2) {
-        const int i = lane & 15;
-        const int row = 16 * s + 8 * (lane >> 5) + (i >> 2);
-        const int col = col0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
         typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-        const int a = tr_addr<T>(row, col >> 3) + ((col >> 2) & 1) * 8;      // rows 4 apart share their permutation
         struct Two { s16x4 lo, hi; } f;
-        f.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + a));
-        f.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + a + 4 * 256));
+        f.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
+        f.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 4 * COLS * (int)sizeof(T)));    // rows 4 apart share their permutation
         return __builtin_bit_cast(typename El<T>::frag, f);
     } else {
-        const int row = 8 * s + 4 * (lane >> 5), col = col0 + (lane & 31);
         f32x4 f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(tile + (row + j) * 544 + col * 4);
+        for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(at + j * COLS * 4);        // so do four rows in a run
         return f;
     }
 }
 
+// ---- copies straight into LDS: lane l of a wave fills bytes 16 l .. of the 1 KiB at `to` (wave-uniform) -------------
+typedef __attribute__((address_space(1))) const char gbl_char;
+typedef __attribute__((address_space(3))) char lds_char;
+__device__ __constant__ const float4 ZERO_PIECE = {0.0f, 0.0f, 0.0f, 0.0f};      // read where an operand has nothing
+__device__ __forceinline__ void copy_piece(const void* from, char* to) {
+    __builtin_amdgcn_global_load_lds((gbl_char*)from, (lds_char*)to, 16, 0, 0);
+}
+
 // ---- pieces from memory ---------------------------------------------------------------------------------------
 // columns c .. of a row that has `cols` of them; zero behind its end and when !ok
-template <typename T, bool WIDE>
+template <typename T, bool WIDE = false>
 __device__ __forceinline__ Pack<T, piece<T>()> load_piece(const T* row, int c, int cols, bool ok) {
     constexpr int E = piece<T>();
     Pack<T, E> p;
@@ -117,6 +143,27 @@ __device__ __forceinline__ void gate_piece(Pack<T, E>& g, const Pack<T, E>& y) {
         if ((float)y.v[e] <= 0.0f) g.v[e] = (T)0.0f;
 }
 
+// The same on fragments.  A layer's output comes from its ReLU, which leaves no sign on a zero or a NaN, so "not zero" is
+// "greater than zero as an integer": two packed comparisons and a product per register instead of eight conversions.
+template <typename T>
+__device__ __forceinline__ typename El<T>::frag gate_frag(typename El<T>::frag g, typename El<T>::frag y) {
+    if constexpr (sizeof(T) == 2) {
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 one = 1, none = 0;
+        const s16x8 keep = __builtin_elementwise_max(__builtin_elementwise_min(__builtin_bit_cast(s16x8, y), one), none);
+        return __builtin_bit_cast(typename El<T>::frag, __builtin_bit_cast(s16x8, g) * keep);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = __builtin_bit_cast(int, (float)y[e]) > 0 ? g[e] : 0.0f;
+        return g;
+    }
+}
+
+// ReLU with least = 0 and no sign bit in `bits` (keeps a NaN, without its sign); the identity with -inf and all bits
+__device__ __forceinline__ float relu_or_not(float v, float least, unsigned bits) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v < least ? 0.0f : v) & bits);
+}
+
 struct Rows {
     int64_t n;
     int n_groups;
@@ -125,7 +172,6 @@ struct Rows {
 
 // row of a position; -1 for an entry that is no row
 __device__ __forceinline__ int row_at(const Rows& r, int64_t pos) {
-    if (!r.order) return (int)pos;
     const int row = r.order[pos];
     return row >= 0 && row < r.n ? row : -1;
 }
@@ -139,17 +185,566 @@ struct LinArgs {
     void* out;
 };
 
+// A tile of a call: group, first position, rows, first output.  Up to 62 groups the lanes of a wave hold both tables, one
+// round trip for the whole call; above, a tile costs two or three.
+struct Tile {
+    int64_t pos0;
+    int group, count, o0;
+};
+struct Tables {
+    int base, off, total, lane;
+    __device__ __forceinline__ Tables(const Rows& r, int lane_) : base(0), off(0), lane(lane_) {
+        if (r.n_groups < 63) {
+            base = r.tile_base[min(lane, r.n_groups + 1)];
+            off = r.offsets[min(lane, r.n_groups)];
+            total = __builtin_amdgcn_readlane(base, r.n_groups + 1);
+        } else {
+            total = r.tile_base[r.n_groups + 1];
+        }
+    }
+    __device__ __forceinline__ Tile tile(const Rows& r, int64_t at, int tiles_o, int bn) const {
+        const int G = r.n_groups;
+        Tile t;
+        const int i = __builtin_amdgcn_readfirstlane((int)(at / tiles_o));
+        t.o0 = (int)(at % tiles_o) * bn;
+        int first, begin, end;
+        if (G < 63) {
+            t.group = __popcll(__ballot(lane <= G && base <= i)) - 1;
+            first = __builtin_amdgcn_readlane(base, t.group);
+            begin = __builtin_amdgcn_readlane(off, t.group);
+            end = __builtin_amdgcn_readlane(off, min(t.group + 1, G));
+        } else {
+            t.group = grp::group_of_tile(r.tile_base, G, i, lane);
+            first = r.tile_base[t.group];
+            begin = r.offsets[t.group];
+            end = r.offsets[min(t.group + 1, G)];
+        }
+        t.pos0 = begin + (int64_t)(i - first) * TILE_ROWS;
+        const int64_t left = (t.group < G ? (int64_t)end : r.n) - t.pos0;
+        t.count = (int)(left < TILE_ROWS ? left : TILE_ROWS);
+        return t;
+    }
+};
+
+// ---- streaming form: operands in whole aligned 16-byte pieces ------------------------------------------------------
 // out[row][o] = sum_c a[row][c] w_g(o, c).  WT = false: w_g is [O][C] (the layer); WT = true: w_g is [C][O] (its data
-// gradient).  A tile is 128 rows x BN outputs, four waves.  The accumulators hold outputs down and rows across, so a
-// lane's four consecutive registers are consecutive outputs of one row.
-template <typename T, bool WT, bool GATE, bool WIDE, int BN>
+// gradient).  One workgroup of eight waves per compute unit for the whole call.  It owns a run of consecutive items (128
+// rows x BN outputs) and streams their contraction steps without a gap between items: the memory system copies step s + 2
+// into a ring of three LDS buffers (global_load_lds, 16 bytes per lane) while step s is multiplied; one barrier per step.
+//
+// vmcnt counts copies and stores in the order they were issued, so a step waits for its own copies only, with the number
+// of younger copies and stores left outstanding.  For that count to be known, every wave issues the same stores for every
+// item: a position behind a tile's rows repeats the tile's last row, outputs behind the last piece repeat that piece, and
+// what they store is what is there already.  LDS is read by inline asm (reads and their wait in one block), because the
+// compiler would wait for every copy in flight in front of a read it can see.
+//
+// The accumulators hold outputs down and rows across: a lane's four consecutive registers are consecutive outputs of one
+// row, and one exchange between the wave's halves (v_permlane32_swap) makes them eight, a 16-byte store.
+constexpr int ST_THREADS = 512;
+constexpr int ST_ITEMS = 12;            // items whose rows and bias are in LDS at a time
+
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ int lds_int(unsigned at) {
+    int v;
+    asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ f32x4 lds_quad(unsigned at) {
+    f32x4 v;
+    asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(at) : "memory");
+    return v;
+}
+
+// The fragments of one product step, all requested before the one wait.  a: MI row tiles 32 rows (4 KiB) apart from one
+// address; b: NJ output tiles, 4 KiB apart (NT).
+template <typename F, int MI, int NJ>
+__device__ __forceinline__ void read_nt(F (&a)[MI], F (&b)[NJ], unsigned pa, unsigned pb) {
+    if constexpr (MI == 2 && NJ == 2)
+        asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %2, %5\n\tds_read_b128 %1, %4 offset:4096\n\tds_read_b128 %3, %5 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(a[0]), "=&v"(a[1]), "=&v"(b[0]), "=&v"(b[1]) : "v"(pa), "v"(pb) : "memory");
+    else if constexpr (MI == 2 && NJ == 1)
+        asm volatile("ds_read_b128 %0, %3\n\tds_read_b128 %2, %4\n\tds_read_b128 %1, %3 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(a[0]), "=&v"(a[1]), "=&v"(b[0]) : "v"(pa), "v"(pb) : "memory");
+    else
+        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(a[0]), "=&v"(b[0]) : "v"(pa), "v"(pb) : "memory");
+}
+template <typename F, int MI>
+__device__ __forceinline__ void read_rows(F (&a)[MI], unsigned pa) {
+    if constexpr (MI == 2)
+        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(a[0]), "=&v"(a[1]) : "v"(pa) : "memory");
+    else
+        asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(a[0]) : "v"(pa) : "memory");
+}
+// A transposed fragment: two reads four rows apart (16-bit) or one per row (fp32; four rows share their permutation)
+template <typename T, int PITCH>
+__device__ __forceinline__ typename El<T>::frag read_tr(unsigned at0) {
+    if constexpr (sizeof(T) == 2) {
+        struct Two { s16x4 lo, hi; } f;
+        asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(f.lo), "=&v"(f.hi) : "v"(at0), "n"(4 * PITCH) : "memory");
+        return __builtin_bit_cast(typename El<T>::frag, f);
+    } else {
+        float x, y, z, w;
+        asm volatile("ds_read_b32 %0, %4\n\tds_read_b32 %1, %4 offset:%5\n\tds_read_b32 %2, %4 offset:%6\n\tds_read_b32 %3, %4 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(x), "=&v"(y), "=&v"(z), "=&v"(w) : "v"(at0), "n"(PITCH), "n"(2 * PITCH), "n"(3 * PITCH) : "memory");
+        return typename El<T>::frag{x, y, z, w};
+    }
+}
+
+// One product step: the fragments of the next step are requested, the products of this one are issued, and only then the
+// requests are waited for, all in one block.  x: rows, w: outputs; nx, nw: the next step's.  The first s_nop covers an
+// accumulator that was just written, settle() the products' own latency in front of anything that reads one.
+#define NERF_BLOCK_HEAD "s_nop 1\n\t"
+#define NERF_BLOCK_TAIL "s_waitcnt lgkmcnt(0)"
+#define NERF_READ_X2 "ds_read_b128 %[nx0], %[pa]\n\tds_read_b128 %[nx1], %[pa] offset:4096\n\t"
+#define NERF_READ_X1 "ds_read_b128 %[nx0], %[pa]\n\t"
+#define NERF_READ_W2 "ds_read_b128 %[nw0], %[pb]\n\tds_read_b128 %[nw1], %[pb] offset:4096\n\t"
+#define NERF_READ_W1 "ds_read_b128 %[nw0], %[pb]\n\t"
+#define NERF_READ_TR(lo, hi, at) "ds_read_b64_tr_b16 %[" lo "], %[" at "]\n\tds_read_b64_tr_b16 %[" hi "], %[" at "] offset:%[rows4]\n\t"
+#define NERF_MFMA(op, c, w, x) op " %[" c "], %[" w "], %[" x "], %[" c "]\n\t"
+#define NERF_MFMA22(op) NERF_MFMA(op, "c00", "w0", "x0") NERF_MFMA(op, "c01", "w1", "x0") NERF_MFMA(op, "c10", "w0", "x1") NERF_MFMA(op, "c11", "w1", "x1")
+#define NERF_MFMA21(op) NERF_MFMA(op, "c00", "w0", "x0") NERF_MFMA(op, "c10", "w0", "x1")
+#define NERF_MFMA11(op) NERF_MFMA(op, "c00", "w0", "x0")
+
+template <typename T, int MI, int NJ>
+__device__ __forceinline__ void settle(f32x16 (&c)[MI][NJ]) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(c[i][j]));
+}
+
+// 16-bit operands; OP names the instruction of the type
+#define NERF_BLOCKS_16(T, OP)                                                                                                           \
+    template <int MI, int NJ, typename F>                                                                                               \
+    __device__ __forceinline__ void block_nt(T, f32x16 (&c)[MI][NJ], F (&x)[MI], F (&w)[NJ], unsigned pa, unsigned pb) {                \
+        F nx[MI], nw[NJ];                                                                                                               \
+        if constexpr (MI == 2 && NJ == 2)                                                                                               \
+            asm volatile(NERF_BLOCK_HEAD NERF_READ_X2 NERF_READ_W2 NERF_MFMA22(OP) NERF_BLOCK_TAIL                                      \
+                         : [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1]), [nx0] "=&v"(nx[0]),      \
+                           [nx1] "=&v"(nx[1]), [nw0] "=&v"(nw[0]), [nw1] "=&v"(nw[1])                                                   \
+                         : [x0] "v"(x[0]), [x1] "v"(x[1]), [w0] "v"(w[0]), [w1] "v"(w[1]), [pa] "v"(pa), [pb] "v"(pb)                   \
+                         : "memory");                                                                                                   \
+        else if constexpr (MI == 2)                                                                                                     \
+            asm volatile(NERF_BLOCK_HEAD NERF_READ_X2 NERF_READ_W1 NERF_MFMA21(OP) NERF_BLOCK_TAIL                                      \
+                         : [c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]), [nx0] "=&v"(nx[0]), [nx1] "=&v"(nx[1]), [nw0] "=&v"(nw[0])         \
+                         : [x0] "v"(x[0]), [x1] "v"(x[1]), [w0] "v"(w[0]), [pa] "v"(pa), [pb] "v"(pb)                                   \
+                         : "memory");                                                                                                   \
+        else                                                                                                                            \
+            asm volatile(NERF_BLOCK_HEAD NERF_READ_X1 NERF_READ_W1 NERF_MFMA11(OP) NERF_BLOCK_TAIL                                      \
+                         : [c00] "+v"(c[0][0]), [nx0] "=&v"(nx[0]), [nw0] "=&v"(nw[0])                                                  \
+                         : [x0] "v"(x[0]), [w0] "v"(w[0]), [pa] "v"(pa), [pb] "v"(pb)                                                   \
+                         : "memory");                                                                                                   \
+        for (int i = 0; i < MI; ++i) x[i] = nx[i];                                                                                      \
+        for (int j = 0; j < NJ; ++j) w[j] = nw[j];                                                                                      \
+    }                                                                                                                                   \
+    template <int PITCH, int MI, int NJ, int NP, typename F>                                                                            \
+    __device__ __forceinline__ void block_tr(T, f32x16 (&c)[MI][NJ], F (&x)[MI], F (&w)[NJ], unsigned pa, const unsigned (&pb)[NP],     \
+                                             unsigned stage) {                                                                          \
+        F nx[MI];                                                                                                                       \
+        struct Two { s16x4 lo, hi; } nw[NJ];                                                                                            \
+        if constexpr (MI == 2 && NJ == 2)                                                                                               \
+            asm volatile(NERF_BLOCK_HEAD NERF_READ_X2 NERF_READ_TR("l0", "h0", "p0") NERF_READ_TR("l1", "h1", "p1") NERF_MFMA22(OP)     \
+                         NERF_BLOCK_TAIL                                                                                                \
+                         : [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1]), [nx0] "=&v"(nx[0]),      \
+                           [nx1] "=&v"(nx[1]), [l0] "=&v"(nw[0].lo), [h0] "=&v"(nw[0].hi), [l1] "=&v"(nw[1].lo), [h1] "=&v"(nw[1].hi)   \
+                         : [x0] "v"(x[0]), [x1] "v"(x[1]), [w0] "v"(w[0]), [w1] "v"(w[1]), [pa] "v"(pa), [p0] "v"(pb[0] + stage),       \
+                           [p1] "v"(pb[1] + stage), [rows4] "n"(4 * PITCH)                                                              \
+                         : "memory");                                                                                                   \
+        else if constexpr (MI == 2)                                                                                                     \
+            asm volatile(NERF_BLOCK_HEAD NERF_READ_X2 NERF_READ_TR("l0", "h0", "p0") NERF_MFMA21(OP) NERF_BLOCK_TAIL                    \
+                         : [c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]), [nx0] "=&v"(nx[0]), [nx1] "=&v"(nx[1]), [l0] "=&v"(nw[0].lo),      \
+                           [h0] "=&v"(nw[0].hi)                                                                                         \
+                         : [x0] "v"(x[0]), [x1] "v"(x[1]), [w0] "v"(w[0]), [pa] "v"(pa), [p0] "v"(pb[0] + stage), [rows4] "n"(4 * PITCH) \
+                         : "memory");                                                                                                   \
+        else                                                                                                                            \
+            asm volatile(NERF_BLOCK_HEAD NERF_READ_X1 NERF_READ_TR("l0", "h0", "p0") NERF_MFMA11(OP) NERF_BLOCK_TAIL                    \
+                         : [c00] "+v"(c[0][0]), [nx0] "=&v"(nx[0]), [l0] "=&v"(nw[0].lo), [h0] "=&v"(nw[0].hi)                          \
+                         : [x0] "v"(x[0]), [w0] "v"(w[0]), [pa] "v"(pa), [p0] "v"(pb[0] + stage), [rows4] "n"(4 * PITCH)                \
+                         : "memory");                                                                                                   \
+        for (int i = 0; i < MI; ++i) x[i] = nx[i];                                                                                      \
+        for (int j = 0; j < NJ; ++j) w[j] = __builtin_bit_cast(F, nw[j]);                                                               \
+    }
+NERF_BLOCKS_16(__bf16, "v_mfma_f32_32x32x16_bf16")
+NERF_BLOCKS_16(_Float16, "v_mfma_f32_32x32x16_f16")
+#undef NERF_BLOCKS_16
+
+// fp32: four products per fragment, alternating between the accumulators
+#define NERF_OP32 "v_mfma_f32_32x32x2_f32"
+#define NERF_MFMA32_1(e) NERF_MFMA(NERF_OP32, "c00", "w" e, "x" e)
+#define NERF_MFMA32_2(e) NERF_MFMA(NERF_OP32, "c00", "w" e, "x" e) NERF_MFMA(NERF_OP32, "c10", "w" e, "y" e)
+#define NERF_IN4(n, v) [n##0] "v"(v[0]), [n##1] "v"(v[1]), [n##2] "v"(v[2]), [n##3] "v"(v[3])
+template <int MI, int NJ, typename F>
+__device__ __forceinline__ void block_nt(float, f32x16 (&c)[MI][NJ], F (&x)[MI], F (&w)[NJ], unsigned pa, unsigned pb) {
+    static_assert(NJ == 1, "fp32 tiles are one output tile wide per wave");
+    F nx[MI], nw[NJ];
+    if constexpr (MI == 2)
+        asm volatile(NERF_BLOCK_HEAD NERF_READ_X2 NERF_READ_W1 NERF_MFMA32_2("0") NERF_MFMA32_2("1") NERF_MFMA32_2("2") NERF_MFMA32_2("3") NERF_BLOCK_TAIL
+                     : [c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]), [nx0] "=&v"(nx[0]), [nx1] "=&v"(nx[1]), [nw0] "=&v"(nw[0])
+                     : NERF_IN4(x, x[0]), NERF_IN4(y, x[1]), NERF_IN4(w, w[0]), [pa] "v"(pa), [pb] "v"(pb)
+                     : "memory");
+    else
+        asm volatile(NERF_BLOCK_HEAD NERF_READ_X1 NERF_READ_W1 NERF_MFMA32_1("0") NERF_MFMA32_1("1") NERF_MFMA32_1("2") NERF_MFMA32_1("3") NERF_BLOCK_TAIL
+                     : [c00] "+v"(c[0][0]), [nx0] "=&v"(nx[0]), [nw0] "=&v"(nw[0])
+                     : NERF_IN4(x, x[0]), NERF_IN4(w, w[0]), [pa] "v"(pa), [pb] "v"(pb)
+                     : "memory");
+    for (int i = 0; i < MI; ++i) x[i] = nx[i];
+    w[0] = nw[0];
+}
+#define NERF_READ_B4 "ds_read_b32 %[n0], %[p0]\n\tds_read_b32 %[n1], %[p0] offset:%[row1]\n\tds_read_b32 %[n2], %[p0] offset:%[row2]\n\tds_read_b32 %[n3], %[p0] offset:%[row3]\n\t"
+template <int PITCH, int MI, int NJ, int NP, typename F>
+__device__ __forceinline__ void block_tr(float, f32x16 (&c)[MI][NJ], F (&x)[MI], F (&w)[NJ], unsigned pa, const unsigned (&pb)[NP], unsigned stage) {
+    static_assert(NJ == 1 && NP == 1, "fp32 tiles are one output tile wide per wave");
+    F nx[MI];
+    float n0, n1, n2, n3;
+    if constexpr (MI == 2)
+        asm volatile(NERF_BLOCK_HEAD NERF_READ_X2 NERF_READ_B4 NERF_MFMA32_2("0") NERF_MFMA32_2("1") NERF_MFMA32_2("2") NERF_MFMA32_2("3") NERF_BLOCK_TAIL
+                     : [c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]), [nx0] "=&v"(nx[0]), [nx1] "=&v"(nx[1]), [n0] "=&v"(n0), [n1] "=&v"(n1),
+                       [n2] "=&v"(n2), [n3] "=&v"(n3)
+                     : NERF_IN4(x, x[0]), NERF_IN4(y, x[1]), NERF_IN4(w, w[0]), [pa] "v"(pa), [p0] "v"(pb[0] + stage), [row1] "n"(PITCH),
+                       [row2] "n"(2 * PITCH), [row3] "n"(3 * PITCH)
+                     : "memory");
+    else
+        asm volatile(NERF_BLOCK_HEAD NERF_READ_X1 NERF_READ_B4 NERF_MFMA32_1("0") NERF_MFMA32_1("1") NERF_MFMA32_1("2") NERF_MFMA32_1("3") NERF_BLOCK_TAIL
+                     : [c00] "+v"(c[0][0]), [nx0] "=&v"(nx[0]), [n0] "=&v"(n0), [n1] "=&v"(n1), [n2] "=&v"(n2), [n3] "=&v"(n3)
+                     : NERF_IN4(x, x[0]), NERF_IN4(w, w[0]), [pa] "v"(pa), [p0] "v"(pb[0] + stage), [row1] "n"(PITCH), [row2] "n"(2 * PITCH),
+                       [row3] "n"(3 * PITCH)
+                     : "memory");
+    for (int i = 0; i < MI; ++i) x[i] = nx[i];
+    w[0] = F{n0, n1, n2, n3};
+}
+
+template <typename T, bool WT, bool GATE, int BN>
+__global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
+    constexpr int E = piece<T>(), BK = step_len<T>(), WAVES = ST_THREADS / 64;
+    constexpr int WM = BN == 64 ? 4 : 2, WO = WAVES / WM;                   // waves along rows and outputs
+    constexpr int MI = TILE_ROWS / WM / 32, NJ = BN / WO / 32;
+    constexpr int A_BYTES = TILE_ROWS * 128, B_BYTES = WT ? tr_bytes<T, BN>() : BN * 128, Y_BYTES = GATE ? A_BYTES : 0;
+    constexpr int STAGE = A_BYTES + B_BYTES + Y_BYTES;
+    constexpr int NA = A_BYTES / 1024 / WAVES, NB = B_BYTES / 1024 / WAVES; // copies of a wave per step
+    constexpr int COPIES = NA + NB + (GATE ? NA : 0);
+    constexpr int STORES = MI * NJ * (sizeof(T) == 2 ? 2 : 4);              // stores of a wave per item
+    static_assert(COPIES + 2 * STORES < 64, "vmcnt counts to 63");
+    __shared__ __attribute__((aligned(1024))) char lds[3 * STAGE];
+    __shared__ int row_tab[ST_ITEMS][TILE_ROWS];
+    __shared__ __attribute__((aligned(16))) T bias_tab[ST_ITEMS][BN];
+    __shared__ int d_grp[ST_ITEMS], d_o0[ST_ITEMS], d_cnt[ST_ITEMS], d_pos[ST_ITEMS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m_off = (wave % WM) * (MI * 32), o_off = (wave / WM) * (NJ * 32);
+    const int G = p.rows.n_groups, O = p.O, C = p.C;
+    const int nk = (C + BK - 1) / BK;
+    T* out = (T*)p.out;
+    const float least = p.relu ? 0.0f : -__builtin_inff();
+    const unsigned bits = p.relu ? 0x7fffffffu : 0xffffffffu;
+    typedef __attribute__((address_space(3))) char* lds_ptr;
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr)lds, rows0 = (unsigned)(uintptr_t)(lds_ptr)row_tab, bias0 = (unsigned)(uintptr_t)(lds_ptr)bias_tab;
+
+    // An XCD takes a run of consecutive items and deals them to its workgroups in turn, so that the output tiles of the same
+    // rows are worked on at the same time and the rows come from memory once (in runs per workgroup, 1024 outputs of 65 536
+    // rows fetched the rows four times).
+    const Tables tables(p.rows, lane);
+    const int64_t work = (int64_t)tables.total * p.tiles_o, xcd = blockIdx.x & 7;
+    const int64_t begin = work * xcd / 8 + (blockIdx.x >> 3), finish = work * (xcd + 1) / 8, stride = gridDim.x >> 3;
+
+    // Copy i of wave w fills LDS slots (w n + i) 64 + lane of its tile; the lane picks the row and the piece that belong there.
+    int a_row[NA], a_q[NA], b_row[NB], b_q[NB];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+        const int slot = (wave * NA + i) * 64 + lane;
+        a_row[i] = slot >> 3;
+        a_q[i] = (slot & 7) ^ ((a_row[i] >> 1) & 7);
+    }
+    constexpr int BPR = BN / E;                                             // pieces per row of a transposed W tile
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int slot = (wave * NB + i) * 64 + lane;
+        b_row[i] = WT ? slot / BPR : slot >> 3;
+        b_q[i] = WT ? (slot % BPR) ^ tr_swap<T, BN>(b_row[i]) : (slot & 7) ^ ((b_row[i] >> 1) & 7);
+    }
+    // LDS addresses of this lane's fragments within a stage, by product step
+    unsigned fa[ROW_PIECES / 2], fb[ROW_PIECES / 2][WT ? NJ : 1];
+#pragma unroll
+    for (int s = 0; s < ROW_PIECES / 2; ++s) {
+        fa[s] = lds0 + nt_addr(m_off + (lane & 31), 2 * s + (lane >> 5));
+        if constexpr (!WT) {
+            fb[s][0] = lds0 + A_BYTES + nt_addr(o_off + (lane & 31), 2 * s + (lane >> 5));
+        } else {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) fb[s][j] = lds0 + A_BYTES + tr_lane<T, BN>(o_off + 32 * j, s, lane);
+        }
+    }
+
+    for (int64_t first = begin; first < finish; first += ST_ITEMS * stride) {
+        const int64_t left = (finish - first + stride - 1) / stride;
+        const int items = (int)(left < ST_ITEMS ? left : ST_ITEMS);
+        __syncthreads();
+        for (int i = wave; i < items; i += WAVES) {
+            const Tile t = tables.tile(p.rows, first + i * stride, p.tiles_o, BN);
+            if (lane == 0) { d_grp[i] = t.group; d_o0[i] = t.o0; d_cnt[i] = t.count; d_pos[i] = (int)t.pos0; }
+        }
+        __syncthreads();
+#pragma unroll 3
+        for (int j = tid; j < items * TILE_ROWS; j += ST_THREADS) {
+            const int i = j / TILE_ROWS, row = p.rows.order[d_pos[i] + min(j % TILE_ROWS, d_cnt[i] - 1)];
+            row_tab[0][j] = min(max(row, 0), (int)p.rows.n - 1);
+        }
+        if (p.bias) {
+#pragma unroll 3
+            for (int j = tid; j < items * BN; j += ST_THREADS) {
+                const int i = j / BN, o = d_o0[i] + j % BN, g = min(d_grp[i], G - 1);
+                bias_tab[0][j] = ((const T*)p.bias)[(int64_t)g * O + (o < O ? o : O - E + o % E)];
+            }
+        } else {
+            for (int j = tid; j < items * BN; j += ST_THREADS) bias_tab[0][j] = (T)0.0f;
+        }
+        __syncthreads();
+        int real = items;                                                   // the rows of no group come last
+        while (real > 0 && d_grp[real - 1] == G) --real;
+        for (int i = real; i < items; ++i) {
+            const int o0 = d_o0[i], pieces = (O - o0 < BN ? O - o0 : BN) / E;
+            Pack<T, E> zero;
+#pragma unroll
+            for (int e = 0; e < E; ++e) zero.v[e] = (T)0.0f;
+            for (int j = tid; j < d_cnt[i] * pieces; j += ST_THREADS)
+                store_pack<T, E>(out + (int64_t)row_tab[i][j / pieces] * O + o0 + (j % pieces) * E, zero);
+        }
+        const int steps = real * nk;
+        if (steps == 0) continue;
+
+        // ---- copies: step c_k of item c_item into buffer c_buf ----
+        int c_item = 0, c_k = 0, c_buf = 0;
+        const T *pa[NA], *py[GATE ? NA : 1], *pb[NB];
+        auto copy_step = [&]() {
+            if (c_k == 0) {
+                const int g = __builtin_amdgcn_readfirstlane(lds_int((unsigned)(uintptr_t)(lds_ptr)&d_grp[c_item]));
+                const int o0 = __builtin_amdgcn_readfirstlane(lds_int((unsigned)(uintptr_t)(lds_ptr)&d_o0[c_item]));
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    const int64_t row = lds_int(rows0 + (c_item * TILE_ROWS + a_row[i]) * 4);
+                    pa[i] = (const T*)p.a + row * p.a_ld + a_q[i] * E;
+                    if constexpr (GATE) py[i] = (const T*)p.gate + row * C + a_q[i] * E;
+                }
+                const T* w = (const T*)p.w + (int64_t)g * O * C;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    if constexpr (WT) {
+                        const int o = o0 + b_q[i] * E;
+                        pb[i] = w + (int64_t)b_row[i] * O + (o < O ? o : O - E);
+                    } else {
+                        const int o = o0 + b_row[i];
+                        pb[i] = w + (int64_t)(o < O ? o : O - E + o % E) * C + b_q[i] * E;
+                    }
+                }
+            }
+            char* const to = lds + c_buf * STAGE + wave * (NA * 1024);
+            char* const to_b = lds + c_buf * STAGE + A_BYTES + wave * (NB * 1024);
+            const int k0 = c_k * BK;
+            if (k0 + BK <= C) {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) copy_piece(pa[i], to + i * 1024);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) copy_piece(pb[i], to_b + i * 1024);
+                if constexpr (GATE)
+#pragma unroll
+                    for (int i = 0; i < NA; ++i) copy_piece(py[i], to + A_BYTES + B_BYTES + i * 1024);
+            } else {                                                        // what lies behind the sum is read as zero
+#pragma unroll
+                for (int i = 0; i < NA; ++i) copy_piece(k0 + a_q[i] * E < C ? (const void*)pa[i] : (const void*)&ZERO_PIECE, to + i * 1024);
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+                    copy_piece(k0 + (WT ? b_row[i] : b_q[i] * E) < C ? (const void*)pb[i] : (const void*)&ZERO_PIECE, to_b + i * 1024);
+                if constexpr (GATE)
+#pragma unroll
+                    for (int i = 0; i < NA; ++i)
+                        copy_piece(k0 + a_q[i] * E < C ? (const void*)py[i] : (const void*)&ZERO_PIECE, to + A_BYTES + B_BYTES + i * 1024);
+            }
+            if (c_item * nk + c_k + 1 < steps) {
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    pa[i] += BK;
+                    if constexpr (GATE) py[i] += BK;
+                }
+#pragma unroll
+                for (int i = 0; i < NB; ++i) pb[i] += WT ? (int64_t)BK * O : BK;
+            }
+            // behind the last step the last one is copied again, into a buffer that nothing reads any more
+            if (c_item * nk + c_k + 1 < steps && ++c_k == nk) { c_k = 0; ++c_item; }
+            c_buf = c_buf == 2 ? 0 : c_buf + 1;
+        };
+        f32x16 acc[MI][NJ];
+        auto clear = [&]() {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        };
+        auto multiply = [&](unsigned stage) {
+#pragma unroll
+            for (int s = 0; s < ROW_PIECES / 2; ++s) {
+                typename El<T>::frag fx[MI], fw[NJ];
+                if constexpr (!WT) {
+                    read_nt<typename El<T>::frag, MI, NJ>(fx, fw, fa[s] + stage, fb[s][0] + stage);
+                } else {
+                    read_rows<typename El<T>::frag, MI>(fx, fa[s] + stage);
+                    if constexpr (GATE) {
+                        typename El<T>::frag fy[MI];
+                        read_rows<typename El<T>::frag, MI>(fy, fa[s] + stage + A_BYTES + B_BYTES);
+#pragma unroll
+                        for (int i = 0; i < MI; ++i) fx[i] = gate_frag<T>(fx[i], fy[i]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        fw[j] = read_tr<T, BN * (int)sizeof(T)>(fb[s][j] + stage);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = El<T>::mfma(fw[j], fx[i], acc[i][j]);
+            }
+        };
+        auto finish_item = [&](int item) {
+            const int o0 = __builtin_amdgcn_readfirstlane(lds_int((unsigned)(uintptr_t)(lds_ptr)&d_o0[item])) + o_off;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                const int64_t row = lds_int(rows0 + (item * TILE_ROWS + m_off + 32 * i + (lane & 31)) * 4);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    float z[16];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const unsigned at = bias0 + (item * BN + o_off + 32 * j + 8 * h + 4 * (lane >> 5)) * (int)sizeof(T);
+                        float b[4];
+                        if constexpr (sizeof(T) == 2) {
+                            uint2 v;
+                            asm volatile("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(at) : "memory");
+                            const Pack<T, 4> q = __builtin_bit_cast(Pack<T, 4>, v);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) b[e] = (float)q.v[e];
+                        } else {
+                            const f32x4 q = lds_quad(at);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) b[e] = q[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float v = acc[i][j][4 * h + e] + b[e];
+                            z[4 * h + e] = relu_or_not(v, least, bits);
+                        }
+                    }
+                    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                        for (int h = 0; h < 4; h += 2) {
+                            unsigned x[2], y[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                Pack<T, 2> u, v;
+                                u.v[0] = (T)z[4 * h + 2 * e]; u.v[1] = (T)z[4 * h + 2 * e + 1];
+                                v.v[0] = (T)z[4 * h + 4 + 2 * e]; v.v[1] = (T)z[4 * h + 4 + 2 * e + 1];
+                                const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, u), __builtin_bit_cast(unsigned, v), false, false);
+                                x[e] = sw[0];
+                                y[e] = sw[1];
+                            }
+                            int o = o0 + 32 * j + 8 * h + 8 * (lane >> 5);
+                            o = o < O ? o : O - E;
+                            *reinterpret_cast<uint4*>(out + row * O + o) = make_uint4(x[0], x[1], y[0], y[1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            int o = o0 + 32 * j + 8 * h + 4 * (lane >> 5);
+                            o = o < O ? o : O - E;
+                            *reinterpret_cast<float4*>(out + row * O + o) = make_float4(z[4 * h], z[4 * h + 1], z[4 * h + 2], z[4 * h + 3]);
+                        }
+                    }
+                }
+            }
+        };
+
+        wait_copies<0>();                                                   // stores of the last round of items
+        clear();
+        int item = 0, k = 0, buf = 0, late = 0;                             // late: bit 0 / 1: stores behind the newest / the other copies
+        auto wait_step = [&]() {
+            if (late == 0) wait_copies<COPIES>();
+            else if (late == 3) wait_copies<COPIES + 2 * STORES>();
+            else wait_copies<COPIES + STORES>();
+            __builtin_amdgcn_s_barrier();
+            late = (late << 1) & 3;
+        };
+        auto end_step = [&]() {
+            if (++k == nk) {
+                if constexpr (!GATE) settle<T, MI, NJ>(acc);
+                finish_item(item);
+                clear();
+                k = 0;
+                ++item;
+                late |= 1;
+            }
+        };
+        copy_step();
+        copy_step();
+        if constexpr (GATE) {
+            // the gate stands between reading a fragment and multiplying it, so nothing is read ahead
+            for (int s = 0; s < steps; ++s) {
+                wait_step();
+                copy_step();
+                multiply(buf * STAGE);
+                end_step();
+                buf = buf == 2 ? 0 : buf + 1;
+            }
+        } else {
+            // The last fragments of a step are in registers one product step before its end: there the barrier frees its
+            // buffer for step s + 3 and the first fragments of step s + 1 are requested.
+            constexpr int S = ROW_PIECES / 2;
+            typename El<T>::frag fx[MI], fw[NJ];
+            copy_step();
+            wait_copies<2 * COPIES>();
+            __builtin_amdgcn_s_barrier();
+            if constexpr (!WT) {
+                read_nt<typename El<T>::frag, MI, NJ>(fx, fw, fa[0], fb[0][0]);
+            } else {
+                read_rows<typename El<T>::frag, MI>(fx, fa[0]);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    fw[j] = read_tr<T, BN * (int)sizeof(T)>(fb[0][j]);
+                }
+            }
+            for (int s = 0; s < steps; ++s) {
+#pragma unroll
+                for (int u = 0; u < S; ++u) {
+                    unsigned stage = buf * STAGE;
+                    if (u == S - 1) {
+                        wait_step();
+                        buf = buf == 2 ? 0 : buf + 1;
+                        stage = buf * STAGE;
+                    }
+                    const int n = (u + 1) % S;
+                    if constexpr (!WT) block_nt<MI, NJ>(T(), acc, fx, fw, fa[n] + stage, fb[n][0] + stage);
+                    else block_tr<BN * (int)sizeof(T)>(T(), acc, fx, fw, fa[n] + stage, fb[n], stage);
+                }
+                copy_step();                                                // beside the last products
+                end_step();
+            }
+        }
+        wait_copies<0>();                                                   // nothing may land once the rows are written anew
+    }
+}
+
+// ---- through registers: any row length, any alignment ------------------------------------------------------------
+// The same product, one workgroup of four waves per tile of 128 rows x BN outputs.  Pieces are put together element by
+// element; a step is requested before the products of the one before it.
+template <typename T, bool WT, bool GATE, int BN>
 __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();
     constexpr int A_BYTES = TILE_ROWS * 128;
-    constexpr int B_BYTES = WT ? tr_bytes<T>() : BN * 128;
-    constexpr int STAGE = A_BYTES + B_BYTES;
+    constexpr int B_BYTES = WT ? tr_bytes<T, BN>() : BN * 128;
     constexpr int PITCH = BN * 2 + 16;                                      // 16-bit output tile in LDS
-    constexpr int LDS = 2 * STAGE > TILE_ROWS * PITCH ? 2 * STAGE : TILE_ROWS * PITCH;
+    constexpr int LDS = sizeof(T) == 2 && TILE_ROWS * PITCH > A_BYTES + B_BYTES ? TILE_ROWS * PITCH : A_BYTES + B_BYTES;
     __shared__ __attribute__((aligned(16))) char lds[LDS];
     __shared__ int row_of[TILE_ROWS];
     constexpr int MI = BN == 128 ? 2 : 1, NJ = 2;                           // 32-row and 32-output tiles of a wave
@@ -157,97 +752,74 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
     const int m_off = BN == 128 ? (wave & 1) * 64 : wave * 32, o_off = BN == 128 ? (wave >> 1) * 64 : 0;
 
     // consecutive tiles on one XCD (workgroups go round the eight XCDs), output tiles of the same rows next to each other
-    const int G = p.rows.n_groups;
-    const int64_t work = (int64_t)p.rows.tile_base[G + 1] * p.tiles_o;
-    const int64_t per_xcd = (work + 7) / 8;
-    const int64_t local = blockIdx.x >> 3;
+    const Tables tables(p.rows, lane);
+    const int64_t work = (int64_t)tables.total * p.tiles_o;
+    const int64_t per_xcd = (work + 7) / 8, local = blockIdx.x >> 3;
     const int64_t at = (blockIdx.x & 7) * per_xcd + local;
     if (local >= per_xcd || at >= work) return;
-    const int t = (int)(at / p.tiles_o), o0 = (int)(at % p.tiles_o) * BN;
-    const int g = grp::group_of_tile(p.rows.tile_base, G, t, lane);
-    const int64_t pos0 = p.rows.offsets[g] + (int64_t)(t - p.rows.tile_base[g]) * TILE_ROWS;
-    const int64_t end = g < G ? (int64_t)p.rows.offsets[g + 1] : p.rows.n;
-    const int count = (int)(end - pos0 < TILE_ROWS ? end - pos0 : TILE_ROWS);
-    if (tid < TILE_ROWS) row_of[tid] = tid < count ? row_at(p.rows, pos0 + tid) : -1;
+    const Tile t = tables.tile(p.rows, at, p.tiles_o, BN);
+    const int g = t.group, o0 = t.o0;
+    if (tid < TILE_ROWS) row_of[tid] = tid < t.count ? row_at(p.rows, t.pos0 + tid) : -1;
     __syncthreads();
     T* out = (T*)p.out;
     const int O = p.O, C = p.C;
-    if (g == G) {                                                           // rows of no group
+    if (g == p.rows.n_groups) {                                             // rows of no group
         const int width = O - o0 < BN ? O - o0 : BN;
-        for (int i = tid; i < count * width; i += THREADS) {
+        for (int i = tid; i < t.count * width; i += THREADS) {
             const int row = row_of[i / width];
             if (row >= 0) out[(int64_t)row * O + o0 + i % width] = (T)0.0f;
         }
         return;
     }
-
     const T* w = (const T*)p.w + (int64_t)g * O * C;
-    // pieces of this thread: rows tid / 8 + 32 i of A (and of W), piece tid % 8
-    const int q = tid & 7, r0 = tid >> 3;
-    const T *arow[4], *yrow[4];
-    bool aok[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = row_of[r0 + 32 * i];
-        aok[i] = row >= 0;
-        arow[i] = (const T*)p.a + (int64_t)(row < 0 ? 0 : row) * p.a_ld;
-        if (GATE) yrow[i] = (const T*)p.gate + (int64_t)(row < 0 ? 0 : row) * C;
-    }
+    char* const A = lds;
+    char* const B = lds + A_BYTES;
     constexpr int BPR = BN / E;                                             // pieces per row of a transposed W tile
-    constexpr int NB = WT ? BK * BPR / THREADS : BN / 32;
-    Pack<T, E> ra[4], rb[NB];
-    auto load = [&](int k0) {
+    constexpr int NA = TILE_ROWS * 8 / THREADS, NB = B_BYTES / 16 / THREADS;
+    const int q = tid & 7, r0 = tid >> 3;
+    int rows[NA];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ra[i] = load_piece<T, WIDE>(arow[i], k0 + q * E, C, aok[i]);
-            if (GATE) {
-                const Pack<T, E> y = load_piece<T, WIDE>(yrow[i], k0 + q * E, C, aok[i]);
+    for (int i = 0; i < NA; ++i) rows[i] = row_of[r0 + 32 * i];
+    Pack<T, E> ra[NA], rb[NB];
+    auto fill = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int64_t row = rows[i] < 0 ? 0 : rows[i];
+            ra[i] = load_piece<T>((const T*)p.a + row * p.a_ld, k0 + q * E, C, rows[i] >= 0);
+            if constexpr (GATE) {
+                const Pack<T, E> y = load_piece<T>((const T*)p.gate + row * C, k0 + q * E, C, rows[i] >= 0);
                 gate_piece<T, E>(ra[i], y);
             }
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             if constexpr (WT) {
-                const int c = k0 + tid / BPR + (THREADS / BPR) * i;
-                rb[i] = load_piece<T, WIDE>(w + (int64_t)c * O, o0 + (tid % BPR) * E, O, c < C);
+                const int c = k0 + (tid + i * THREADS) / BPR;
+                rb[i] = load_piece<T>(w + (int64_t)c * O, o0 + (tid + i * THREADS) % BPR * E, O, c < C);
             } else {
                 const int o = o0 + r0 + 32 * i;
-                rb[i] = load_piece<T, WIDE>(w + (int64_t)o * C, k0 + q * E, C, o < O);
+                rb[i] = load_piece<T>(w + (int64_t)o * C, k0 + q * E, C, o < O);
             }
         }
     };
-    auto put = [&](int buf) {
-        char* A = lds + buf * STAGE;
-        char* B = A + A_BYTES;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) put_piece<T, E>(A + nt_addr(r0 + 32 * i, q), ra[i]);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            if constexpr (WT) put_piece<T, E>(B + tr_addr<T>(tid / BPR + (THREADS / BPR) * i, tid % BPR), rb[i]);
-            else put_piece<T, E>(B + nt_addr(r0 + 32 * i, q), rb[i]);
-        }
-    };
-
     f32x16 acc[MI][NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        f32x16 b0;
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int o = o0 + o_off + 32 * j + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-            b0[r] = p.bias && o < O ? (float)((const T*)p.bias)[(int64_t)g * O + o] : 0.0f;
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    fill(0);
+    for (int k0 = 0; k0 < C; k0 += BK) {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) put_piece<T, E>(A + nt_addr(r0 + 32 * i, q), ra[i]);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            if constexpr (WT) put_piece<T, E>(B + tr_addr<T, BN>((tid + i * THREADS) / BPR, (tid + i * THREADS) % BPR), rb[i]);
+            else put_piece<T, E>(B + nt_addr(r0 + 32 * i, q), rb[i]);
         }
-#pragma unroll
-        for (int i = 0; i < MI; ++i) acc[i][j] = b0;
-    }
-    const int steps = (C + BK - 1) / BK;
-    load(0);
-    put(0);
-    __syncthreads();
-    for (int k = 0; k < steps; ++k) {
-        if (k + 1 < steps) load((k + 1) * BK);
-        const char* A = lds + (k & 1) * STAGE;
-        const char* B = A + A_BYTES;
+        __syncthreads();
+        if (k0 + BK < C) fill(k0 + BK);
 #pragma unroll
         for (int s = 0; s < ROW_PIECES / 2; ++s) {
             typename El<T>::frag fx[MI], fw[NJ];
@@ -255,7 +827,7 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
             for (int i = 0; i < MI; ++i) fx[i] = nt_frag<T>(A, m_off + 32 * i, s, lane);
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                if constexpr (WT) fw[j] = tr_frag<T>(B, o_off + 32 * j, s, lane);
+                if constexpr (WT) fw[j] = tr_frag<T, BN>(B, o_off + 32 * j, s, lane);
                 else fw[j] = nt_frag<T>(B, o_off + 32 * j, s, lane);
             }
 #pragma unroll
@@ -263,19 +835,30 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) acc[i][j] = El<T>::mfma(fw[j], fx[i], acc[i][j]);
         }
-        if (k + 1 < steps) put((k + 1) & 1);
-        __syncthreads();
+        __syncthreads();                                                    // every wave has read the step
     }
-    if (p.relu) {
+
+    // bias, ReLU, and the rows back to where they belong
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+        for (int h = 0; h < 4; ++h) {
+            const int o = o0 + o_off + 32 * j + 8 * h + 4 * (lane >> 5);
+            float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.bias)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = acc[i][j][r] < 0.0f ? 0.0f : acc[i][j][r];   // keeps a NaN
-    }
+                for (int e = 0; e < 4; ++e) b[e] = o + e < O ? (float)((const T*)p.bias)[(int64_t)g * O + o + e] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float z = acc[i][j][4 * h + e] + b[e];
+                    if (p.relu) z = z < 0.0f ? 0.0f : fabsf(z);             // keeps a NaN, without its sign
+                    acc[i][j][4 * h + e] = z;
+                }
+        }
     if constexpr (sizeof(T) == 2) {
-        // through LDS, so that rows leave in 16-byte pieces of whole lines
+        // through LDS, so that a wave stores neighbouring outputs of a row together
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -288,18 +871,10 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
                     put_piece<T, 4>(lds + (m_off + 32 * i + (lane & 31)) * PITCH + (o_off + 32 * j + 8 * h + 4 * (lane >> 5)) * 2, v);
                 }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < TILE_ROWS * BN / E / THREADS; ++i) {
-            const int at2 = tid + i * THREADS, m = at2 / (BN / E), c = (at2 % (BN / E)) * E;
-            const int row = row_of[m];
-            if (row < 0 || o0 + c >= O) continue;
-            const Pack<T, E> v = *reinterpret_cast<const Pack<T, E>*>(lds + m * PITCH + c * 2);
-            T* to = out + (int64_t)row * O + o0 + c;
-            if constexpr (WIDE) store_pack<T, E>(to, v);
-            else
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (o0 + c + e < O) to[e] = v.v[e];
+#pragma unroll 4
+        for (int i = tid; i < TILE_ROWS * BN; i += THREADS) {
+            const int m = i / BN, c = i % BN, row = row_of[m];
+            if (row >= 0 && o0 + c < O) out[(int64_t)row * O + o0 + c] = *reinterpret_cast<const T*>(lds + m * PITCH + c * 2);
         }
     } else {
 #pragma unroll
@@ -309,16 +884,9 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const int o = o0 + o_off + 32 * j + 8 * h + 4 * (lane >> 5);
-                    T* to = out + (int64_t)row * O + o;
-                    if constexpr (WIDE) {
-                        if (o < O) store_pack<float, 4>((float*)to, Pack<float, 4>{{acc[i][j][4 * h], acc[i][j][4 * h + 1], acc[i][j][4 * h + 2], acc[i][j][4 * h + 3]}});
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (o + e < O) to[e] = (T)acc[i][j][4 * h + e];
-                    }
+                for (int r = 0; r < 16; ++r) {
+                    const int o = o0 + o_off + 32 * j + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                    if (o < O) out[(int64_t)row * O + o] = (T)acc[i][j][r];
                 }
         }
     }
@@ -334,16 +902,294 @@ struct WgradArgs {
     float *part_w, *part_b;          // [2 * chunks][N * K], [2 * chunks][N]: slot 2c a group that came in from the left of
 };                                   // chunk c, slot 2c + 1 one that began in it and goes on to the right
 
+// dW[n][k] = sum over rows dZ[row][n] x[row][k], streaming form.  A workgroup of eight waves owns one BD x BX block of every
+// dW it meets and walks `chunk` consecutive tiles of the flat tile list, whatever groups they belong to, so all workgroups
+// have equal work however uneven the groups are.  A group that lies inside one chunk is finished here; the pieces of a longer
+// one go to the workspace and are added up in order by wgrad_join_kernel (no atomics: the result does not depend on timing).
+//
+// Rows of both operands (and of the layer's output, when it gates) are copied as they are into a ring of three LDS buffers,
+// as in stream_kernel; a row behind the end of a tile is read from a piece of zeros.  The sum of dZ over the rows comes from
+// the fragments: the four waves that share a range of n take one product step of four each.
+constexpr int WG_TILES = 24;            // tiles whose rows are in LDS at a time
+
+#define NERF_WG_BLOCK(T, OP)                                                                                                            \
+    template <int PD, int PX, int NJ, typename F>                                                                                       \
+    __device__ __forceinline__ void block_wgrad(T, f32x16 (&c)[2][NJ], F (&d)[2], F (&x)[NJ], unsigned d0, unsigned d1, unsigned x0,    \
+                                                unsigned x1) {                                                                          \
+        struct Two { s16x4 lo, hi; } nd[2], nx[NJ];                                                                                     \
+        if constexpr (NJ == 2)                                                                                                          \
+            asm volatile(NERF_BLOCK_HEAD NERF_READ_TRD("l0", "h0", "d0") NERF_READ_TRX("l2", "h2", "x0") NERF_READ_TRD("l1", "h1", "d1") \
+                         NERF_READ_TRX("l3", "h3", "x1") NERF_MFMA(OP, "c00", "e0", "f0") NERF_MFMA(OP, "c01", "e0", "f1")              \
+                         NERF_MFMA(OP, "c10", "e1", "f0") NERF_MFMA(OP, "c11", "e1", "f1") NERF_BLOCK_TAIL                              \
+                         : [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1]), [l0] "=&v"(nd[0].lo),    \
+                           [h0] "=&v"(nd[0].hi), [l1] "=&v"(nd[1].lo), [h1] "=&v"(nd[1].hi), [l2] "=&v"(nx[0].lo), [h2] "=&v"(nx[0].hi), \
+                           [l3] "=&v"(nx[1].lo), [h3] "=&v"(nx[1].hi)                                                                   \
+                         : [e0] "v"(d[0]), [e1] "v"(d[1]), [f0] "v"(x[0]), [f1] "v"(x[1]), [d0] "v"(d0), [d1] "v"(d1), [x0] "v"(x0),    \
+                           [x1] "v"(x1), [rowsd] "n"(4 * PD), [rowsx] "n"(4 * PX)                                                       \
+                         : "memory");                                                                                                   \
+        else                                                                                                                            \
+            asm volatile(NERF_BLOCK_HEAD NERF_READ_TRD("l0", "h0", "d0") NERF_READ_TRX("l2", "h2", "x0") NERF_READ_TRD("l1", "h1", "d1") \
+                         NERF_MFMA(OP, "c00", "e0", "f0") NERF_MFMA(OP, "c10", "e1", "f0") NERF_BLOCK_TAIL                              \
+                         : [c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]), [l0] "=&v"(nd[0].lo), [h0] "=&v"(nd[0].hi), [l1] "=&v"(nd[1].lo),  \
+                           [h1] "=&v"(nd[1].hi), [l2] "=&v"(nx[0].lo), [h2] "=&v"(nx[0].hi)                                             \
+                         : [e0] "v"(d[0]), [e1] "v"(d[1]), [f0] "v"(x[0]), [d0] "v"(d0), [d1] "v"(d1), [x0] "v"(x0),                    \
+                           [rowsd] "n"(4 * PD), [rowsx] "n"(4 * PX)                                                                     \
+                         : "memory");                                                                                                   \
+        for (int i = 0; i < 2; ++i) d[i] = __builtin_bit_cast(F, nd[i]);                                                                \
+        for (int j = 0; j < NJ; ++j) x[j] = __builtin_bit_cast(F, nx[j]);                                                               \
+    }
+#define NERF_READ_TRD(lo, hi, at) "ds_read_b64_tr_b16 %[" lo "], %[" at "]\n\tds_read_b64_tr_b16 %[" hi "], %[" at "] offset:%[rowsd]\n\t"
+#define NERF_READ_TRX(lo, hi, at) "ds_read_b64_tr_b16 %[" lo "], %[" at "]\n\tds_read_b64_tr_b16 %[" hi "], %[" at "] offset:%[rowsx]\n\t"
+NERF_WG_BLOCK(__bf16, "v_mfma_f32_32x32x16_bf16")
+NERF_WG_BLOCK(_Float16, "v_mfma_f32_32x32x16_f16")
+#undef NERF_WG_BLOCK
+
+template <typename T, bool GATE, int BX>
+__global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
+    constexpr int E = piece<T>(), BK = step_len<T>(), WAVES = ST_THREADS / 64, BD = 128;
+    constexpr bool AHEAD = sizeof(T) == 2 && !GATE;                         // fragments read one product step ahead
+    constexpr int PER_TILE = TILE_ROWS / BK, S = ROW_PIECES / 2;
+    constexpr int MI = 2, NJ = BX / 4 / 32;                                 // waves: 2 along n, 4 along k
+    constexpr int D_BYTES = tr_bytes<T, BD>(), X_BYTES = tr_bytes<T, BX>(), Y_BYTES = GATE ? D_BYTES : 0;
+    constexpr int STAGE = D_BYTES + X_BYTES + Y_BYTES;
+    constexpr int ND = D_BYTES / 1024 / WAVES, NX = X_BYTES / 1024 / WAVES;
+    constexpr int COPIES = ND + NX + (GATE ? ND : 0);
+    constexpr int DPR = BD / E, XPR = BX / E;                               // pieces of a row
+    __shared__ __attribute__((aligned(1024))) char lds[3 * STAGE];
+    __shared__ int row_tab[WG_TILES][TILE_ROWS];
+    __shared__ int tile_pos[WG_TILES], tile_cnt[WG_TILES], tile_grp[WG_TILES + 1];
+    __shared__ float red[4][BD];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n_off = (wave & 1) * 64, wk = wave >> 1, k_off = wk * (BX / 4);
+    typedef __attribute__((address_space(3))) char* lds_ptr;
+    const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr)lds, rows0 = (unsigned)(uintptr_t)(lds_ptr)row_tab, grp0 = (unsigned)(uintptr_t)(lds_ptr)tile_grp;
+
+    // the blocks of one chunk next to each other on one XCD: they read the same rows
+    const int G = p.rows.n_groups, K = p.K, N = p.N;
+    const int tiles = p.rows.tile_base[G];                                  // the rows of no group stay out
+    const int blocks = p.tiles_n * p.tiles_k;
+    const int64_t chunks = (tiles + p.chunk - 1) / p.chunk;
+    const int64_t per_xcd = (chunks + 7) / 8 * blocks, local = blockIdx.x >> 3;
+    const int64_t at = (blockIdx.x & 7) * per_xcd + local;
+    if (local >= per_xcd || at >= chunks * blocks) return;
+    const int c = (int)(at / blocks), blk = (int)(at % blocks);
+    const int n0 = (blk / p.tiles_k) * BD, k0 = (blk % p.tiles_k) * BX;
+    const int t0 = c * p.chunk, t1 = t0 + p.chunk < tiles ? t0 + p.chunk : tiles;
+
+    int d_row[ND], x_row[NX];
+    int64_t d_col[ND], x_col[NX];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+        const int slot = (wave * ND + i) * 64 + lane;
+        d_row[i] = slot / DPR;
+        const int col = n0 + ((slot % DPR) ^ tr_swap<T, BD>(d_row[i])) * E;
+        d_col[i] = col < N ? col : N - E;                                   // columns behind the last are not stored
+    }
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+        const int slot = (wave * NX + i) * 64 + lane;
+        x_row[i] = slot / XPR;
+        const int col = k0 + ((slot % XPR) ^ tr_swap<T, BX>(x_row[i])) * E;
+        x_col[i] = col < K ? col : K - E;
+    }
+    unsigned fd[S][MI], fx[S][NJ];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fd[s][i] = lds0 + tr_lane<T, BD>(n_off + 32 * i, s, lane);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fx[s][j] = lds0 + D_BYTES + tr_lane<T, BX>(k_off + 32 * j, s, lane);
+    }
+    f32x16 acc[MI][NJ];
+    float sum[MI];                                                          // of dZ over this lane's rows
+    auto clear = [&]() {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            sum[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        }
+    };
+    const bool bias = p.db && k0 == 0;
+    auto flush = [&](int g) {
+        const int b0 = p.rows.tile_base[g], b1 = p.rows.tile_base[g + 1];
+        const bool whole = b0 >= t0 && b1 <= t1;
+        const int64_t slot = 2 * (int64_t)c + (b0 >= t0 ? 1 : 0);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int n = n0 + n_off + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                if (n >= N) continue;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int k = k0 + k_off + 32 * j + (lane & 31);
+                    if (k >= K) continue;
+                    if (whole) ((T*)p.dw)[((int64_t)g * N + n) * K + k] = (T)acc[i][j][r];
+                    else p.part_w[(slot * N + n) * K + k] = acc[i][j][r];
+                }
+            }
+        if (bias) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                const float v = sum[i] + __shfl_xor(sum[i], 32, 64);
+                if (lane < 32) red[wk][n_off + 32 * i + lane] = v;
+            }
+            __syncthreads();
+            if (tid < BD && n0 + tid < N) {
+                const float v = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+                if (whole) ((T*)p.db)[(int64_t)g * N + n0 + tid] = (T)v;
+                else p.part_b[slot * N + n0 + tid] = v;
+            }
+            __syncthreads();
+        }
+        wait_copies<0>();                                                   // the counts of the steps to come have no stores in them
+    };
+    clear();
+
+    for (int first = t0; first < t1; first += WG_TILES) {
+        const int here = t1 - first < WG_TILES ? t1 - first : WG_TILES;
+        __syncthreads();
+        for (int i = tid; i <= here; i += ST_THREADS) {
+            const int t = first + i;
+            int lo = 0, hi = G;                                             // last group with tile_base <= t
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (p.rows.tile_base[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            tile_grp[i] = t < t1 ? lo : -1;                                 // of the tile behind the last one here too
+            if (i < here) {
+                const int64_t pos = p.rows.offsets[lo] + (int64_t)(t - p.rows.tile_base[lo]) * TILE_ROWS;
+                const int64_t left = p.rows.offsets[lo + 1] - pos;
+                tile_pos[i] = (int)pos;
+                tile_cnt[i] = (int)(left < TILE_ROWS ? left : TILE_ROWS);
+            }
+        }
+        __syncthreads();
+#pragma unroll 3
+        for (int j = tid; j < here * TILE_ROWS; j += ST_THREADS) {
+            const int i = j / TILE_ROWS, r = j % TILE_ROWS, cnt = tile_cnt[i];
+            const int row = p.rows.order[tile_pos[i] + (r < cnt ? r : 0)];
+            row_tab[0][j] = r < cnt && row >= 0 && row < p.rows.n ? row : -1;
+        }
+        __syncthreads();
+        const int steps = here * PER_TILE;
+        int c_step = 0, c_buf = 0;
+        auto copy_step = [&]() {
+            char* const to = lds + c_buf * STAGE;
+            const unsigned rows = rows0 + c_step * (BK * 4);
+            int rd[ND], rx[NX];
+            if constexpr (ND == 2 && NX == 4)
+                asm volatile("ds_read_b32 %0, %6\n\tds_read_b32 %1, %7\n\tds_read_b32 %2, %8\n\tds_read_b32 %3, %9\n\tds_read_b32 %4, %10\n\tds_read_b32 %5, %11\n\ts_waitcnt lgkmcnt(0)"
+                             : "=&v"(rd[0]), "=&v"(rd[1]), "=&v"(rx[0]), "=&v"(rx[1]), "=&v"(rx[2]), "=&v"(rx[3])
+                             : "v"(rows + d_row[0] * 4), "v"(rows + d_row[1] * 4), "v"(rows + x_row[0] * 4), "v"(rows + x_row[1] * 4),
+                               "v"(rows + x_row[2] * 4), "v"(rows + x_row[3] * 4) : "memory");
+            else
+                asm volatile("ds_read_b32 %0, %4\n\tds_read_b32 %1, %5\n\tds_read_b32 %2, %6\n\tds_read_b32 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+                             : "=&v"(rd[0]), "=&v"(rd[1]), "=&v"(rx[0]), "=&v"(rx[1])
+                             : "v"(rows + d_row[0] * 4), "v"(rows + d_row[1] * 4), "v"(rows + x_row[0] * 4), "v"(rows + x_row[1] * 4) : "memory");
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+                copy_piece(rd[i] >= 0 ? (const void*)((const T*)p.dy + rd[i] * p.dy_ld + d_col[i]) : (const void*)&ZERO_PIECE, to + (wave * ND + i) * 1024);
+#pragma unroll
+            for (int i = 0; i < NX; ++i)
+                copy_piece(rx[i] >= 0 ? (const void*)((const T*)p.x + rx[i] * p.x_ld + x_col[i]) : (const void*)&ZERO_PIECE, to + D_BYTES + (wave * NX + i) * 1024);
+            if constexpr (GATE)
+#pragma unroll
+                for (int i = 0; i < ND; ++i)
+                    copy_piece(rd[i] >= 0 ? (const void*)((const T*)p.y + rd[i] * (int64_t)N + d_col[i]) : (const void*)&ZERO_PIECE,
+                               to + D_BYTES + X_BYTES + (wave * ND + i) * 1024);
+            if (c_step + 1 < steps) ++c_step;                               // behind the last step the last one is copied again
+            c_buf = c_buf == 2 ? 0 : c_buf + 1;
+        };
+        auto add_rows = [&](const typename El<T>::frag (&d)[MI], int u) {
+            if (!bias || u != wk) return;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[i] += (float)d[i][e];
+        };
+        auto end_step = [&](int s) {
+            if ((s + 1) % PER_TILE) return;
+            const int i = s / PER_TILE;
+            const int g = __builtin_amdgcn_readfirstlane(lds_int(grp0 + i * 4)), next = __builtin_amdgcn_readfirstlane(lds_int(grp0 + i * 4 + 4));
+            if (g != next) {
+                if constexpr (AHEAD) settle<T, MI, NJ>(acc);
+                flush(g);
+                clear();
+            }
+        };
+        wait_copies<0>();
+        copy_step();
+        copy_step();
+        int buf = 0;
+        typename El<T>::frag d[MI], x[NJ];
+        if constexpr (AHEAD) {
+            copy_step();
+            wait_copies<2 * COPIES>();
+            __builtin_amdgcn_s_barrier();
+#pragma unroll
+            for (int i = 0; i < MI; ++i) d[i] = read_tr<T, BD * (int)sizeof(T)>(fd[0][i]);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) x[j] = read_tr<T, BX * (int)sizeof(T)>(fx[0][j]);
+            for (int s = 0; s < steps; ++s) {
+#pragma unroll
+                for (int u = 0; u < S; ++u) {
+                    add_rows(d, u);
+                    if (u == S - 1) {
+                        wait_copies<COPIES>();
+                        __builtin_amdgcn_s_barrier();
+                        buf = buf == 2 ? 0 : buf + 1;
+                    }
+                    const int n = (u + 1) % S;
+                    const unsigned stage = buf * STAGE;
+                    block_wgrad<BD * 2, BX * 2, NJ>(T(), acc, d, x, fd[n][0] + stage, fd[n][1] + stage, fx[n][0] + stage, fx[n][NJ - 1] + stage);
+                }
+                copy_step();
+                end_step(s);
+            }
+        } else {
+            for (int s = 0; s < steps; ++s) {
+                wait_copies<COPIES>();
+                __builtin_amdgcn_s_barrier();
+                copy_step();
+                const unsigned stage = buf * STAGE;
+#pragma unroll
+                for (int u = 0; u < S; ++u) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) {
+                        d[i] = read_tr<T, BD * (int)sizeof(T)>(fd[u][i] + stage);
+                        if constexpr (GATE) d[i] = gate_frag<T>(d[i], read_tr<T, BD * (int)sizeof(T)>(fd[u][i] + stage + D_BYTES + X_BYTES));
+                    }
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) x[j] = read_tr<T, BX * (int)sizeof(T)>(fx[u][j] + stage);
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) acc[i][j] = El<T>::mfma(d[i], x[j], acc[i][j]);
+                    add_rows(d, u);
+                }
+                end_step(s);
+                buf = buf == 2 ? 0 : buf + 1;
+            }
+        }
+        wait_copies<0>();                                                   // nothing may land once the rows are written anew
+    }
+}
+
 // dW[n][k] = sum over rows dZ[row][n] x[row][k].  A workgroup owns one BT x BT block of every dW it meets and walks
 // `chunk` consecutive tiles of the flat tile list, whatever groups they belong to, so all workgroups have equal work
 // however uneven the groups are.  A group that lies inside one chunk is finished here; the pieces of a longer one go to
 // the workspace and are added up in order by wgrad_join_kernel (no atomics: the result does not depend on timing).
-template <typename T, bool GATE, bool WIDE, int BT>
+// The same through registers: any row length, any alignment.
+template <typename T, bool GATE, int BT>
 __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();                       // rows of one step
-    constexpr int PER_TILE = TILE_ROWS / BK;
-    constexpr int STAGE = 2 * tr_bytes<T>();
-    __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+    constexpr int PER_TILE = TILE_ROWS / BK, S = ROW_PIECES / 2;
+    __shared__ __attribute__((aligned(16))) char lds[2 * tr_bytes<T, BT>()];
     __shared__ int tile_pos[MAX_CHUNK_TILES], tile_cnt[MAX_CHUNK_TILES], tile_grp[MAX_CHUNK_TILES];
     constexpr int M = BT / 64;                                              // 32 x 32 blocks of a wave: M x M
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -378,60 +1224,59 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
     __syncthreads();
 
     const int K = p.K, N = p.N;
-    constexpr int BPR = BT / E, RSTEP = THREADS / BPR, NP = BK / RSTEP;     // pieces of a row, rows between a thread's pieces
-    const int q = tid % BPR, r0 = tid / BPR;
+    constexpr int BPR = BT / E, NP = BK * BPR / THREADS;                    // pieces of a row, of a thread
+    char* const X = lds;
+    char* const D = lds + tr_bytes<T, BT>();
+    int prow[NP], pq[NP], rows[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        prow[j] = (tid + j * THREADS) / BPR;
+        pq[j] = (tid + j * THREADS) % BPR;
+    }
     Pack<T, E> rx[NP], rd[NP];
-    int rows[NP];
     const int steps = (t1 - t0) * PER_TILE;
-    auto find = [&](int s) {                                                // rows of step s
-        const int i = s / PER_TILE, first = (s % PER_TILE) * BK;
+    auto find = [&](int s) {                                                // rows of step s; -1 where it has none
+        const int i = s < steps ? s / PER_TILE : 0, first = (s % PER_TILE) * BK;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-            const int r = first + r0 + RSTEP * j;
-            rows[j] = s < steps && r < tile_cnt[i < t1 - t0 ? i : 0] ? row_at(p.rows, (int64_t)tile_pos[i] + r) : -1;
+            const int r = first + prow[j], cnt = tile_cnt[i];
+            const int row = row_at(p.rows, (int64_t)tile_pos[i] + (r < cnt ? r : 0));
+            rows[j] = s < steps && r < cnt ? row : -1;
         }
     };
-    auto load = [&]() {
+    auto fill = [&]() {
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const bool ok = rows[j] >= 0;
             const int64_t row = ok ? rows[j] : 0;
-            rx[j] = load_piece<T, WIDE>((const T*)p.x + row * p.x_ld, k0 + q * E, K, ok);
-            rd[j] = load_piece<T, WIDE>((const T*)p.dy + row * p.dy_ld, n0 + q * E, N, ok);
-            if (GATE) {
-                const Pack<T, E> y = load_piece<T, WIDE>((const T*)p.y + row * N, n0 + q * E, N, ok);
+            const T *xrow = (const T*)p.x + row * p.x_ld, *drow = (const T*)p.dy + row * p.dy_ld;
+            rx[j] = load_piece<T>(xrow, k0 + pq[j] * E, K, ok);
+            rd[j] = load_piece<T>(drow, n0 + pq[j] * E, N, ok);
+            if constexpr (GATE) {
+                const Pack<T, E> y = load_piece<T>((const T*)p.y + row * N, n0 + pq[j] * E, N, ok);
                 gate_piece<T, E>(rd[j], y);
             }
         }
     };
-    auto put = [&](int buf) {
-        char* X = lds + buf * STAGE;
-        char* D = X + tr_bytes<T>();
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            put_piece<T, E>(X + tr_addr<T>(r0 + RSTEP * j, q), rx[j]);
-            put_piece<T, E>(D + tr_addr<T>(r0 + RSTEP * j, q), rd[j]);
-        }
-    };
-    f32x16 acc[M][M], accb[M];
+    f32x16 acc[M][M];
+    float sum[M];                                                           // of dZ over this lane's rows
     auto clear = [&]() {
 #pragma unroll
         for (int i = 0; i < M; ++i) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) accb[i][r] = 0.0f;
+            sum[i] = 0.0f;
 #pragma unroll
             for (int j = 0; j < M; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
         }
     };
-    const bool bias = p.db && k0 == 0 && k_off == 0;                        // this wave also sums dZ over the rows
+    const bool bias = p.db && k0 == 0 && k_off == 0;
     auto flush = [&](int g) {
         const int b0 = p.rows.tile_base[g], b1 = p.rows.tile_base[g + 1];
         const bool whole = b0 >= t0 && b1 <= t1;
         const int64_t slot = 2 * (int64_t)c + (b0 >= t0 ? 1 : 0);
 #pragma unroll
-        for (int i = 0; i < M; ++i)
+        for (int i = 0; i < M; ++i) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int n = n0 + n_off + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
@@ -443,45 +1288,51 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
                     if (whole) ((T*)p.dw)[((int64_t)g * N + n) * K + k] = (T)acc[i][j][r];
                     else p.part_w[(slot * N + n) * K + k] = acc[i][j][r];
                 }
-                if (bias && (lane & 31) == 0) {
-                    if (whole) ((T*)p.db)[(int64_t)g * N + n] = (T)accb[i][r];
-                    else p.part_b[slot * N + n] = accb[i][r];
+            }
+            if (bias) {
+                const float s = sum[i] + __shfl_xor(sum[i], 32, 64);
+                const int n = n0 + n_off + 32 * i + lane;
+                if (lane < 32 && n < N) {
+                    if (whole) ((T*)p.db)[(int64_t)g * N + n] = (T)s;
+                    else p.part_b[slot * N + n] = s;
                 }
             }
+        }
     };
-    typename El<T>::frag ones;
-#pragma unroll
-    for (int e = 0; e < E; ++e) ones[e] = (T)1.0f;
 
     clear();
     find(0);
-    load();
-    find(1);
-    put(0);
-    __syncthreads();
     for (int s = 0; s < steps; ++s) {
-        if (s + 1 < steps) {
-            load();
-            find(s + 2);
-        }
-        const char* X = lds + (s & 1) * STAGE;
-        const char* D = X + tr_bytes<T>();
+        fill();                                                             // no registers left to hold a step ahead
+        find(s + 1);
 #pragma unroll
-        for (int u = 0; u < ROW_PIECES / 2; ++u) {
-            typename El<T>::frag fx[M], fd[M];
+        for (int j = 0; j < NP; ++j) {
+            put_piece<T, E>(X + tr_addr<T, BT>(prow[j], pq[j]), rx[j]);
+            put_piece<T, E>(D + tr_addr<T, BT>(prow[j], pq[j]), rd[j]);
+        }
+        __syncthreads();
+        typename El<T>::frag fx[S][M], fd[S][M];
+#pragma unroll
+        for (int u = 0; u < S; ++u)
 #pragma unroll
             for (int i = 0; i < M; ++i) {
-                fx[i] = tr_frag<T>(X, k_off + 32 * i, u, lane);
-                fd[i] = tr_frag<T>(D, n_off + 32 * i, u, lane);
+                fx[u][i] = tr_frag<T, BT>(X, k_off + 32 * i, u, lane);
+                fd[u][i] = tr_frag<T, BT>(D, n_off + 32 * i, u, lane);
             }
+        __syncthreads();                                                    // every wave has read the step
+#pragma unroll
+        for (int u = 0; u < S; ++u)
 #pragma unroll
             for (int i = 0; i < M; ++i)
 #pragma unroll
-                for (int j = 0; j < M; ++j) acc[i][j] = El<T>::mfma(fd[i], fx[j], acc[i][j]);
-            if (bias)
+                for (int j = 0; j < M; ++j) acc[i][j] = El<T>::mfma(fd[u][i], fx[u][j], acc[i][j]);
+        if (bias)
 #pragma unroll
-                for (int i = 0; i < M; ++i) accb[i] = El<T>::mfma(fd[i], ones, accb[i]);
-        }
+            for (int u = 0; u < S; ++u)
+#pragma unroll
+                for (int i = 0; i < M; ++i)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) sum[i] += (float)fd[u][i][e];
         if ((s + 1) % PER_TILE == 0) {
             const int i = s / PER_TILE;
             if (i + 1 == t1 - t0 || tile_grp[i + 1] != tile_grp[i]) {
@@ -489,8 +1340,6 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
                 clear();
             }
         }
-        if (s + 1 < steps) put((s + 1) & 1);
-        __syncthreads();
     }
 }
 
@@ -502,23 +1351,19 @@ __global__ __launch_bounds__(THREADS) void wgrad_join_kernel(WgradArgs p) {
     const int c0 = b0 / p.chunk, c1 = b1 > b0 ? (b1 - 1) / p.chunk : c0;
     if (b1 > b0 && c0 == c1) return;
     const int64_t NK = (int64_t)p.N * p.K;
-    const int64_t first = (int64_t)blockIdx.x * (THREADS * 4) + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int64_t i = first + u * THREADS;
-        const bool is_w = i < NK;
-        if (!is_w && !(p.db && i < NK + p.N)) continue;
-        const float* part = is_w ? p.part_w + i : p.part_b + (i - NK);
-        const int64_t ld = is_w ? NK : p.N;
-        float sum = 0.0f;
-        if (b1 > b0) {
-            sum = part[(2 * (int64_t)c0 + 1) * ld];
+    const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+    const bool is_w = i < NK;
+    if (!is_w && !(p.db && i < NK + p.N)) return;
+    const float* part = is_w ? p.part_w + i : p.part_b + (i - NK);
+    const int64_t ld = is_w ? NK : p.N;
+    float sum = 0.0f;
+    if (b1 > b0) {
+        sum = part[(2 * (int64_t)c0 + 1) * ld];
 #pragma unroll 8
-            for (int c = c0 + 1; c <= c1; ++c) sum += part[2 * (int64_t)c * ld];
-        }
-        if (is_w) ((T*)p.dw)[g * NK + i] = (T)sum;
-        else ((T*)p.db)[(int64_t)g * p.N + (i - NK)] = (T)sum;
+        for (int c = c0 + 1; c <= c1; ++c) sum += part[2 * (int64_t)c * ld];
     }
+    if (is_w) ((T*)p.dw)[g * NK + i] = (T)sum;
+    else ((T*)p.db)[(int64_t)g * p.N + (i - NK)] = (T)sum;
 }
 
 static inline bool sizes_ok(int64_t n, int64_t n_groups, int K, int N) {
@@ -530,16 +1375,18 @@ static inline int64_t max_tiles(int64_t n, int64_t n_groups) { return n / TILE_R
 static inline int64_t xcd_grid(int64_t work, int64_t unit) { return ((work + unit - 1) / unit + 7) / 8 * unit * 8; }
 
 struct WgradPlan {
-    int bt, tiles_n, tiles_k, chunk;
+    int bd, bx, tiles_n, tiles_k, chunk;
     int64_t chunks, part_w, part_b, bytes;
 };
-static WgradPlan wgrad_plan(int64_t n, int64_t n_groups, int K, int N) {
+// wide: whole aligned pieces (one workgroup per compute unit), else through registers (two)
+static WgradPlan wgrad_plan(int64_t n, int64_t n_groups, int K, int N, bool wide, bool gate, int precision) {
     WgradPlan w = {};
-    w.bt = K <= 64 && N <= 64 ? 64 : 128;
-    w.tiles_n = (N + w.bt - 1) / w.bt;
-    w.tiles_k = (K + w.bt - 1) / w.bt;
+    w.bd = !wide && K <= 64 && N <= 64 ? 64 : 128;
+    w.bx = wide && !gate && precision != NERF_PREC_FP32 && K > 128 ? 256 : w.bd;
+    w.tiles_n = (N + w.bd - 1) / w.bd;
+    w.tiles_k = (K + w.bx - 1) / w.bx;
     const int64_t tiles = max_tiles(n, n_groups), blocks = (int64_t)w.tiles_n * w.tiles_k;
-    int64_t chunks = 512 / blocks;                       // two workgroups per compute unit
+    int64_t chunks = (wide ? 256 : 512) / blocks;
     if (chunks < 1) chunks = 1;
     int64_t chunk = (tiles + chunks - 1) / chunks;
     if (chunk < 2) chunk = 2;
@@ -558,32 +1405,58 @@ static WgradPlan wgrad_plan(int64_t n, int64_t n_groups, int K, int N) {
 template <bool WT>
 static int launch_linear(const LinArgs& args, int precision, bool wide, void* stream) {
     LinArgs p = args;
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t tiles = max_tiles(p.rows.n, p.rows.n_groups);
+    if (wide) {
+        // Output tile: the width with the least work on the busiest compute unit, ceil(items / 256) tiles of BN + an
+        // overhead for reading the rows once more per tile (which weighs more where the products are fast).
+        const int most = p.gate || precision == NERF_PREC_FP32 ? 128 : 256, extra = precision == NERF_PREC_FP32 ? 8 : 32;
+        int bn = 64;
+        int64_t least = -1;
+        for (int b = 64; b <= most; b *= 2) {
+            const int64_t cost = (tiles * ((p.O + b - 1) / b) + 255) / 256 * (b + extra);
+            if (least < 0 || cost < least) { least = cost; bn = b; }
+        }
+        p.tiles_o = (p.O + bn - 1) / bn;
+        int64_t grid = (tiles * p.tiles_o + 7) / 8 * 8;
+        if (grid > 256) grid = 256;
+#define NERF_ST(T, GATE, BN) hipLaunchKernelGGL((stream_kernel<T, WT, GATE, BN>), dim3((unsigned)grid), dim3(ST_THREADS), 0, st, p)
+#define NERF_CALL(T)                                                \
+    do {                                                            \
+        if constexpr (WT) {                                         \
+            if (p.gate && bn == 128) { NERF_ST(T, true, 128); break; } \
+            if (p.gate) { NERF_ST(T, true, 64); break; }            \
+        }                                                           \
+        if constexpr (sizeof(T) == 2)                               \
+            if (bn == 256) { NERF_ST(T, false, 256); break; }       \
+        if (bn == 128) NERF_ST(T, false, 128);                      \
+        else NERF_ST(T, false, 64);                                 \
+    } while (0)
+        NERF_ELEM_DISPATCH(precision, NERF_CALL);
+#undef NERF_CALL
+#undef NERF_ST
+        return nerf_launch_status();
+    }
     const int bn = p.O <= 64 ? 64 : 128;
     p.tiles_o = (p.O + bn - 1) / bn;
-    const int64_t grid = xcd_grid(max_tiles(p.rows.n, p.rows.n_groups) * p.tiles_o, 1);
+    const int64_t grid = xcd_grid(tiles * p.tiles_o, 1);
     NERF_REQUIRE(grid < ((int64_t)1 << 31), NERF_E_SHAPE);
-    hipStream_t st = (hipStream_t)stream;
-#define NERF_LIN(T, GATE, WIDE, BN) \
-    hipLaunchKernelGGL((linear_kernel<T, WT, GATE, WIDE, BN>), dim3((unsigned)grid), dim3(THREADS), 0, st, p)
-#define NERF_LIN_G(T, GATE)                               \
-    do {                                                  \
-        if (wide && bn == 128) NERF_LIN(T, GATE, true, 128); \
-        else if (wide) NERF_LIN(T, GATE, true, 64);       \
-        else if (bn == 128) NERF_LIN(T, GATE, false, 128); \
-        else NERF_LIN(T, GATE, false, 64);                \
+#define NERF_LIN(T, GATE)                                                                                                      \
+    do {                                                                                                                       \
+        if (bn == 128) hipLaunchKernelGGL((linear_kernel<T, WT, GATE, 128>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);   \
+        else hipLaunchKernelGGL((linear_kernel<T, WT, GATE, 64>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);              \
     } while (0)
 #define NERF_CALL(T)                                      \
     do {                                                  \
         if constexpr (WT) {                               \
-            if (p.gate) NERF_LIN_G(T, true);              \
-            else NERF_LIN_G(T, false);                    \
+            if (p.gate) NERF_LIN(T, true);                \
+            else NERF_LIN(T, false);                      \
         } else {                                          \
-            NERF_LIN_G(T, false);                         \
+            NERF_LIN(T, false);                           \
         }                                                 \
     } while (0)
     NERF_ELEM_DISPATCH(precision, NERF_CALL);
 #undef NERF_CALL
-#undef NERF_LIN_G
 #undef NERF_LIN
     return nerf_launch_status();
 }
@@ -598,7 +1471,7 @@ extern "C" int nerf_grouped_fwd(int64_t n, int64_t n_groups, const int32_t* orde
     NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && x_ld >= K, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(offsets && tile_base && x && weight && y, NERF_E_NULL);
+    NERF_REQUIRE(order && offsets && tile_base && x && weight && y, NERF_E_NULL);
     const int es = elem_bytes(precision), E = 16 / es;
     NERF_REQUIRE(nerf_aligned(x, (uintptr_t)es) && nerf_aligned(weight, (uintptr_t)es) && nerf_aligned(y, (uintptr_t)es) &&
                  nerf_aligned(bias, (uintptr_t)es), NERF_E_ALIGN);
@@ -616,7 +1489,7 @@ extern "C" int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t*
     NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && d_y_ld >= N, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(offsets && tile_base && d_y && weight && d_x, NERF_E_NULL);
+    NERF_REQUIRE(order && offsets && tile_base && d_y && weight && d_x, NERF_E_NULL);
     const int es = elem_bytes(precision), E = 16 / es;
     NERF_REQUIRE(nerf_aligned(d_y, (uintptr_t)es) && nerf_aligned(weight, (uintptr_t)es) && nerf_aligned(d_x, (uintptr_t)es) &&
                  nerf_aligned(y, (uintptr_t)es), NERF_E_ALIGN);
@@ -630,7 +1503,13 @@ extern "C" int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t*
 
 extern "C" int64_t nerf_grouped_bwd_weights_workspace_bytes(int64_t n, int64_t n_groups, int K, int N) {
     if (!nerf::gl::sizes_ok(n, n_groups, K, N)) return NERF_E_SHAPE;
-    return nerf::gl::wgrad_plan(n, n_groups, K, N).bytes;
+    // what alignment, gate and type lead to differs in the number of chunks: enough for any of them
+    int64_t most = 0;
+    for (int way = 0; way < 3; ++way) {
+        const int64_t b = nerf::gl::wgrad_plan(n, n_groups, K, N, way > 0, way > 1, NERF_PREC_BF16).bytes;
+        if (b > most) most = b;
+    }
+    return most;
 }
 
 extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32_t* order, const int32_t* offsets,
@@ -641,14 +1520,14 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
     NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && d_y_ld >= N && x_ld >= K, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(offsets && tile_base && d_y && x && d_weight && workspace, NERF_E_NULL);
+    NERF_REQUIRE(order && offsets && tile_base && d_y && x && d_weight && workspace, NERF_E_NULL);
     const int es = elem_bytes(precision), E = 16 / es;
     NERF_REQUIRE(nerf_aligned(d_y, (uintptr_t)es) && nerf_aligned(x, (uintptr_t)es) && nerf_aligned(y, (uintptr_t)es) &&
                  nerf_aligned(d_weight, (uintptr_t)es) && nerf_aligned(d_bias, (uintptr_t)es) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
-    const gl::WgradPlan w = gl::wgrad_plan(n, n_groups, K, N);
-    NERF_REQUIRE(workspace_bytes >= w.bytes, NERF_E_WORKSPACE);
+    NERF_REQUIRE(workspace_bytes >= nerf_grouped_bwd_weights_workspace_bytes(n, n_groups, K, N), NERF_E_WORKSPACE);
     const bool wide = K % E == 0 && N % E == 0 && d_y_ld % E == 0 && x_ld % E == 0 && nerf_aligned(d_y, 16) && nerf_aligned(x, 16) &&
                       nerf_aligned(y, 16);
+    const gl::WgradPlan w = gl::wgrad_plan(n, n_groups, K, N, wide, y != nullptr, precision);
     gl::WgradArgs p = {};
     p.rows = {n, (int)n_groups, order, offsets, tile_base};
     p.K = K; p.N = N; p.tiles_k = w.tiles_k; p.tiles_n = w.tiles_n; p.chunk = w.chunk;
@@ -659,25 +1538,30 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
     const int64_t grid = gl::xcd_grid(w.chunks * blocks, blocks);
     NERF_REQUIRE(grid < ((int64_t)1 << 31), NERF_E_SHAPE);
     hipStream_t st = (hipStream_t)stream;
-    const dim3 join((unsigned)(((int64_t)N * K + N + gl::THREADS * 4 - 1) / (gl::THREADS * 4)), (unsigned)n_groups);
-#define NERF_WG(T, GATE, WIDE, BT) \
-    hipLaunchKernelGGL((gl::wgrad_kernel<T, GATE, WIDE, BT>), dim3((unsigned)grid), dim3(gl::THREADS), 0, st, p)
+    const dim3 join((unsigned)(((int64_t)N * K + N + gl::THREADS - 1) / gl::THREADS), (unsigned)n_groups);
+#define NERF_WG(T, GATE, BT) hipLaunchKernelGGL((gl::wgrad_kernel<T, GATE, BT>), dim3((unsigned)grid), dim3(gl::THREADS), 0, st, p)
+#define NERF_WS(T, GATE, BX) \
+    hipLaunchKernelGGL((gl::wgrad_stream_kernel<T, GATE, BX>), dim3((unsigned)grid), dim3(gl::ST_THREADS), 0, st, p)
 #define NERF_WG_G(T, GATE)                                  \
     do {                                                    \
-        if (wide && w.bt == 128) NERF_WG(T, GATE, true, 128); \
-        else if (wide) NERF_WG(T, GATE, true, 64);          \
-        else if (w.bt == 128) NERF_WG(T, GATE, false, 128); \
-        else NERF_WG(T, GATE, false, 64);                   \
+        if (wide) NERF_WS(T, GATE, 128);                    \
+        else if (w.bd == 128) NERF_WG(T, GATE, 128);        \
+        else NERF_WG(T, GATE, 64);                          \
     } while (0)
 #define NERF_CALL(T)                                                                                   \
     do {                                                                                               \
-        if (p.y) NERF_WG_G(T, true);                                                                   \
+        bool done = false;                                                                             \
+        if constexpr (sizeof(T) == 2)                                                                  \
+            if (w.bx == 256) { NERF_WS(T, false, 256); done = true; }                                  \
+        if (done) {}                                                                                   \
+        else if (p.y) NERF_WG_G(T, true);                                                              \
         else NERF_WG_G(T, false);                                                                      \
         hipLaunchKernelGGL(gl::wgrad_join_kernel<T>, join, dim3(gl::THREADS), 0, st, p);               \
     } while (0)
     NERF_ELEM_DISPATCH(precision, NERF_CALL);
 #undef NERF_CALL
 #undef NERF_WG_G
+#undef NERF_WS
 #undef NERF_WG
     return nerf_launch_status();
 }

@@ -781,7 +781,7 @@ class RowGroups:
     """Rows dealt out to groups: what ``group_rows`` and ``row_groups`` return and ``grouped_linear`` takes.
 
     ``offsets`` [n_groups + 1] int32: positions offsets[g] .. offsets[g+1] - 1 hold the rows of group g.  ``order`` [n] int32:
-    the row at each position (None: the rows are in group order already).  Rows behind offsets[n_groups] belong to no group.
+    the row at each position (every row once).  Rows behind offsets[n_groups] belong to no group.
     All on the GPU; nothing is read back to the host.  Treat the tensors as read-only.
     """
     __slots__ = ("order", "offsets", "tile_base", "n_rows", "n_groups")
@@ -837,7 +837,7 @@ def row_groups(offsets: torch.Tensor, n_rows: int) -> RowGroups:
     clean = new((n_groups + 1,), dtype=torch.int32, device=dev)
     base = new((n_groups + 2,), dtype=torch.int32, device=dev)
     _call("nerf_group_offsets", "group_offsets", dev, n_rows, n_rows, n_groups, given.data_ptr(), clean.data_ptr(), base.data_ptr())
-    return RowGroups(None, clean, base, n_rows, n_groups)
+    return RowGroups(torch.arange(n_rows, dtype=torch.int32, device=dev), clean, base, n_rows, n_groups)
 
 
 def _embed_fwd(ids, table, scale):
@@ -903,7 +903,7 @@ def _grouped_fwd(x, weight, bias, groups, relu):
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     y = torch.empty((n, N), dtype=x.dtype, device=dev)
-    _call("nerf_grouped_fwd", "grouped_fwd", dev, n, n, G, _ptr(groups.order), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N,
+    _call("nerf_grouped_fwd", "grouped_fwd", dev, n, n, G, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N,
           x.data_ptr(), ld, weight.data_ptr(), _ptr(bias), int(relu), _ELEM[x.dtype], y.data_ptr())
     return y, x, weight
 
@@ -930,7 +930,7 @@ class _GroupedLinear(torch.autograd.Function):
             return (torch.zeros((0, K), dtype=d_y.dtype, device=dev) if need_x else None, torch.zeros_like(weight) if need_w else None,
                     torch.zeros((G, N), dtype=d_y.dtype, device=dev) if need_b else None, None, None)
         g, ld = _row_major(d_y)
-        at = (n, G, _ptr(groups.order), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N, g.data_ptr(), ld, _ptr(y))
+        at = (n, G, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N, g.data_ptr(), ld, _ptr(y))
         if need_x:
             dx = torch.empty((n, K), dtype=g.dtype, device=dev)
             _call("nerf_grouped_bwd_data", "grouped_bwd_data", dev, n, *at, weight.data_ptr(), prec, dx.data_ptr())

@@ -87,7 +87,7 @@ def test_group_rows_of_nothing_and_row_groups():
     # boundaries out of order, out of range, beyond 32 bits
     off = torch.tensor([7, 3, 300, 200, -5, 2 ** 40, 500], device=DEV)
     got = ops.row_groups(off, 600)
-    assert got.order is None and got.offsets.tolist() == [0, 3, 300, 300, 300, 600, 600]
+    assert got.order.tolist() == list(range(600)) and got.offsets.tolist() == [0, 3, 300, 300, 300, 600, 600]
     assert got.tile_base.tolist() == [0, 1, 4, 4, 4, 7, 7, 7]
     big = torch.arange(0, 3001, dtype=torch.int32, device=DEV) * 5
     got = ops.row_groups(big, 20000)
@@ -215,6 +215,16 @@ def test_grouped_linear(n, G, K, N, kind, relu, dtype):
     y2 = ops.grouped_linear(xs, ws, groups, bias=bs, relu=relu)
     again = torch.autograd.grad(y2, [xs, ws, bs], d_y.to(DEV))
     assert torch.equal(y, y2) and all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N,relu", [(256, 256, True), (248, 232, False), (40, 1000, False), (1000, 24, True)])
+def test_grouped_linear_many_rows(K, N, relu, dtype):
+    """enough tiles for the widest output tiles, several tiles per workgroup, some with a ragged last step or last tile"""
+    from nerf_amd import ops
+    ids, x, w, b, d_y, rows_of = linear_case(60000, 3, K, N, "random", dtype)
+    xs, ws, bs = (t.to(DEV).requires_grad_(True) for t in (x, w, b))
+    check_linear(x, w, b, d_y, rows_of, ops.group_rows(ids.to(DEV), 3), relu, xs, ws, bs)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -77,6 +77,7 @@ def test_cabi_refuses_bad_grouped_layer_arguments(lib):
         assert w(5000, G, P, P, P, K, N, P, 70000, None, P, 70000, 0, P, P, P, need, None) == SHAPE
     assert f(5000, 3, P, P, P, 40, 24, P, 39, P, P, 0, 0, P, None) == SHAPE and d(5000, 3, P, P, P, 40, 24, P, 23, None, P, 0, P, None) == SHAPE
     assert f(5000, 3, P, P, P, 40, 24, P, 40, P, P, 0, 3, P, None) == DTYPE and d(5000, 3, P, P, P, 40, 24, P, 24, None, P, -1, P, None) == DTYPE
+    assert f(5000, 3, None, P, P, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL
     assert f(5000, 3, P, None, P, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL and f(5000, 3, P, P, None, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL
     assert f(5000, 3, P, P, P, 40, 24, P + 1, 40, P, P, 0, 0, P, None) == ALIGN and d(5000, 3, P, P, P, 40, 24, P, 24, P + 2, P, 2, P, None) == ALIGN
     assert w(5000, 3, P, P, P, 40, 24, P, 24, None, P, 40, 0, P, P, P, need - 1, None) == WORK
@@ -148,7 +149,7 @@ def test_cpu_tensors_are_refused():
     from nerf_amd import ops
     i, f = torch.zeros(4, dtype=torch.int64), torch.zeros(4, 8)
     for call in (lambda: ops.group_rows(i, 2), lambda: ops.row_groups(i, 2), lambda: ops.embed_rows(i, f), lambda: ops.gated_scan(f[None], f[None]),
-                 lambda: ops.grouped_linear(f, torch.zeros(2, 3, 8), ops.RowGroups(None, i, i, 4, 2))):
+                 lambda: ops.grouped_linear(f, torch.zeros(2, 3, 8), ops.RowGroups(i, i, i, 4, 2))):
         with pytest.raises(RuntimeError):
             call()
     for call in (lambda: ops.group_rows([0, 1], 2), lambda: ops.embed_rows([0], f), lambda: ops.grouped_linear(f, f, None), lambda: ops.gated_scan(1.0, 2.0)):
