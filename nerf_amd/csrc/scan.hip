@@ -166,17 +166,39 @@ __device__ __forceinline__ void compose(const Geo& g, const Place& p, float (&A)
     for (int v = 0; v < V; ++v) in[v] = apply(ea[VA == 1 ? 0 : v], in[v], eh[v]);
 }
 
+// outputs are not read again by the call: kept out of the caches where the inputs are
+template <typename T, int V>
+__device__ __forceinline__ void put(T* p, const Pack<T, V>& x) {
+    if constexpr (sizeof(T) * V == 16) {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(__builtin_bit_cast(i32x4, x), reinterpret_cast<i32x4*>(p));
+    } else {
+        store_pack<T, V>(p, x);
+    }
+}
+
+// inputs of the backward's last pass, which nothing reads again
+template <typename T, int V, bool LAST>
+__device__ __forceinline__ Pack<T, V> take(const T* p) {
+    if constexpr (LAST && sizeof(T) * V == 16) {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(Pack<T, V>, __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p)));
+    } else {
+        return load_pack<T, V>(p);
+    }
+}
+
 template <typename T, int V>
 struct Raw { Pack<T, V> x[max_len<V>()]; };
 
 // samples t0 .. t0 + len - 1 of one input, `fill` where there is none
-template <typename T, int V>
+template <typename T, int V, bool LAST>
 __device__ __forceinline__ void fetch(Raw<T, V>& r, const In& in, const Geo& g, int reverse, int64_t b, int64_t t0, int ch, bool on, float fill) {
     const T* base = (const T*)in.p + b * in.sb + ch;
 #pragma unroll
     for (int j = 0; j < max_len<V>(); ++j) {
         const int64_t t = t0 + j;
-        if (on && j < g.len && t < g.T) r.x[j] = load_pack<T, V>(base + (reverse ? g.T - 1 - t : t) * in.st);
+        if (on && j < g.len && t < g.T) r.x[j] = take<T, V, LAST>(base + (reverse ? g.T - 1 - t : t) * in.st);
         else
 #pragma unroll
             for (int v = 0; v < V; ++v) r.x[j].v[v] = (T)fill;
@@ -190,14 +212,14 @@ struct Gates {
     Pack<T, VA> x[max_len<V>()];
     __device__ __forceinline__ float at(int j, int v) const { return (float)x[j].v[SHARED ? 0 : v]; }
 };
-template <typename T, int V, bool SHARED>
+template <typename T, int V, bool SHARED, bool LAST>
 __device__ __forceinline__ void fetch_gates(Gates<T, V, SHARED>& r, const Args& a, int64_t b, int64_t t0, int ch, bool on) {
     constexpr int VA = SHARED ? 1 : V;
     const T* base = (const T*)a.gate.p + b * a.gate.sb + (SHARED ? 0 : ch);
 #pragma unroll
     for (int j = 0; j < max_len<V>(); ++j) {
         const int64_t t = t0 + j;
-        if (on && j < a.g.len && t < a.g.T) r.x[j] = load_pack<T, VA>(base + (a.reverse ? a.g.T - 1 - t : t) * a.gate.st);
+        if (on && j < a.g.len && t < a.g.T) r.x[j] = take<T, VA, LAST>(base + (a.reverse ? a.g.T - 1 - t : t) * a.gate.st);
         else
 #pragma unroll
             for (int v = 0; v < VA; ++v) r.x[j].v[v] = (T)1.0f;
@@ -222,7 +244,8 @@ __global__ __launch_bounds__(THREADS) void fwd_kernel(Args a) {
     __shared__ float sm[WAVES * 64 * (V + VA)];
     const Geo& g = a.g;
     const Place p = place<V>(g);
-    const int64_t seg = blockIdx.z;
+    // the main pass begins with the segments that the first one read last: they are still in the last-level cache
+    const int64_t seg = AGG ? blockIdx.z : g.segs - 1 - blockIdx.z;
     const int64_t first = seg * g.per_seg, stop = first + g.per_seg < g.tiles ? first + g.per_seg : g.tiles;
     const int64_t row = p.b * g.D + p.ch;
     float carry[V], allA[VA];
@@ -233,12 +256,20 @@ __global__ __launch_bounds__(THREADS) void fwd_kernel(Args a) {
     for (int v = 0; v < VA; ++v) allA[v] = 1.0f;
     const int steps = g.tg * g.len;
     T* h_out = (T*)a.h + p.b * g.T * g.D + p.ch;
+    Gates<T, V, SHARED> ga, next_ga;                     // a tile is requested while the one before it is worked on
+    Raw<T, V> va, next_va;
+    auto request = [&](int64_t i) {
+        const int64_t t0 = i * steps + p.tgi * g.len;
+        const bool on = p.on && i < stop;
+        fetch_gates<T, V, SHARED, false>(next_ga, a, p.b, t0, p.ch, on);
+        fetch<T, V, false>(next_va, a.value, g, a.reverse, p.b, t0, p.ch, on, 0.0f);
+    };
+    request(first);
     for (int64_t i = first; i < stop; ++i) {
         const int64_t t0 = i * steps + p.tgi * g.len;
-        Gates<T, V, SHARED> ga;
-        Raw<T, V> va;
-        fetch_gates<T, V, SHARED>(ga, a, p.b, t0, p.ch, p.on);
-        fetch<T, V>(va, a.value, g, a.reverse, p.b, t0, p.ch, p.on, 0.0f);
+        ga = next_ga;
+        va = next_va;
+        request(i + 1);
         if (!AGG && a.states && i > 0 && p.on && p.tgi == 0)
             store_floats<V>(a.states + (p.b * (g.tiles - 1) + i - 1) * g.D + p.ch, carry);
         float A[VA], H[V], x[V];
@@ -268,7 +299,7 @@ __global__ __launch_bounds__(THREADS) void fwd_kernel(Args a) {
                 y.v[v] = (T)x[v];
             }
             const int64_t t = t0 + j;
-            if (p.on && j < g.len && t < g.T) store_pack<T, V>(h_out + (a.reverse ? g.T - 1 - t : t) * g.D, y);
+            if (p.on && j < g.len && t < g.T) put<T, V>(h_out + (a.reverse ? g.T - 1 - t : t) * g.D, y);
         }
     }
     if (!p.on || p.tgi != 0) return;
@@ -284,12 +315,16 @@ __global__ __launch_bounds__(THREADS) void fwd_kernel(Args a) {
 
 // The same backwards in time.  AGG: the map of u over each segment.
 template <typename T, int V, bool SHARED, bool AGG>
-__global__ __launch_bounds__(THREADS) void bwd_kernel(Args a) {
+__global__ __launch_bounds__(THREADS, 2) void bwd_kernel(Args a) {
     constexpr int VA = SHARED ? 1 : V, L = max_len<V>();
+    // A tile is requested ahead, except where three fp32 tensors per channel would leave one wave per SIMD (or spill):
+    // 2 x 262 144 x 64 fp32, gate per channel: 225 us ahead, 203 not; 4096 x 192 x 64 bf16, one gate: 102 ahead, 152 not.
+    constexpr bool AHEAD = AGG || SHARED || V != 4;
     __shared__ float sm[WAVES * 64 * (V + VA)];
     const Geo& g = a.g;
     const Place p = place<V>(g);
-    const int64_t seg = blockIdx.z;
+    // the main pass begins with the segments that the first one read last: they are still in the last-level cache
+    const int64_t seg = AGG ? blockIdx.z : g.segs - 1 - blockIdx.z;
     const int64_t first = seg * g.per_seg, stop = first + g.per_seg < g.tiles ? first + g.per_seg : g.tiles;
     const int64_t row = p.b * g.D + p.ch;
     float carry[V], allA[VA];                            // u behind the tile
@@ -300,13 +335,23 @@ __global__ __launch_bounds__(THREADS) void bwd_kernel(Args a) {
     for (int v = 0; v < VA; ++v) allA[v] = 1.0f;
     const int steps = g.tg * g.len;
     const In gin = {a.d_h, g.T * g.D, g.D};
+    Gates<T, V, SHARED> ga, next_ga;                     // a tile is requested while the one behind it is worked on
+    Raw<T, V> va, gr, next_va, next_gr;
+    auto request = [&](int64_t i) {
+        const int64_t t0 = i * steps + p.tgi * g.len;
+        const bool on = p.on && i >= first;
+        fetch_gates<T, V, SHARED, !AGG>(next_ga, a, p.b, t0, p.ch, on);
+        fetch<T, V, !AGG>(next_gr, gin, g, a.reverse, p.b, t0, p.ch, on && a.d_h, 0.0f);
+        if (!AGG) fetch<T, V, !AGG>(next_va, a.value, g, a.reverse, p.b, t0, p.ch, on, 0.0f);
+    };
+    if (AHEAD) request(stop - 1);
     for (int64_t i = stop - 1; i >= first; --i) {
         const int64_t t0 = i * steps + p.tgi * g.len;
-        Gates<T, V, SHARED> ga;
-        Raw<T, V> va, gr;
-        fetch_gates<T, V, SHARED>(ga, a, p.b, t0, p.ch, p.on);
-        fetch<T, V>(gr, gin, g, a.reverse, p.b, t0, p.ch, p.on && a.d_h, 0.0f);
-        if (!AGG) fetch<T, V>(va, a.value, g, a.reverse, p.b, t0, p.ch, p.on, 0.0f);
+        if (!AHEAD) request(i);
+        ga = next_ga;
+        gr = next_gr;
+        if (!AGG) va = next_va;
+        if (AHEAD) request(i - 1);
         float A[VA], U[V], u[V];
 #pragma unroll
         for (int v = 0; v < VA; ++v) A[v] = 1.0f;
@@ -350,7 +395,7 @@ __global__ __launch_bounds__(THREADS) void bwd_kernel(Args a) {
             }
             const int64_t t = t0 + j;
             if (a.d_value && p.on && j < g.len && t < g.T)
-                store_pack<T, V>((T*)a.d_value + (p.b * g.T + (a.reverse ? g.T - 1 - t : t)) * g.D + p.ch, y);
+                put<T, V>((T*)a.d_value + (p.b * g.T + (a.reverse ? g.T - 1 - t : t)) * g.D + p.ch, y);
         }
         if (i == 0 && p.tgi == 0 && p.on && a.d_state) store_floats<V>(a.d_state + row, u);
         if (!a.d_gate) continue;
@@ -372,7 +417,7 @@ __global__ __launch_bounds__(THREADS) void bwd_kernel(Args a) {
                 Pack<T, V> y;
 #pragma unroll
                 for (int v = 0; v < V; ++v) y.v[v] = (T)(G[j][v] * h[v]);
-                store_pack<T, V>((T*)a.d_gate + at * g.D + p.ch, y);
+                put<T, V>((T*)a.d_gate + at * g.D + p.ch, y);
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = fmaf(ga.at(j, v), h[v], (float)va.x[j].v[v]);
@@ -447,8 +492,11 @@ static Geo geometry(int64_t B, int64_t T, int64_t D, int precision) {
     while (g.cgl < 6 && ((int64_t)v << g.cgl) < D) ++g.cgl;
     const int units = THREADS >> g.cgl;
     g.col_blocks = (int)((D + ((int64_t)v << g.cgl) - 1) / ((int64_t)v << g.cgl));
+    // Threads along time only as far as sequences and channels leave the chip short of them (16 waves per compute unit):
+    // composing costs several shuffles per channel for every doubling.
+    const int64_t rows = B * g.col_blocks << g.cgl;
     g.tg = 1;
-    while (g.tg < units && (int64_t)g.tg * max_l < T) g.tg <<= 1;
+    while (g.tg < units && (int64_t)g.tg * max_l < T && rows * g.tg < 256 * 16 * 64) g.tg <<= 1;
     g.tiles = (T + (int64_t)g.tg * max_l - 1) / ((int64_t)g.tg * max_l);
     if (g.tiles < 1) g.tiles = 1;
     g.len = (int)((T + g.tiles * g.tg - 1) / (g.tiles * g.tg));
