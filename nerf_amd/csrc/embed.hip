@@ -19,6 +19,7 @@ namespace emb {
 
 constexpr int THREADS = 256;
 constexpr int FWD_ROWS = 4;      // rows a lane group has in flight
+constexpr int SMALL_N = 4096;    // positions of a call that one kernel serves
 constexpr int LONG_RUN = 16;     // workgroup partials of one row above which a whole workgroup adds them up
 
 // LPR lanes share a row; columns beyond LPR * VEC are walked by the same lanes
@@ -101,7 +102,7 @@ __device__ __forceinline__ void add_part(float (&acc)[VEC], const float* p) {
 }
 
 template <typename T, int VEC>
-__global__ __launch_bounds__(THREADS) void bwd_sum_kernel(BwdArgs a, const T* __restrict__ d_out, int64_t ld, T* __restrict__ d_table) {
+__global__ __launch_bounds__(THREADS, 4) void bwd_sum_kernel(BwdArgs a, const T* __restrict__ d_out, int64_t ld, T* __restrict__ d_table) {
     constexpr int BATCH = 8;
     __shared__ float head[THREADS * VEC], tail[THREADS * VEC];
     __shared__ int head_state[THREADS], tail_key[THREADS];         // head: 0 none, 1 ends in its lane group, 2 goes on
@@ -119,20 +120,37 @@ __global__ __launch_bounds__(THREADS) void bwd_sum_kernel(BwdArgs a, const T* __
         for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
         int key = a.keys[p0];
         bool from_left = p0 > 0 && a.keys[p0 - 1] == key;
-        for (int64_t p = p0; p < p1; p += BATCH) {
-            int k[BATCH];
-            Pack<T, VEC> x[BATCH];
+        // rows of d_out are requested a batch ahead, their numbers two
+        int k[BATCH], next_k[BATCH], row[BATCH];
+        Pack<T, VEC> x[BATCH], next_x[BATCH];
+        auto numbers = [&](int64_t p) {
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
                 const int64_t q = p + j < p1 ? p + j : p1 - 1;
-                k[j] = a.keys[q];
-                const int64_t row = a.order[q];
-                if (on) x[j] = load_pack<T, VEC>(d_out + row * ld + col);
+                next_k[j] = a.keys[q];
+                row[j] = a.order[q];
             }
+        };
+        auto request = [&]() {
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) {
+                k[j] = next_k[j];
+                if (on) next_x[j] = load_pack<T, VEC>(d_out + row[j] * ld + col);
+            }
+        };
+        numbers(p0);
+        request();
+        numbers(p0 + BATCH);
+        for (int64_t p = p0; p < p1; p += BATCH) {
+            int now[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j) { now[j] = k[j]; x[j] = next_x[j]; }
+            request();
+            numbers(p + 2 * BATCH);
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
                 if (p + j >= p1) break;
-                if (k[j] != key) {                                 // the run of `key` ends here
+                if (now[j] != key) {                               // the run of `key` ends here
                     if (from_left) {
                         hstate = 1;
                         if (on)
@@ -142,7 +160,7 @@ __global__ __launch_bounds__(THREADS) void bwd_sum_kernel(BwdArgs a, const T* __
                         write_row<T, VEC>(d_table, key, a.dim, col, acc, a.scale);
                     }
                     from_left = false;
-                    key = k[j];
+                    key = now[j];
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
                 }
@@ -264,6 +282,67 @@ __global__ __launch_bounds__(THREADS) void bwd_join_kernel(BwdArgs a, T* __restr
     }
 }
 
+// Few positions and few rows: a workgroup per table row looks through all ids, keeps the positions that name its row (in
+// order, each wave its own quarter) and sums their rows of d_out, one launch instead of five.  1024 positions over 100 rows
+// of 48 fp32: 16 us for the call with grouping, see the limit below for where it stops paying.
+template <typename T, int VEC, typename ID>
+__global__ __launch_bounds__(THREADS) void bwd_small_kernel(int n, const ID* __restrict__ ids, int dim, int lpr, const T* __restrict__ d_out,
+                                                            int64_t ld, float scale, T* __restrict__ d_table) {
+    constexpr int ROUNDS = SMALL_N / THREADS;
+    __shared__ int list[SMALL_N];
+    __shared__ int count[THREADS / 64];
+    __shared__ float red[THREADS * VEC];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row = blockIdx.x, quarter = (n + THREADS - 1) / THREADS * 64;
+    ID id[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int p = wave * quarter + r * 64 + lane;
+        id[r] = r * 64 < quarter && p < n ? ids[p] : (ID)-1;
+    }
+    int cnt = 0;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const bool mine = id[r] == (ID)row;
+        const unsigned long long m = __ballot(mine);
+        if (mine) list[wave * quarter + cnt + __popcll(m & ((1ull << lane) - 1ull))] = wave * quarter + r * 64 + lane;
+        cnt += __popcll(m);
+    }
+    if (lane == 0) count[wave] = cnt;
+    __syncthreads();
+    const int groups = THREADS / lpr, sub = (int)threadIdx.x / lpr, l = (int)threadIdx.x % lpr;
+    for (int col = l * VEC; col - l * VEC < dim; col += lpr * VEC) {
+        const bool on = col < dim;
+        float acc[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) acc[v] = 0.0f;
+        int at = sub;                                              // positions sub, sub + groups, .. of the four lists in a row
+        for (int w = 0; w < THREADS / 64; ++w) {
+            for (; at < count[w]; at += groups) {
+                if (!on) continue;
+                const Pack<T, VEC> x = load_pack<T, VEC>(d_out + list[w * quarter + at] * ld + col);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) acc[v] += (float)x.v[v];
+            }
+            at -= count[w];
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) red[threadIdx.x * VEC + v] = acc[v];
+        __syncthreads();
+        if (sub == 0 && on) {
+            for (int k = 1; k < groups; ++k)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) acc[v] += red[(k * lpr + l) * VEC + v];
+            write_row<T, VEC>(d_table, row, dim, col, acc, scale);
+        }
+        __syncthreads();
+    }
+}
+
+// up to four million comparisons of ids with rows, at most 4096 ids: 4096 positions over 256 rows take 5 us, over 1024 rows 6,
+// grouped first 24
+static inline bool small_call(int64_t n, int64_t rows) { return n <= SMALL_N && n * rows <= ((int64_t)1 << 22); }
+
 static inline int lanes_per_row(int64_t dim, int vec) {
     int l = 4;
     while (l < 64 && (int64_t)l * vec < dim) l <<= 1;
@@ -367,13 +446,29 @@ extern "C" int nerf_embed_bwd(int64_t n, const void* ids, int id_bytes, int64_t 
     char* ws = (char*)workspace;
     hipStream_t st = (hipStream_t)stream;
     int32_t *order = (int32_t*)(ws + plan.order), *offsets = (int32_t*)(ws + plan.offsets), *keys = (int32_t*)(ws + plan.keys);
+    const bool wide = dim % full == 0 && d_out_ld % full == 0 && nerf_aligned(d_out, 16) && nerf_aligned(d_table, 16);
+    const int vec = wide ? full : 1, lpr = emb::lanes_per_row(dim, vec);
+    if (emb::small_call(n, rows)) {
+#define NERF_SMALL(T, V, ID)                                                                                                      \
+    hipLaunchKernelGGL((emb::bwd_small_kernel<T, V, ID>), dim3((unsigned)rows), dim3(emb::THREADS), 0, st, (int)n, (const ID*)ids, (int)dim, \
+                       lpr, (const T*)d_out, d_out_ld, scale, (T*)d_table)
+#define NERF_CALL(T)                                                                      \
+    do {                                                                                  \
+        if (wide && id_bytes == 8) NERF_SMALL(T, full_vec<T>(), int64_t);                 \
+        else if (wide) NERF_SMALL(T, full_vec<T>(), int32_t);                             \
+        else if (id_bytes == 8) NERF_SMALL(T, 1, int64_t);                                \
+        else NERF_SMALL(T, 1, int32_t);                                                   \
+    } while (0)
+        NERF_ELEM_DISPATCH(precision, NERF_CALL);
+#undef NERF_CALL
+#undef NERF_SMALL
+        return nerf_launch_status();
+    }
     const int rc = grp::launch_group_rows(n, ids, id_bytes, rows, order, offsets, nullptr, keys, ws + plan.group, st);
     if (rc != NERF_OK) return rc;
-    const bool wide = dim % full == 0 && d_out_ld % full == 0 && nerf_aligned(d_out, 16) && nerf_aligned(d_table, 16);
-    const int vec = wide ? full : 1;
     emb::BwdArgs a = {};
     a.n = n; a.rows = rows; a.dim = (int)dim;
-    a.lpr = emb::lanes_per_row(dim, vec);
+    a.lpr = lpr;
     const int groups = emb::THREADS / a.lpr;
     a.per = emb::positions_per_group(n, groups);
     a.order = order; a.offsets = offsets; a.keys = keys; a.scale = scale; a.part = (float*)(ws + plan.part);

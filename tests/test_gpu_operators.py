@@ -61,7 +61,7 @@ def make_ids(n, groups, kind, g, dtype=torch.int64):
 # ---- grouping ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
-@pytest.mark.parametrize("n,groups", [(1, 1), (2, 1), (63, 2), (64, 3), (65, 255), (1000, 256), (1025, 257), (4096, 8), (4096, 5000), (4097, 8),
+@pytest.mark.parametrize("n,groups", [(1, 1), (2, 1), (63, 2), (64, 3), (65, 255), (1000, 256), (1025, 257), (2048, 8), (2048, 5000), (2049, 8), (2049, 300), (300001, 3000), (4096, 8), (4096, 5000), (4097, 8),
                                       (4097, 255), (8192, 256), (12289, 70000), (100003, 64), (300000, 1), (50000, 65535)])
 def test_group_rows(n, groups, dtype):
     from nerf_amd import ops
@@ -99,7 +99,8 @@ def test_group_rows_of_nothing_and_row_groups():
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,rows,dim,kind", [(1, 1, 1, "one"), (1024, 100, 48, "random"), (513, 7, 63, "random"), (5000, 9, 3, "skewed"),
                                              (40000, 3, 16, "skewed"), (30000, 1, 40, "one"), (3000, 20000, 8, "random"), (70000, 300, 48, "runs"),
-                                             (2000, 50, 1000, "random"), (600, 11, 517, "skewed"), (64, 5, 2, "none"), (200000, 4096, 4, "skewed")])
+                                             (2000, 50, 1000, "random"), (600, 11, 517, "skewed"), (64, 5, 2, "none"), (200000, 4096, 4, "skewed"), (4096, 1024, 20, "random"), (4096, 1025, 20, "random"), (4097, 10, 24, "skewed"),
+                                             (3000, 2, 1, "one")])
 def test_embed_rows(n, rows, dim, kind, dtype):
     from nerf_amd import ops
     g = gen(n + dim)
