@@ -116,20 +116,35 @@ __device__ __forceinline__ void copy_piece(const void* from, char* to) {
 }
 
 // ---- pieces from memory ---------------------------------------------------------------------------------------
-// columns c .. of a row that has `cols` of them; zero behind its end and when !ok
-template <typename T, bool WIDE = false>
+// columns c .. of a row that has `cols` of them; zero behind its end and when !ok.  The row may begin anywhere (memory
+// instructions take any address that its elements are aligned to).  The last piece of a row is read where it ends and
+// shifted into place, so nothing behind the row is touched; rows shorter than a piece go element by element.
+template <typename T>
 __device__ __forceinline__ Pack<T, piece<T>()> load_piece(const T* row, int c, int cols, bool ok) {
     constexpr int E = piece<T>();
+    struct __attribute__((packed, aligned(sizeof(T)))) Any { unsigned long long lo, hi; };
     Pack<T, E> p;
-    if constexpr (WIDE) {
-        if (ok && c < cols) return load_pack<T, E>(row + c);
-#pragma unroll
-        for (int e = 0; e < E; ++e) p.v[e] = (T)0.0f;
-    } else {
+    if (cols < E) {
 #pragma unroll
         for (int e = 0; e < E; ++e) p.v[e] = ok && c + e < cols ? row[c + e] : (T)0.0f;
+        return p;
     }
-    return p;
+    const int over = c + E - cols;                                          // elements of the piece behind the row
+    const Any raw = *reinterpret_cast<const Any*>(row + (over > 0 ? cols - E : c));
+    unsigned long long lo = raw.lo, hi = raw.hi;
+    if (over > 0) {
+        const int bits = min(over, E) * (int)sizeof(T) * 8;
+        if (bits >= 64) {
+            lo = bits == 128 ? 0 : hi >> (bits - 64);
+            hi = 0;
+        } else {
+            lo = (lo >> bits) | (hi << (64 - bits));
+            hi >>= bits;
+        }
+    }
+    if (!ok) lo = hi = 0;
+    struct Two { unsigned long long lo, hi; } two = {lo, hi};
+    return __builtin_bit_cast(Pack<T, E>, two);
 }
 
 template <typename T, int E>
@@ -795,10 +810,10 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
         for (int i = 0; i < NB; ++i) {
             if constexpr (WT) {
                 const int c = k0 + (tid + i * THREADS) / BPR;
-                rb[i] = load_piece<T>(w + (int64_t)c * O, o0 + (tid + i * THREADS) % BPR * E, O, c < C);
+                rb[i] = load_piece<T>(w + (int64_t)(c < C ? c : 0) * O, o0 + (tid + i * THREADS) % BPR * E, O, c < C);
             } else {
                 const int o = o0 + r0 + 32 * i;
-                rb[i] = load_piece<T>(w + (int64_t)o * C, k0 + q * E, C, o < O);
+                rb[i] = load_piece<T>(w + (int64_t)(o < O ? o : 0) * C, k0 + q * E, C, o < O);
             }
         }
     };
@@ -871,10 +886,18 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
                     put_piece<T, 4>(lds + (m_off + 32 * i + (lane & 31)) * PITCH + (o_off + 32 * j + 8 * h + 4 * (lane >> 5)) * 2, v);
                 }
         __syncthreads();
-#pragma unroll 4
-        for (int i = tid; i < TILE_ROWS * BN; i += THREADS) {
-            const int m = i / BN, c = i % BN, row = row_of[m];
-            if (row >= 0 && o0 + c < O) out[(int64_t)row * O + o0 + c] = *reinterpret_cast<const T*>(lds + m * PITCH + c * 2);
+        struct __attribute__((packed, aligned(sizeof(T)))) Any { unsigned long long lo, hi; };
+#pragma unroll
+        for (int i = 0; i < TILE_ROWS * BN / E / THREADS; ++i) {
+            const int at = tid + i * THREADS, m = at / (BN / E), c = at % (BN / E) * E, row = row_of[m];
+            if (row < 0 || o0 + c >= O) continue;
+            const Pack<T, E> v = *reinterpret_cast<const Pack<T, E>*>(lds + m * PITCH + c * 2);
+            T* to = out + (int64_t)row * O + o0 + c;
+            if (o0 + c + E <= O) *reinterpret_cast<Any*>(to) = __builtin_bit_cast(Any, v);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (o0 + c + e < O) to[e] = v.v[e];
         }
     } else {
 #pragma unroll
