@@ -399,25 +399,27 @@ int nerf_embed_bwd(int64_t n, const void *ids, int id_bytes, int64_t rows, int64
 
 /* Linear layers of n_groups sub-networks, weight [n_groups, N, K], bias (nullable) [n_groups, N]:
  *   y[i] = act(weight[g(i)] x[i] + bias[g(i)]), act = ReLU when relu (keeps a NaN), zeros for rows of no group.
- * order (nullable: rows are in group order), offsets and tile_base from nerf_group_rows or nerf_group_offsets for the same
- * n and n_groups; rows are read and written where they are (row order[p] of x [n, K], y [n, N]).  order must not name a
- * row twice (nerf_group_rows never does).
- * The backward calls take the layer's output y when it had a ReLU, else NULL: dZ = d_y [y > 0].
- *   nerf_grouped_bwd_data:    d_x[i] = weight[g(i)]^T dZ[i] [n, K], zeros for rows of no group
- *   nerf_grouped_bwd_weights: d_weight[g] = sum dZ[i] x[i]^T, d_bias[g] (nullable) = sum dZ[i] over the rows of g; written,
+ * order, offsets and tile_base from nerf_group_rows or nerf_group_offsets (order 0 .. n-1) for the same n and n_groups; rows
+ * are read and written where they are (row order[p] of x [n, K], y [n, N]).  order must not name a row twice
+ * (nerf_group_rows never does).
+ * The backward calls take dZ [n, N], the gradient in front of the activation:
+ *   nerf_relu_bwd:            d_z[i] = d_y[i] where y[i] is not <= 0, else 0 (contiguous [n, N]; needed after a ReLU only)
+ *   nerf_grouped_bwd_data:    d_x[i] = weight[g(i)]^T d_z[i] [n, K], zeros for rows of no group
+ *   nerf_grouped_bwd_weights: d_weight[g] = sum d_z[i] x[i]^T, d_bias[g] (nullable) = sum d_z[i] over the rows of g; written,
  *                             zeros for a group without rows; fixed order of summation, no atomics
  * Products are summed in fp32 (fp32 operands: exact products).  n_groups <= 65535, K and N <= 65536.  *_ld: elements
  * between rows.  workspace 256-byte aligned. */
 int nerf_grouped_fwd(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets, const int32_t *tile_base,
                      int K, int N, const void *x, int64_t x_ld, const void *weight, const void *bias, int relu,
                      int precision, void *y, void *stream);
+int nerf_relu_bwd(int64_t n, int N, const void *d_y, int64_t d_y_ld, const void *y, int precision, void *d_z, void *stream);
 int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets, const int32_t *tile_base,
-                          int K, int N, const void *d_y, int64_t d_y_ld, const void *y, const void *weight, int precision,
-                          void *d_x, void *stream);
+                          int K, int N, const void *d_z, int64_t d_z_ld, const void *weight, int precision, void *d_x,
+                          void *stream);
 int64_t nerf_grouped_bwd_weights_workspace_bytes(int64_t n, int64_t n_groups, int K, int N);
 int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets,
-                             const int32_t *tile_base, int K, int N, const void *d_y, int64_t d_y_ld, const void *y,
-                             const void *x, int64_t x_ld, int precision, void *d_weight, void *d_bias, void *workspace,
+                             const int32_t *tile_base, int K, int N, const void *d_z, int64_t d_z_ld, const void *x,
+                             int64_t x_ld, int precision, void *d_weight, void *d_bias, void *workspace,
                              int64_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------

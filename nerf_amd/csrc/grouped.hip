@@ -8,13 +8,15 @@
 // number of tiles is known on the device only: the grid is the upper bound n / 128 + groups + 1 and a workgroup finds its
 // group in tile_base, the running number of tiles, with a 64-wide comparison.
 //
-// A workgroup of four waves multiplies 128 rows by 128 (64) outputs.  One contraction step of both operands, 32 KiB, is
-// copied into LDS by the memory system itself (global_load_lds, 16 bytes per lane), read whole into registers, and the
-// copy of the next step runs while the products of this one are formed: v_mfma_f32_32x32x16_{bf16,f16} or, in fp32,
-// v_mfma_f32_32x32x2_f32 (exact products, fp32 sums).  One buffer is enough for that, so three workgroups share a compute
-// unit and one's reads sit beside the others' products; a persistent form with two buffers and register staging was slower
-// (its copies had to be waited for together).  Operands that are not in whole aligned 16-byte pieces, and gradients that a
-// ReLU gates, go through registers instead of the direct copy, in the same loop.
+// Operands in whole aligned 16-byte pieces are copied into a ring of LDS buffers by the memory system itself
+// (global_load_lds, 16 bytes per lane) and multiplied by persistent workgroups, one per compute unit (stream_kernel,
+// wgrad_stream_kernel): v_mfma_f32_32x32x16_{bf16,f16} or, in fp32, v_mfma_f32_32x32x2_f32 (exact products, fp32 sums).
+// Anything else goes through registers, one workgroup per tile (linear_kernel, wgrad_kernel).
+//
+// Bounds: 256 -> 256 features move 1 KiB per row for 128 kflop, memory at 16 bits (floor 39 us for 196 608 rows; 57 forward,
+// 59 data gradient, 65 weight gradient) and the fp32 matrix instructions at 32 (65 536 rows: 56 us; 107, 108, 122).  1024 ->
+// 1024 features are bound by the copies into LDS, 29 bytes per ns and compute unit (65 536 rows fp16, 64 uneven groups: 220 to
+// 239 us; one group 170 us, 0.81 PFLOP/s, where a large library product reaches 1.06).
 //
 // A 16-byte piece holds the values of consecutive contraction indices of one row; operands whose contraction index is the
 // row (W in dX, both in dW) are read with ds_read_b64_tr_b16, which hands a lane four rows of its column, or in fp32 with
@@ -147,6 +149,17 @@ __device__ __forceinline__ Pack<T, piece<T>()> load_piece(const T* row, int c, i
     return __builtin_bit_cast(Pack<T, E>, two);
 }
 
+// columns c .. of a row of `cols`, written; nothing behind the row is touched
+template <typename T>
+__device__ __forceinline__ void put_row_piece(T* row, int c, int cols, const Pack<T, piece<T>()>& v) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Any { unsigned long long lo, hi; };
+    if (c + piece<T>() <= cols) *reinterpret_cast<Any*>(row + c) = __builtin_bit_cast(Any, v);
+    else
+#pragma unroll
+        for (int e = 0; e < piece<T>(); ++e)
+            if (c + e < cols) row[c + e] = v.v[e];
+}
+
 template <typename T, int E>
 __device__ __forceinline__ void put_piece(char* at, const Pack<T, E>& p) { *reinterpret_cast<Pack<T, E>*>(at) = p; }
 
@@ -156,22 +169,6 @@ __device__ __forceinline__ void gate_piece(Pack<T, E>& g, const Pack<T, E>& y) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
         if ((float)y.v[e] <= 0.0f) g.v[e] = (T)0.0f;
-}
-
-// The same on fragments.  A layer's output comes from its ReLU, which leaves no sign on a zero or a NaN, so "not zero" is
-// "greater than zero as an integer": two packed comparisons and a product per register instead of eight conversions.
-template <typename T>
-__device__ __forceinline__ typename El<T>::frag gate_frag(typename El<T>::frag g, typename El<T>::frag y) {
-    if constexpr (sizeof(T) == 2) {
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 one = 1, none = 0;
-        const s16x8 keep = __builtin_elementwise_max(__builtin_elementwise_min(__builtin_bit_cast(s16x8, y), one), none);
-        return __builtin_bit_cast(typename El<T>::frag, __builtin_bit_cast(s16x8, g) * keep);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) g[e] = __builtin_bit_cast(int, (float)y[e]) > 0 ? g[e] : 0.0f;
-        return g;
-    }
 }
 
 // ReLU with least = 0 and no sign bit in `bits` (keeps a NaN, without its sign); the identity with -inf and all bits
@@ -195,7 +192,7 @@ struct LinArgs {
     Rows rows;
     int C, O, tiles_o;           // contraction length, outputs, output tiles
     int64_t a_ld;
-    const void *a, *gate, *w, *bias;
+    const void *a, *w, *bias;
     int relu;
     void* out;
 };
@@ -432,15 +429,14 @@ __device__ __forceinline__ void block_tr(float, f32x16 (&c)[MI][NJ], F (&x)[MI],
     w[0] = F{n0, n1, n2, n3};
 }
 
-template <typename T, bool WT, bool GATE, int BN>
+template <typename T, bool WT, int BN>
 __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>(), WAVES = ST_THREADS / 64;
     constexpr int WM = BN == 64 ? 4 : 2, WO = WAVES / WM;                   // waves along rows and outputs
     constexpr int MI = TILE_ROWS / WM / 32, NJ = BN / WO / 32;
-    constexpr int A_BYTES = TILE_ROWS * 128, B_BYTES = WT ? tr_bytes<T, BN>() : BN * 128, Y_BYTES = GATE ? A_BYTES : 0;
-    constexpr int STAGE = A_BYTES + B_BYTES + Y_BYTES;
+    constexpr int A_BYTES = TILE_ROWS * 128, B_BYTES = WT ? tr_bytes<T, BN>() : BN * 128, STAGE = A_BYTES + B_BYTES;
     constexpr int NA = A_BYTES / 1024 / WAVES, NB = B_BYTES / 1024 / WAVES; // copies of a wave per step
-    constexpr int COPIES = NA + NB + (GATE ? NA : 0);
+    constexpr int COPIES = NA + NB;
     constexpr int STORES = MI * NJ * (sizeof(T) == 2 ? 2 : 4);              // stores of a wave per item
     static_assert(COPIES + 2 * STORES < 64, "vmcnt counts to 63");
     __shared__ __attribute__((aligned(1024))) char lds[3 * STAGE];
@@ -531,7 +527,7 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
 
         // ---- copies: step c_k of item c_item into buffer c_buf ----
         int c_item = 0, c_k = 0, c_buf = 0;
-        const T *pa[NA], *py[GATE ? NA : 1], *pb[NB];
+        const T *pa[NA], *pb[NB];
         auto copy_step = [&]() {
             if (c_k == 0) {
                 const int g = __builtin_amdgcn_readfirstlane(lds_int((unsigned)(uintptr_t)(lds_ptr)&d_grp[c_item]));
@@ -540,7 +536,6 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
                 for (int i = 0; i < NA; ++i) {
                     const int64_t row = lds_int(rows0 + (c_item * TILE_ROWS + a_row[i]) * 4);
                     pa[i] = (const T*)p.a + row * p.a_ld + a_q[i] * E;
-                    if constexpr (GATE) py[i] = (const T*)p.gate + row * C + a_q[i] * E;
                 }
                 const T* w = (const T*)p.w + (int64_t)g * O * C;
 #pragma unroll
@@ -562,26 +557,16 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
                 for (int i = 0; i < NA; ++i) copy_piece(pa[i], to + i * 1024);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) copy_piece(pb[i], to_b + i * 1024);
-                if constexpr (GATE)
-#pragma unroll
-                    for (int i = 0; i < NA; ++i) copy_piece(py[i], to + A_BYTES + B_BYTES + i * 1024);
             } else {                                                        // what lies behind the sum is read as zero
 #pragma unroll
                 for (int i = 0; i < NA; ++i) copy_piece(k0 + a_q[i] * E < C ? (const void*)pa[i] : (const void*)&ZERO_PIECE, to + i * 1024);
 #pragma unroll
                 for (int i = 0; i < NB; ++i)
                     copy_piece(k0 + (WT ? b_row[i] : b_q[i] * E) < C ? (const void*)pb[i] : (const void*)&ZERO_PIECE, to_b + i * 1024);
-                if constexpr (GATE)
-#pragma unroll
-                    for (int i = 0; i < NA; ++i)
-                        copy_piece(k0 + a_q[i] * E < C ? (const void*)py[i] : (const void*)&ZERO_PIECE, to + A_BYTES + B_BYTES + i * 1024);
             }
             if (c_item * nk + c_k + 1 < steps) {
 #pragma unroll
-                for (int i = 0; i < NA; ++i) {
-                    pa[i] += BK;
-                    if constexpr (GATE) py[i] += BK;
-                }
+                for (int i = 0; i < NA; ++i) pa[i] += BK;
 #pragma unroll
                 for (int i = 0; i < NB; ++i) pb[i] += WT ? (int64_t)BK * O : BK;
             }
@@ -597,31 +582,6 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-        };
-        auto multiply = [&](unsigned stage) {
-#pragma unroll
-            for (int s = 0; s < ROW_PIECES / 2; ++s) {
-                typename El<T>::frag fx[MI], fw[NJ];
-                if constexpr (!WT) {
-                    read_nt<typename El<T>::frag, MI, NJ>(fx, fw, fa[s] + stage, fb[s][0] + stage);
-                } else {
-                    read_rows<typename El<T>::frag, MI>(fx, fa[s] + stage);
-                    if constexpr (GATE) {
-                        typename El<T>::frag fy[MI];
-                        read_rows<typename El<T>::frag, MI>(fy, fa[s] + stage + A_BYTES + B_BYTES);
-#pragma unroll
-                        for (int i = 0; i < MI; ++i) fx[i] = gate_frag<T>(fx[i], fy[i]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        fw[j] = read_tr<T, BN * (int)sizeof(T)>(fb[s][j] + stage);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) acc[i][j] = El<T>::mfma(fw[j], fx[i], acc[i][j]);
-            }
         };
         auto finish_item = [&](int item) {
             const int o0 = __builtin_amdgcn_readfirstlane(lds_int((unsigned)(uintptr_t)(lds_ptr)&d_o0[item])) + o_off;
@@ -693,7 +653,7 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
         };
         auto end_step = [&]() {
             if (++k == nk) {
-                if constexpr (!GATE) settle<T, MI, NJ>(acc);
+                settle<T, MI, NJ>(acc);
                 finish_item(item);
                 clear();
                 k = 0;
@@ -703,48 +663,35 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
         };
         copy_step();
         copy_step();
-        if constexpr (GATE) {
-            // the gate stands between reading a fragment and multiplying it, so nothing is read ahead
-            for (int s = 0; s < steps; ++s) {
-                wait_step();
-                copy_step();
-                multiply(buf * STAGE);
-                end_step();
-                buf = buf == 2 ? 0 : buf + 1;
-            }
+        copy_step();
+        // The last fragments of a step are in registers one product step before its end: there the barrier frees its buffer for
+        // step s + 3 and the first fragments of step s + 1 are requested.
+        constexpr int S = ROW_PIECES / 2;
+        typename El<T>::frag fx[MI], fw[NJ];
+        wait_copies<2 * COPIES>();
+        __builtin_amdgcn_s_barrier();
+        if constexpr (!WT) {
+            read_nt<typename El<T>::frag, MI, NJ>(fx, fw, fa[0], fb[0][0]);
         } else {
-            // The last fragments of a step are in registers one product step before its end: there the barrier frees its
-            // buffer for step s + 3 and the first fragments of step s + 1 are requested.
-            constexpr int S = ROW_PIECES / 2;
-            typename El<T>::frag fx[MI], fw[NJ];
-            copy_step();
-            wait_copies<2 * COPIES>();
-            __builtin_amdgcn_s_barrier();
-            if constexpr (!WT) {
-                read_nt<typename El<T>::frag, MI, NJ>(fx, fw, fa[0], fb[0][0]);
-            } else {
-                read_rows<typename El<T>::frag, MI>(fx, fa[0]);
+            read_rows<typename El<T>::frag, MI>(fx, fa[0]);
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    fw[j] = read_tr<T, BN * (int)sizeof(T)>(fb[0][j]);
-                }
-            }
-            for (int s = 0; s < steps; ++s) {
+            for (int j = 0; j < NJ; ++j) fw[j] = read_tr<T, BN * (int)sizeof(T)>(fb[0][j]);
+        }
+        for (int s = 0; s < steps; ++s) {
 #pragma unroll
-                for (int u = 0; u < S; ++u) {
-                    unsigned stage = buf * STAGE;
-                    if (u == S - 1) {
-                        wait_step();
-                        buf = buf == 2 ? 0 : buf + 1;
-                        stage = buf * STAGE;
-                    }
-                    const int n = (u + 1) % S;
-                    if constexpr (!WT) block_nt<MI, NJ>(T(), acc, fx, fw, fa[n] + stage, fb[n][0] + stage);
-                    else block_tr<BN * (int)sizeof(T)>(T(), acc, fx, fw, fa[n] + stage, fb[n], stage);
+            for (int u = 0; u < S; ++u) {
+                unsigned stage = buf * STAGE;
+                if (u == S - 1) {
+                    wait_step();
+                    buf = buf == 2 ? 0 : buf + 1;
+                    stage = buf * STAGE;
                 }
-                copy_step();                                                // beside the last products
-                end_step();
+                const int n = (u + 1) % S;
+                if constexpr (!WT) block_nt<MI, NJ>(T(), acc, fx, fw, fa[n] + stage, fb[n][0] + stage);
+                else block_tr<BN * (int)sizeof(T)>(T(), acc, fx, fw, fa[n] + stage, fb[n], stage);
             }
+            copy_step();                                                    // beside the last products
+            end_step();
         }
         wait_copies<0>();                                                   // nothing may land once the rows are written anew
     }
@@ -753,7 +700,7 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
 // ---- through registers: any row length, any alignment ------------------------------------------------------------
 // The same product, one workgroup of four waves per tile of 128 rows x BN outputs.  Pieces are put together element by
 // element; a step is requested before the products of the one before it.
-template <typename T, bool WT, bool GATE, int BN>
+template <typename T, bool WT, int BN>
 __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();
     constexpr int A_BYTES = TILE_ROWS * 128;
@@ -801,10 +748,6 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
         for (int i = 0; i < NA; ++i) {
             const int64_t row = rows[i] < 0 ? 0 : rows[i];
             ra[i] = load_piece<T>((const T*)p.a + row * p.a_ld, k0 + q * E, C, rows[i] >= 0);
-            if constexpr (GATE) {
-                const Pack<T, E> y = load_piece<T>((const T*)p.gate + row * C, k0 + q * E, C, rows[i] >= 0);
-                gate_piece<T, E>(ra[i], y);
-            }
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -886,18 +829,11 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
                     put_piece<T, 4>(lds + (m_off + 32 * i + (lane & 31)) * PITCH + (o_off + 32 * j + 8 * h + 4 * (lane >> 5)) * 2, v);
                 }
         __syncthreads();
-        struct __attribute__((packed, aligned(sizeof(T)))) Any { unsigned long long lo, hi; };
 #pragma unroll
         for (int i = 0; i < TILE_ROWS * BN / E / THREADS; ++i) {
             const int at = tid + i * THREADS, m = at / (BN / E), c = at % (BN / E) * E, row = row_of[m];
             if (row < 0 || o0 + c >= O) continue;
-            const Pack<T, E> v = *reinterpret_cast<const Pack<T, E>*>(lds + m * PITCH + c * 2);
-            T* to = out + (int64_t)row * O + o0 + c;
-            if (o0 + c + E <= O) *reinterpret_cast<Any*>(to) = __builtin_bit_cast(Any, v);
-            else
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (o0 + c + e < O) to[e] = v.v[e];
+            put_row_piece<T>(out + (int64_t)row * O, o0 + c, O, *reinterpret_cast<const Pack<T, E>*>(lds + m * PITCH + c * 2));
         }
     } else {
 #pragma unroll
@@ -920,7 +856,7 @@ struct WgradArgs {
     int K, N, tiles_k, tiles_n;
     int chunk;                       // tiles of one workgroup
     int64_t x_ld, dy_ld;
-    const void *x, *dy, *y;
+    const void *x, *dy;
     void *dw, *db;
     float *part_w, *part_b;          // [2 * chunks][N * K], [2 * chunks][N]: slot 2c a group that came in from the left of
 };                                   // chunk c, slot 2c + 1 one that began in it and goes on to the right
@@ -930,7 +866,7 @@ struct WgradArgs {
 // have equal work however uneven the groups are.  A group that lies inside one chunk is finished here; the pieces of a longer
 // one go to the workspace and are added up in order by wgrad_join_kernel (no atomics: the result does not depend on timing).
 //
-// Rows of both operands (and of the layer's output, when it gates) are copied as they are into a ring of three LDS buffers,
+// Rows of both operands are copied as they are into a ring of three LDS buffers,
 // as in stream_kernel; a row behind the end of a tile is read from a piece of zeros.  The sum of dZ over the rows comes from
 // the fragments: the four waves that share a range of n take one product step of four each.
 constexpr int WG_TILES = 24;            // tiles whose rows are in LDS at a time
@@ -967,16 +903,15 @@ NERF_WG_BLOCK(__bf16, "v_mfma_f32_32x32x16_bf16")
 NERF_WG_BLOCK(_Float16, "v_mfma_f32_32x32x16_f16")
 #undef NERF_WG_BLOCK
 
-template <typename T, bool GATE, int BX>
+template <typename T, int BX>
 __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>(), WAVES = ST_THREADS / 64, BD = 128;
-    constexpr bool AHEAD = sizeof(T) == 2 && !GATE;                         // fragments read one product step ahead
+    constexpr bool AHEAD = sizeof(T) == 2;                                  // fragments read one product step ahead
     constexpr int PER_TILE = TILE_ROWS / BK, S = ROW_PIECES / 2;
     constexpr int MI = 2, NJ = BX / 4 / 32;                                 // waves: 2 along n, 4 along k
-    constexpr int D_BYTES = tr_bytes<T, BD>(), X_BYTES = tr_bytes<T, BX>(), Y_BYTES = GATE ? D_BYTES : 0;
-    constexpr int STAGE = D_BYTES + X_BYTES + Y_BYTES;
+    constexpr int D_BYTES = tr_bytes<T, BD>(), X_BYTES = tr_bytes<T, BX>(), STAGE = D_BYTES + X_BYTES;
     constexpr int ND = D_BYTES / 1024 / WAVES, NX = X_BYTES / 1024 / WAVES;
-    constexpr int COPIES = ND + NX + (GATE ? ND : 0);
+    constexpr int COPIES = ND + NX;
     constexpr int DPR = BD / E, XPR = BX / E;                               // pieces of a row
     __shared__ __attribute__((aligned(1024))) char lds[3 * STAGE];
     __shared__ int row_tab[WG_TILES][TILE_ROWS];
@@ -1120,11 +1055,6 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
 #pragma unroll
             for (int i = 0; i < NX; ++i)
                 copy_piece(rx[i] >= 0 ? (const void*)((const T*)p.x + rx[i] * p.x_ld + x_col[i]) : (const void*)&ZERO_PIECE, to + D_BYTES + (wave * NX + i) * 1024);
-            if constexpr (GATE)
-#pragma unroll
-                for (int i = 0; i < ND; ++i)
-                    copy_piece(rd[i] >= 0 ? (const void*)((const T*)p.y + rd[i] * (int64_t)N + d_col[i]) : (const void*)&ZERO_PIECE,
-                               to + D_BYTES + X_BYTES + (wave * ND + i) * 1024);
             if (c_step + 1 < steps) ++c_step;                               // behind the last step the last one is copied again
             c_buf = c_buf == 2 ? 0 : c_buf + 1;
         };
@@ -1183,10 +1113,7 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
 #pragma unroll
                 for (int u = 0; u < S; ++u) {
 #pragma unroll
-                    for (int i = 0; i < MI; ++i) {
-                        d[i] = read_tr<T, BD * (int)sizeof(T)>(fd[u][i] + stage);
-                        if constexpr (GATE) d[i] = gate_frag<T>(d[i], read_tr<T, BD * (int)sizeof(T)>(fd[u][i] + stage + D_BYTES + X_BYTES));
-                    }
+                    for (int i = 0; i < MI; ++i) d[i] = read_tr<T, BD * (int)sizeof(T)>(fd[u][i] + stage);
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) x[j] = read_tr<T, BX * (int)sizeof(T)>(fx[u][j] + stage);
 #pragma unroll
@@ -1208,7 +1135,7 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
 // however uneven the groups are.  A group that lies inside one chunk is finished here; the pieces of a longer one go to
 // the workspace and are added up in order by wgrad_join_kernel (no atomics: the result does not depend on timing).
 // The same through registers: any row length, any alignment.
-template <typename T, bool GATE, int BT>
+template <typename T, int BT>
 __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();                       // rows of one step
     constexpr int PER_TILE = TILE_ROWS / BK, S = ROW_PIECES / 2;
@@ -1275,10 +1202,6 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
             const T *xrow = (const T*)p.x + row * p.x_ld, *drow = (const T*)p.dy + row * p.dy_ld;
             rx[j] = load_piece<T>(xrow, k0 + pq[j] * E, K, ok);
             rd[j] = load_piece<T>(drow, n0 + pq[j] * E, N, ok);
-            if constexpr (GATE) {
-                const Pack<T, E> y = load_piece<T>((const T*)p.y + row * N, n0 + pq[j] * E, N, ok);
-                gate_piece<T, E>(rd[j], y);
-            }
         }
     };
     f32x16 acc[M][M];
@@ -1389,6 +1312,23 @@ __global__ __launch_bounds__(THREADS) void wgrad_join_kernel(WgradArgs p) {
     else ((T*)p.db)[(int64_t)g * p.N + (i - NK)] = (T)sum;
 }
 
+// dZ = dY where the ReLU let something through.  Memory bound: 196 608 x 256 bf16 in 51 us, 5.9 TB/s.  Written out once, because
+// the gate inside the two products costs more: their tiles are bound by what they copy into LDS, and the gate is a third
+// operand (in the same shape, data gradient 125 us gated and 59 not, weight gradient 116 and 66).
+template <typename T>
+__global__ __launch_bounds__(THREADS) void relu_bwd_kernel(int64_t n, int N, const T* dy, int64_t ld, const T* y, T* dz) {
+    constexpr int E = piece<T>();
+    const int pieces = (N + E - 1) / E;
+    const int64_t total = n * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * THREADS) {
+        const int64_t row = total <= 0x7fffffff ? (int)i / pieces : i / pieces;
+        const int c = (int)(i - row * pieces) * E;
+        Pack<T, E> g = load_piece<T>(dy + row * ld, c, N, true);
+        gate_piece<T, E>(g, load_piece<T>(y + row * N, c, N, true));
+        put_row_piece<T>(dz + row * N, c, N, g);
+    }
+}
+
 static inline bool sizes_ok(int64_t n, int64_t n_groups, int K, int N) {
     return n >= 0 && n <= grp::MAX_ROWS && n_groups >= 1 && n_groups <= 65535 && K >= 1 && K <= 65536 && N >= 1 && N <= 65536;
 }
@@ -1402,10 +1342,10 @@ struct WgradPlan {
     int64_t chunks, part_w, part_b, bytes;
 };
 // wide: whole aligned pieces (one workgroup per compute unit), else through registers (two)
-static WgradPlan wgrad_plan(int64_t n, int64_t n_groups, int K, int N, bool wide, bool gate, int precision) {
+static WgradPlan wgrad_plan(int64_t n, int64_t n_groups, int K, int N, bool wide, int precision) {
     WgradPlan w = {};
     w.bd = !wide && K <= 64 && N <= 64 ? 64 : 128;
-    w.bx = wide && !gate && precision != NERF_PREC_FP32 && K > 128 ? 256 : w.bd;
+    w.bx = wide && precision != NERF_PREC_FP32 && K > 128 ? 256 : w.bd;
     w.tiles_n = (N + w.bd - 1) / w.bd;
     w.tiles_k = (K + w.bx - 1) / w.bx;
     const int64_t tiles = max_tiles(n, n_groups), blocks = (int64_t)w.tiles_n * w.tiles_k;
@@ -1433,7 +1373,7 @@ static int launch_linear(const LinArgs& args, int precision, bool wide, void* st
     if (wide) {
         // Output tile: the width with the least work on the busiest compute unit, ceil(items / 256) tiles of BN + an
         // overhead for reading the rows once more per tile (which weighs more where the products are fast).
-        const int most = p.gate || precision == NERF_PREC_FP32 ? 128 : 256, extra = precision == NERF_PREC_FP32 ? 8 : 32;
+        const int most = precision == NERF_PREC_FP32 ? 128 : 256, extra = precision == NERF_PREC_FP32 ? 8 : 32;
         int bn = 64;
         int64_t least = -1;
         for (int b = 64; b <= most; b *= 2) {
@@ -1443,17 +1383,13 @@ static int launch_linear(const LinArgs& args, int precision, bool wide, void* st
         p.tiles_o = (p.O + bn - 1) / bn;
         int64_t grid = (tiles * p.tiles_o + 7) / 8 * 8;
         if (grid > 256) grid = 256;
-#define NERF_ST(T, GATE, BN) hipLaunchKernelGGL((stream_kernel<T, WT, GATE, BN>), dim3((unsigned)grid), dim3(ST_THREADS), 0, st, p)
+#define NERF_ST(T, BN) hipLaunchKernelGGL((stream_kernel<T, WT, BN>), dim3((unsigned)grid), dim3(ST_THREADS), 0, st, p)
 #define NERF_CALL(T)                                                \
     do {                                                            \
-        if constexpr (WT) {                                         \
-            if (p.gate && bn == 128) { NERF_ST(T, true, 128); break; } \
-            if (p.gate) { NERF_ST(T, true, 64); break; }            \
-        }                                                           \
         if constexpr (sizeof(T) == 2)                               \
-            if (bn == 256) { NERF_ST(T, false, 256); break; }       \
-        if (bn == 128) NERF_ST(T, false, 128);                      \
-        else NERF_ST(T, false, 64);                                 \
+            if (bn == 256) { NERF_ST(T, 256); break; }              \
+        if (bn == 128) NERF_ST(T, 128);                             \
+        else NERF_ST(T, 64);                                        \
     } while (0)
         NERF_ELEM_DISPATCH(precision, NERF_CALL);
 #undef NERF_CALL
@@ -1464,23 +1400,13 @@ static int launch_linear(const LinArgs& args, int precision, bool wide, void* st
     p.tiles_o = (p.O + bn - 1) / bn;
     const int64_t grid = xcd_grid(tiles * p.tiles_o, 1);
     NERF_REQUIRE(grid < ((int64_t)1 << 31), NERF_E_SHAPE);
-#define NERF_LIN(T, GATE)                                                                                                      \
+#define NERF_CALL(T)                                                                                                           \
     do {                                                                                                                       \
-        if (bn == 128) hipLaunchKernelGGL((linear_kernel<T, WT, GATE, 128>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);   \
-        else hipLaunchKernelGGL((linear_kernel<T, WT, GATE, 64>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);              \
-    } while (0)
-#define NERF_CALL(T)                                      \
-    do {                                                  \
-        if constexpr (WT) {                               \
-            if (p.gate) NERF_LIN(T, true);                \
-            else NERF_LIN(T, false);                      \
-        } else {                                          \
-            NERF_LIN(T, false);                           \
-        }                                                 \
+        if (bn == 128) hipLaunchKernelGGL((linear_kernel<T, WT, 128>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);         \
+        else hipLaunchKernelGGL((linear_kernel<T, WT, 64>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);                    \
     } while (0)
     NERF_ELEM_DISPATCH(precision, NERF_CALL);
 #undef NERF_CALL
-#undef NERF_LIN
     return nerf_launch_status();
 }
 
@@ -1505,56 +1431,70 @@ extern "C" int nerf_grouped_fwd(int64_t n, int64_t n_groups, const int32_t* orde
     return gl::launch_linear<false>(p, precision, wide, stream);
 }
 
-extern "C" int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t* order, const int32_t* offsets, const int32_t* tile_base,
-                                     int K, int N, const void* d_y, int64_t d_y_ld, const void* y, const void* weight, int precision,
-                                     void* d_x, void* stream) {
+extern "C" int nerf_relu_bwd(int64_t n, int N, const void* d_y, int64_t d_y_ld, const void* y, int precision, void* d_z, void* stream) {
     using namespace nerf;
-    NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && d_y_ld >= N, NERF_E_SHAPE);
+    NERF_REQUIRE(gl::sizes_ok(n, 1, 1, N) && d_y_ld >= N, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(order && offsets && tile_base && d_y && weight && d_x, NERF_E_NULL);
+    NERF_REQUIRE(d_y && y && d_z, NERF_E_NULL);
     const int es = elem_bytes(precision), E = 16 / es;
-    NERF_REQUIRE(nerf_aligned(d_y, (uintptr_t)es) && nerf_aligned(weight, (uintptr_t)es) && nerf_aligned(d_x, (uintptr_t)es) &&
-                 nerf_aligned(y, (uintptr_t)es), NERF_E_ALIGN);
-    const bool wide = K % E == 0 && N % E == 0 && d_y_ld % E == 0 && nerf_aligned(d_y, 16) && nerf_aligned(weight, 16) &&
-                      nerf_aligned(d_x, 16) && nerf_aligned(y, 16);
+    NERF_REQUIRE(nerf_aligned(d_y, (uintptr_t)es) && nerf_aligned(y, (uintptr_t)es) && nerf_aligned(d_z, (uintptr_t)es), NERF_E_ALIGN);
+    const int64_t pieces = n * ((N + E - 1) / E), most = (int64_t)1 << 22;
+    const unsigned grid = (unsigned)((pieces + gl::THREADS - 1) / gl::THREADS < most ? (pieces + gl::THREADS - 1) / gl::THREADS : most);
+#define NERF_CALL(T) \
+    hipLaunchKernelGGL(gl::relu_bwd_kernel<T>, dim3(grid), dim3(gl::THREADS), 0, (hipStream_t)stream, n, N, (const T*)d_y, d_y_ld, (const T*)y, (T*)d_z)
+    NERF_ELEM_DISPATCH(precision, NERF_CALL);
+#undef NERF_CALL
+    return nerf_launch_status();
+}
+
+extern "C" int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t* order, const int32_t* offsets, const int32_t* tile_base,
+                                     int K, int N, const void* d_z, int64_t d_z_ld, const void* weight, int precision, void* d_x,
+                                     void* stream) {
+    using namespace nerf;
+    NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && d_z_ld >= N, NERF_E_SHAPE);
+    NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
+    if (n == 0) return NERF_OK;
+    NERF_REQUIRE(order && offsets && tile_base && d_z && weight && d_x, NERF_E_NULL);
+    const int es = elem_bytes(precision), E = 16 / es;
+    NERF_REQUIRE(nerf_aligned(d_z, (uintptr_t)es) && nerf_aligned(weight, (uintptr_t)es) && nerf_aligned(d_x, (uintptr_t)es), NERF_E_ALIGN);
+    const bool wide = K % E == 0 && N % E == 0 && d_z_ld % E == 0 && nerf_aligned(d_z, 16) && nerf_aligned(weight, 16) && nerf_aligned(d_x, 16);
     gl::LinArgs p = {};
     p.rows = {n, (int)n_groups, order, offsets, tile_base};
-    p.C = N; p.O = K; p.a = d_y; p.a_ld = d_y_ld; p.gate = y; p.w = weight; p.out = d_x;
+    p.C = N; p.O = K; p.a = d_z; p.a_ld = d_z_ld; p.w = weight; p.out = d_x;
     return gl::launch_linear<true>(p, precision, wide, stream);
 }
 
 extern "C" int64_t nerf_grouped_bwd_weights_workspace_bytes(int64_t n, int64_t n_groups, int K, int N) {
     if (!nerf::gl::sizes_ok(n, n_groups, K, N)) return NERF_E_SHAPE;
-    // what alignment, gate and type lead to differs in the number of chunks: enough for any of them
+    // what alignment and type lead to differs in the number of chunks: enough for any of them
     int64_t most = 0;
     for (int way = 0; way < 3; ++way) {
-        const int64_t b = nerf::gl::wgrad_plan(n, n_groups, K, N, way > 0, way > 1, NERF_PREC_BF16).bytes;
+        const int64_t b = nerf::gl::wgrad_plan(n, n_groups, K, N, way > 0, way > 1 ? NERF_PREC_FP32 : NERF_PREC_BF16).bytes;
         if (b > most) most = b;
     }
     return most;
 }
 
 extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32_t* order, const int32_t* offsets,
-                                        const int32_t* tile_base, int K, int N, const void* d_y, int64_t d_y_ld, const void* y,
-                                        const void* x, int64_t x_ld, int precision, void* d_weight, void* d_bias, void* workspace,
+                                        const int32_t* tile_base, int K, int N, const void* d_z, int64_t d_z_ld, const void* x,
+                                        int64_t x_ld, int precision, void* d_weight, void* d_bias, void* workspace,
                                         int64_t workspace_bytes, void* stream) {
     using namespace nerf;
-    NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && d_y_ld >= N && x_ld >= K, NERF_E_SHAPE);
+    NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && d_z_ld >= N && x_ld >= K, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(order && offsets && tile_base && d_y && x && d_weight && workspace, NERF_E_NULL);
+    NERF_REQUIRE(order && offsets && tile_base && d_z && x && d_weight && workspace, NERF_E_NULL);
     const int es = elem_bytes(precision), E = 16 / es;
-    NERF_REQUIRE(nerf_aligned(d_y, (uintptr_t)es) && nerf_aligned(x, (uintptr_t)es) && nerf_aligned(y, (uintptr_t)es) &&
-                 nerf_aligned(d_weight, (uintptr_t)es) && nerf_aligned(d_bias, (uintptr_t)es) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
+    NERF_REQUIRE(nerf_aligned(d_z, (uintptr_t)es) && nerf_aligned(x, (uintptr_t)es) && nerf_aligned(d_weight, (uintptr_t)es) &&
+                 nerf_aligned(d_bias, (uintptr_t)es) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
     NERF_REQUIRE(workspace_bytes >= nerf_grouped_bwd_weights_workspace_bytes(n, n_groups, K, N), NERF_E_WORKSPACE);
-    const bool wide = K % E == 0 && N % E == 0 && d_y_ld % E == 0 && x_ld % E == 0 && nerf_aligned(d_y, 16) && nerf_aligned(x, 16) &&
-                      nerf_aligned(y, 16);
-    const gl::WgradPlan w = gl::wgrad_plan(n, n_groups, K, N, wide, y != nullptr, precision);
+    const bool wide = K % E == 0 && N % E == 0 && d_z_ld % E == 0 && x_ld % E == 0 && nerf_aligned(d_z, 16) && nerf_aligned(x, 16);
+    const gl::WgradPlan w = gl::wgrad_plan(n, n_groups, K, N, wide, precision);
     gl::WgradArgs p = {};
     p.rows = {n, (int)n_groups, order, offsets, tile_base};
     p.K = K; p.N = N; p.tiles_k = w.tiles_k; p.tiles_n = w.tiles_n; p.chunk = w.chunk;
-    p.x_ld = x_ld; p.dy_ld = d_y_ld; p.x = x; p.dy = d_y; p.y = y; p.dw = d_weight; p.db = d_bias;
+    p.x_ld = x_ld; p.dy_ld = d_z_ld; p.x = x; p.dy = d_z; p.dw = d_weight; p.db = d_bias;
     p.part_w = (float*)((char*)workspace + w.part_w);
     p.part_b = (float*)((char*)workspace + w.part_b);
     const int64_t blocks = (int64_t)w.tiles_n * w.tiles_k;
@@ -1562,28 +1502,21 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
     NERF_REQUIRE(grid < ((int64_t)1 << 31), NERF_E_SHAPE);
     hipStream_t st = (hipStream_t)stream;
     const dim3 join((unsigned)(((int64_t)N * K + N + gl::THREADS - 1) / gl::THREADS), (unsigned)n_groups);
-#define NERF_WG(T, GATE, BT) hipLaunchKernelGGL((gl::wgrad_kernel<T, GATE, BT>), dim3((unsigned)grid), dim3(gl::THREADS), 0, st, p)
-#define NERF_WS(T, GATE, BX) \
-    hipLaunchKernelGGL((gl::wgrad_stream_kernel<T, GATE, BX>), dim3((unsigned)grid), dim3(gl::ST_THREADS), 0, st, p)
-#define NERF_WG_G(T, GATE)                                  \
-    do {                                                    \
-        if (wide) NERF_WS(T, GATE, 128);                    \
-        else if (w.bd == 128) NERF_WG(T, GATE, 128);        \
-        else NERF_WG(T, GATE, 64);                          \
-    } while (0)
+#define NERF_WG(T, BT) hipLaunchKernelGGL((gl::wgrad_kernel<T, BT>), dim3((unsigned)grid), dim3(gl::THREADS), 0, st, p)
+#define NERF_WS(T, BX) hipLaunchKernelGGL((gl::wgrad_stream_kernel<T, BX>), dim3((unsigned)grid), dim3(gl::ST_THREADS), 0, st, p)
 #define NERF_CALL(T)                                                                                   \
     do {                                                                                               \
         bool done = false;                                                                             \
         if constexpr (sizeof(T) == 2)                                                                  \
-            if (w.bx == 256) { NERF_WS(T, false, 256); done = true; }                                  \
+            if (w.bx == 256) { NERF_WS(T, 256); done = true; }                                         \
         if (done) {}                                                                                   \
-        else if (p.y) NERF_WG_G(T, true);                                                              \
-        else NERF_WG_G(T, false);                                                                      \
+        else if (wide) NERF_WS(T, 128);                                                                \
+        else if (w.bd == 128) NERF_WG(T, 128);                                                         \
+        else NERF_WG(T, 64);                                                                           \
         hipLaunchKernelGGL(gl::wgrad_join_kernel<T>, join, dim3(gl::THREADS), 0, st, p);               \
     } while (0)
     NERF_ELEM_DISPATCH(precision, NERF_CALL);
 #undef NERF_CALL
-#undef NERF_WG_G
 #undef NERF_WS
 #undef NERF_WG
     return nerf_launch_status();

@@ -930,7 +930,11 @@ class _GroupedLinear(torch.autograd.Function):
             return (torch.zeros((0, K), dtype=d_y.dtype, device=dev) if need_x else None, torch.zeros_like(weight) if need_w else None,
                     torch.zeros((G, N), dtype=d_y.dtype, device=dev) if need_b else None, None, None)
         g, ld = _row_major(d_y)
-        at = (n, G, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N, g.data_ptr(), ld, _ptr(y))
+        if y is not None and (need_x or need_w or need_b):
+            dz = torch.empty((n, N), dtype=g.dtype, device=dev)
+            _call("nerf_relu_bwd", "relu_bwd", dev, n, n, N, g.data_ptr(), ld, y.data_ptr(), prec, dz.data_ptr())
+            g, ld = dz, N
+        at = (n, G, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N, g.data_ptr(), ld)
         if need_x:
             dx = torch.empty((n, K), dtype=g.dtype, device=dev)
             _call("nerf_grouped_bwd_data", "grouped_bwd_data", dev, n, *at, weight.data_ptr(), prec, dx.data_ptr())

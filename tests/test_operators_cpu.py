@@ -72,18 +72,22 @@ def test_cabi_refuses_bad_grouped_layer_arguments(lib):
     need = lib.nerf_grouped_bwd_weights_workspace_bytes(5000, 3, 40, 24)
     for G, K, N in ((0, 40, 24), (65536, 40, 24), (3, 0, 24), (3, 40, 0), (3, 65537, 24), (3, 40, 65537)):
         assert f(5000, G, P, P, P, K, N, P, 70000, P, P, 0, 0, P, None) == SHAPE
-        assert d(5000, G, P, P, P, K, N, P, 70000, None, P, 0, P, None) == SHAPE
+        assert d(5000, G, P, P, P, K, N, P, 70000, P, 0, P, None) == SHAPE
         assert lib.nerf_grouped_bwd_weights_workspace_bytes(5000, G, K, N) == SHAPE
-        assert w(5000, G, P, P, P, K, N, P, 70000, None, P, 70000, 0, P, P, P, need, None) == SHAPE
-    assert f(5000, 3, P, P, P, 40, 24, P, 39, P, P, 0, 0, P, None) == SHAPE and d(5000, 3, P, P, P, 40, 24, P, 23, None, P, 0, P, None) == SHAPE
-    assert f(5000, 3, P, P, P, 40, 24, P, 40, P, P, 0, 3, P, None) == DTYPE and d(5000, 3, P, P, P, 40, 24, P, 24, None, P, -1, P, None) == DTYPE
+        assert w(5000, G, P, P, P, K, N, P, 70000, P, 70000, 0, P, P, P, need, None) == SHAPE
+    assert f(5000, 3, P, P, P, 40, 24, P, 39, P, P, 0, 0, P, None) == SHAPE and d(5000, 3, P, P, P, 40, 24, P, 23, P, 0, P, None) == SHAPE
+    assert f(5000, 3, P, P, P, 40, 24, P, 40, P, P, 0, 3, P, None) == DTYPE and d(5000, 3, P, P, P, 40, 24, P, 24, P, -1, P, None) == DTYPE
     assert f(5000, 3, None, P, P, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL
     assert f(5000, 3, P, None, P, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL and f(5000, 3, P, P, None, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL
-    assert f(5000, 3, P, P, P, 40, 24, P + 1, 40, P, P, 0, 0, P, None) == ALIGN and d(5000, 3, P, P, P, 40, 24, P, 24, P + 2, P, 2, P, None) == ALIGN
-    assert w(5000, 3, P, P, P, 40, 24, P, 24, None, P, 40, 0, P, P, P, need - 1, None) == WORK
-    assert w(5000, 3, P, P, P, 40, 24, P, 24, None, P, 40, 0, P, P, P + 8, need, None) == ALIGN
-    assert w(5000, 3, P, P, P, 40, 24, P, 24, None, P, 40, 0, None, P, P, need, None) == NULL
+    assert f(5000, 3, P, P, P, 40, 24, P + 1, 40, P, P, 0, 0, P, None) == ALIGN and d(5000, 3, P, P, P, 40, 24, P, 24, P + 2, 2, P, None) == ALIGN
+    assert w(5000, 3, P, P, P, 40, 24, P, 24, P, 40, 0, P, P, P, need - 1, None) == WORK
+    assert w(5000, 3, P, P, P, 40, 24, P, 24, P, 40, 0, P, P, P + 8, need, None) == ALIGN
+    assert w(5000, 3, P, P, P, 40, 24, P, 24, P, 40, 0, None, P, P, need, None) == NULL
     assert f(0, 3, None, None, None, 40, 24, None, 40, None, None, 0, 0, None, None) == OK
+    r = lib.nerf_relu_bwd
+    assert r(-1, 24, P, 24, P, 0, P, None) == r(50, 0, P, 24, P, 0, P, None) == r(50, 24, P, 23, P, 0, P, None) == SHAPE
+    assert r(50, 24, P, 24, P, 3, P, None) == DTYPE and r(50, 24, P, 24, P + 1, 0, P, None) == r(50, 24, P, 24, P, 2, P + 2, None) == ALIGN
+    assert r(50, 24, None, 24, P, 0, P, None) == r(50, 24, P, 24, None, 0, P, None) == NULL and r(0, 24, None, 24, None, 0, None, None) == OK
 
 
 def test_cabi_refuses_bad_scan_arguments(lib):
