@@ -428,8 +428,7 @@ int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32_t *order, 
  * models/nerf.py:430-456 for features of any width.  gate_shared: one gate per sample, else one per channel.
  * *_sb, *_st: elements between sequences and between samples (0 to repeat); channels are contiguous.  reverse: from the
  * last sample to the first.  state, last, d_last, d_state: fp32 [B, D]; h, d_h, d_value [B, T, D], d_gate [B, T, D or 1]
- * contiguous.  Where D is a multiple of 16 bytes, value, h, d_h and d_value (and a gate per channel) are 16-byte aligned
- * and their strides multiples of it (NERF_E_ALIGN).
+ * contiguous.
  * states (nullable in the forward): nerf_scan_states_floats floats, the fp32 states the backward starts from.
  * Backward: d_h, d_last nullable = 0; d_gate, d_value, d_state nullable = not wanted.  T = 0 writes nothing.
  * The product of consecutive gates has to stay in the range of fp32 wherever the state in front of them is not zero. */

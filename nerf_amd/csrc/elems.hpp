@@ -20,6 +20,21 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& x) {
     *reinterpret_cast<Pack<T, V>*>(p) = x;
 }
 
+// The same at any address that the elements themselves are aligned to (memory instructions ask for no more); a row of `cols`
+// elements is then covered whatever its length by pieces that begin at min(c, cols - V): the last one repeats some columns.
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+    T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_any(const T* p) {
+    return __builtin_bit_cast(Pack<T, V>, *reinterpret_cast<const Loose<T, V>*>(p));
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_any(T* p, const Pack<T, V>& x) {
+    *reinterpret_cast<Loose<T, V>*>(p) = __builtin_bit_cast(Loose<T, V>, x);
+}
+
 // elements of a 16-byte access
 template <typename T>
 constexpr int full_vec() { return 16 / (int)sizeof(T); }

@@ -989,12 +989,12 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
 # gated linear recurrence along a ray
 # ---------------------------------------------------------------------------
 
-def _scan_input(t: torch.Tensor, vec: int) -> Tuple[torch.Tensor, int, int]:
-    """(tensor, elements between sequences, between samples) as the kernels read it: channels contiguous, pieces of ``vec``
-    elements aligned; copied when it is not."""
+def _scan_input(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """(tensor, elements between sequences, between samples) as the kernels read it, with its channels contiguous; copied when
+    they are not."""
     (B, T, D), (sb, st, sc) = t.shape, t.stride()
     sb, st = sb if B > 1 else 0, st if T > 1 else 0
-    if D > 1 and sc != 1 or sb % vec or st % vec or t.data_ptr() % (vec * t.element_size()):
+    if D > 1 and sc != 1:
         t = t.clone(memory_format=torch.contiguous_format)
         sb, st = T * D if B > 1 else 0, D if T > 1 else 0
     return t, sb, st
@@ -1003,11 +1003,9 @@ def _scan_input(t: torch.Tensor, vec: int) -> Tuple[torch.Tensor, int, int]:
 def _scan_fwd(gate, value, state, reverse, need):
     """(h, last, gate, value and state as they were read, the states the backward starts from)"""
     (B, T, D), dev, prec = value.shape, value.device, _ELEM[value.dtype]
-    full = 16 // value.element_size()
     shared = gate.shape[2] == 1 and D > 1
-    vec = full if D % full == 0 else 1
-    value, vsb, vst = _scan_input(value, vec)
-    gate, gsb, gst = _scan_input(gate, 1 if shared else vec)
+    value, vsb, vst = _scan_input(value)
+    gate, gsb, gst = _scan_input(gate)
     state = None if state is None else state.contiguous()
     h = torch.empty((B, T, D), dtype=value.dtype, device=dev)
     last = torch.empty((B, D), dtype=torch.float32, device=dev)
@@ -1039,14 +1037,9 @@ class _GatedScan(torch.autograd.Function):
         (B, T, D), dev, prec = value.shape, value.device, _ELEM[value.dtype]
         need_gate, need_value, need_state = ctx.needs_input_grad[:3]
         shared = gate.shape[2] == 1 and D > 1
-        full = 16 // value.element_size()
-        vec = full if D % full == 0 else 1
-        gate, gsb, gst = _scan_input(gate, 1 if shared else vec)
-        value, vsb, vst = _scan_input(value, vec)
-        if d_h is not None:
-            d_h = d_h.contiguous()
-            if d_h.data_ptr() % (vec * d_h.element_size()):
-                d_h = d_h.clone()
+        gate, gsb, gst = _scan_input(gate)
+        value, vsb, vst = _scan_input(value)
+        d_h = None if d_h is None else d_h.contiguous()
         d_last = None if d_last is None else d_last.contiguous()
         d_gate = torch.empty((B, T, 1 if shared else D), dtype=value.dtype, device=dev) if need_gate else None
         d_value = torch.empty((B, T, D), dtype=value.dtype, device=dev) if need_value else None

@@ -97,7 +97,7 @@ def test_group_rows_of_nothing_and_row_groups():
 # ---- rows of a table -----------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,rows,dim,kind", [(1, 1, 1, "one"), (1024, 100, 48, "random"), (513, 7, 63, "random"), (5000, 9, 3, "skewed"),
+@pytest.mark.parametrize("n,rows,dim,kind", [(1, 1, 1, "one"), (1024, 100, 48, "random"), (513, 7, 63, "random"), (5000, 9, 3, "skewed"), (30000, 50, 9, "skewed"), (30000, 1, 131, "one"), (20000, 30000, 67, "random"), (3000, 40, 5, "random"),
                                              (40000, 3, 16, "skewed"), (30000, 1, 40, "one"), (3000, 20000, 8, "random"), (70000, 300, 48, "runs"),
                                              (2000, 50, 1000, "random"), (600, 11, 517, "skewed"), (64, 5, 2, "none"), (200000, 4096, 4, "skewed"), (4096, 1024, 20, "random"), (4096, 1025, 20, "random"), (4097, 10, 24, "skewed"),
                                              (3000, 2, 1, "one")])
@@ -346,7 +346,7 @@ def check_scan(gate, value, st, d_h, d_last, reverse, ga, va, sa):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("B,T,D", [(1, 1, 1), (3, 1, 256), (5, 2, 3), (2, 64, 64), (7, 192, 64), (3, 100, 4), (9, 33, 40), (2, 129, 520), (1, 1000, 16),
-                                   (4, 257, 67), (300, 5, 8), (1, 20000, 8), (2, 9000, 3), (1, 3000, 256), (2, 1500, 1), (1, 2500, 130)])
+                                   (4, 257, 67), (300, 5, 8), (1, 20000, 8), (2, 9000, 3), (1, 3000, 256), (2, 1500, 1), (1, 2500, 130), (50, 300, 9), (2, 5000, 13), (6, 70, 8)])
 def test_gated_scan(B, T, D, dtype):
     for k, (shared, reverse, state) in enumerate(((True, False, True), (False, True, False), (True, True, False), (False, False, True))):
         if T * B * D > 300000 and k > 1:

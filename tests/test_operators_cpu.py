@@ -102,14 +102,13 @@ def test_cabi_refuses_bad_scan_arguments(lib):
         return f(*a)
     assert call(a0=-1) == call(a1=-1) == call(a2=0) == call(a2=65537) == call(a4=-1) == call(a9=-8) == SHAPE
     assert call(a12=3) == DTYPE and call(a3=None) == call(a7=None) == call(a13=None) == call(a14=None) == call(a16=None) == NULL
-    assert call(a7=P + 8) == call(a9=36) == call(a13=P + 2) == call(a3=P + 1) == call(a16=P + 4) == ALIGN and call(a17=need - 1) == WORK
-    assert call(a3=P + 2, a17=0) == WORK                                       # a shared gate needs no more than its own alignment
-    assert call(a6=0, a5=33) == ALIGN                                          # one per channel does
+    assert call(a7=P + 1) == call(a13=P + 1) == call(a3=P + 1) == call(a14=P + 2) == call(a16=P + 4) == ALIGN and call(a17=need - 1) == WORK
+    assert call(a7=P + 2, a8=36001, a9=33, a3=P + 2, a17=0) == WORK            # no more than the elements' own alignment is asked for
     assert f(0, 5, 8, None, 0, 0, 1, None, 0, 0, None, 0, 0, None, None, None, None, 0, None) == OK
     assert lib.nerf_scan_states_floats(2, 5000, 32, 7) == DTYPE and lib.nerf_scan_workspace_bytes(2, 5000, 0, 1, 0, 0) == SHAPE
     need = lib.nerf_scan_workspace_bytes(2, 5000, 32, 1, 1, 0)
     good_b = [2, 5000, 32, P, 5000, 1, 1, P, 160000, 32, None, P, P, P, 0, 0, P, P, P, P, need, None]
-    for at, bad, code in ((0, -1, SHAPE), (15, 5, DTYPE), (11, None, NULL), (3, None, NULL), (12, P + 2, ALIGN), (17, P + 8, ALIGN), (20, need - 1, WORK)):
+    for at, bad, code in ((0, -1, SHAPE), (15, 5, DTYPE), (11, None, NULL), (3, None, NULL), (12, P + 1, ALIGN), (17, P + 1, ALIGN), (20, need - 1, WORK)):
         a = list(good_b)
         a[at] = bad
         assert b(*a) == code, at
