@@ -287,7 +287,7 @@ __global__ __launch_bounds__(THREADS) void bwd_join_kernel(BwdArgs a, T* __restr
 
 // Few positions and few rows: a workgroup per table row looks through all ids, keeps the positions that name its row (in
 // order, each wave its own quarter) and sums their rows of d_out, one launch instead of five.  1024 positions over 100 rows
-// of 48 fp32: 16 us for the call with grouping, see the limit below for where it stops paying.
+// of 48 fp32: 5 us, grouped first 16; small_call() says where it stops paying.
 template <typename T, int VEC, typename ID>
 __global__ __launch_bounds__(THREADS) void bwd_small_kernel(int n, const ID* __restrict__ ids, int dim, int lpr, const T* __restrict__ d_out,
                                                             int64_t ld, float scale, T* __restrict__ d_table) {
@@ -312,6 +312,7 @@ __global__ __launch_bounds__(THREADS) void bwd_small_kernel(int n, const ID* __r
         cnt += __popcll(m);
     }
     if (lane == 0) count[wave] = cnt;
+    const bool any = __syncthreads_or(cnt);                        // a row that nothing reads gets zeros, whatever the scale is
     __syncthreads();
     const int groups = THREADS / lpr, sub = (int)threadIdx.x / lpr, l = (int)threadIdx.x % lpr;
     for (int col0 = l * VEC; col0 - l * VEC < dim; col0 += lpr * VEC) {
@@ -337,15 +338,15 @@ __global__ __launch_bounds__(THREADS) void bwd_small_kernel(int n, const ID* __r
             for (int k = 1; k < groups; ++k)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) acc[v] += red[(k * lpr + l) * VEC + v];
-            write_row<T, VEC>(d_table, row, dim, col, acc, scale);
+            write_row<T, VEC>(d_table, row, dim, col, acc, any ? scale : 0.0f);
         }
         __syncthreads();
     }
 }
 
-// up to four million comparisons of ids with rows, at most 4096 ids: 4096 positions over 256 rows take 5 us, over 1024 rows 6,
-// grouped first 24
-static inline bool small_call(int64_t n, int64_t rows) { return n <= SMALL_N && n * rows <= ((int64_t)1 << 22); }
+// up to four million comparisons of ids with rows, at most 4096 of each: 4096 positions over 256 rows take 5 us, over 1024 rows 7
+// (grouped first 24 to 27), 64 positions over 4096 rows 10 (18)
+static inline bool small_call(int64_t n, int64_t rows) { return n <= SMALL_N && rows <= SMALL_N && n * rows <= ((int64_t)1 << 22); }
 
 static inline int lanes_per_row(int64_t dim, int vec) {
     int l = 4;

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -808,7 +809,7 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
     ids = _gpu_ids(ids, "ids")
     if ids.dim() != 1:
         raise ValueError(f"ids must be 1-D, got {tuple(ids.shape)}")
-    n, n_groups, dev = ids.numel(), int(n_groups), ids.device
+    n, n_groups, dev = ids.numel(), operator.index(n_groups), ids.device
     _group_sizes(n, n_groups)
     new = torch.zeros if n == 0 else torch.empty
     order = torch.empty((n,), dtype=torch.int32, device=dev)
@@ -828,7 +829,7 @@ def row_groups(offsets: torch.Tensor, n_rows: int) -> RowGroups:
     offsets = _gpu_ids(offsets, "offsets")
     if offsets.dim() != 1 or offsets.numel() < 2:
         raise ValueError(f"offsets must be 1-D with one entry more than there are groups, got {tuple(offsets.shape)}")
-    n_rows, n_groups, dev = int(n_rows), offsets.numel() - 1, offsets.device
+    n_rows, n_groups, dev = operator.index(n_rows), offsets.numel() - 1, offsets.device
     if n_rows < 0:
         raise ValueError(f"n_rows must not be negative, got {n_rows}")
     _group_sizes(n_rows, n_groups)

@@ -155,6 +155,10 @@ def test_embed_rows_shapes_strides_and_differences():
 
 def test_embed_rows_keeps_non_finite_values_in_their_rows():
     from nerf_amd import ops
+    for n, rows in ((3, 5), (5000, 40), (3, 5000)):                        # rows that nothing reads have no part in an infinite scale
+        leaf = torch.ones(rows, 8, device=DEV, requires_grad=True)
+        grad = torch.autograd.grad(ops.embed_rows(torch.full((n,), 2, device=DEV), leaf, float("inf")).sum(), leaf)[0]
+        assert torch.isinf(grad[2]).all() and grad[:2].eq(0).all() and grad[3:].eq(0).all()
     table = torch.ones(5, 8, device=DEV)
     table[1], table[3] = float("nan"), float("inf")
     out = ops.embed_rows(torch.tensor([0, 1, 2, 3, 7, -1], device=DEV), table, 2.0)
@@ -570,6 +574,78 @@ def test_calls_on_two_streams():
             assert all(torch.equal(a, b) for a, b in zip(g, w))
 
 
+# ---- offsets that pass 32 bits --------------------------------------------------------------------------------------------
+
+def big(shape, dtype):
+    """zeros of more than 2^31 elements; the tests put values into the last rows only"""
+    assert math.prod(shape) > 2 ** 31
+    return torch.zeros(shape, dtype=dtype, device=DEV)
+
+
+def test_embed_rows_beyond_32_bits():
+    from nerf_amd import ops
+    n, dim = 2 ** 21 + 5, 1031
+    ids = torch.zeros(n, dtype=torch.int64, device=DEV)
+    ids[-3:] = torch.tensor([2, 1, 2], device=DEV)
+    table = torch.randn(3, dim, device=DEV, generator=torch.Generator(DEV).manual_seed(0)).half().requires_grad_(True)
+    out = ops.embed_rows(ids, table)
+    assert torch.equal(out[-4:].detach(), table.detach()[ids[-4:]])
+    d_out = big((n, dim), torch.float16)
+    d_out[-3:] = torch.randint(-8, 9, (3, dim), device=DEV).half()
+    grad = torch.autograd.grad(out, table, d_out)[0]
+    assert grad[0].eq(0).all() and torch.equal(grad[1], d_out[-2]) and torch.equal(grad[2], d_out[-3] + d_out[-1])
+
+
+@pytest.mark.parametrize("K,N", [(1024, 16), (1031, 15)])
+def test_grouped_linear_beyond_32_bits(K, N):
+    """small whole numbers: every sum is exact, in any order"""
+    from nerf_amd import ops
+    n = 2 ** 21 + 5
+    ids = torch.zeros(n, dtype=torch.int32, device=DEV)
+    ids[-3:] = torch.tensor([1, 2, 1], device=DEV, dtype=torch.int32)
+    groups = ops.group_rows(ids, 2)
+    x = big((n, K), torch.bfloat16)
+    x[-4:] = torch.randint(-1, 2, (4, K), device=DEV).bfloat16()
+    x.requires_grad_(True)
+    w = torch.randint(-1, 2, (2, N, K), device=DEV).bfloat16().requires_grad_(True)
+    w.data[:, :, 40:] = 0                                                   # sums of at most 40 terms, whole in bf16
+    y = ops.grouped_linear(x, w, groups)
+    d_y = torch.zeros_like(y)
+    d_y[-4:] = torch.randint(-1, 2, (4, N), device=DEV).bfloat16()
+    dx, dw = torch.autograd.grad(y, (x, w), d_y)
+    xs, ws, ds = x.detach()[-4:].double(), w.detach().double(), d_y[-4:].double()
+    own = (0, 1, None, 1)
+    for i, g in enumerate(own):
+        assert torch.equal(y[-4 + i].detach().double(), ws[g] @ xs[i] if g is not None else torch.zeros(N, device=DEV).double())
+        assert torch.equal(dx[-4 + i].double(), ws[g].t() @ ds[i] if g is not None else torch.zeros(K, device=DEV).double())
+    for g in (0, 1):
+        assert torch.equal(dw[g].double(), sum(torch.outer(ds[i], xs[i]) for i in range(4) if own[i] == g))
+    assert y.detach()[:-4].eq(0).all() and not dx[:-4].any()
+
+
+@pytest.mark.parametrize("B,T,D", [(2, 2 ** 22 + 3, 256), (2 ** 21 + 1, 4, 260)])
+def test_gated_scan_beyond_32_bits(B, T, D):
+    """zero gates and one of 1/2: h is the value, and the sample behind the gate adds half the one before it"""
+    from nerf_amd import ops
+    value = big((B, T, D), torch.bfloat16)
+    tail = torch.randint(-8, 9, (3, D), device=DEV).bfloat16()
+    value[-1, -3:] = tail
+    gate = torch.zeros(B, T, 1, dtype=torch.bfloat16, device=DEV)
+    gate[-1, -1] = 0.5
+    value.requires_grad_(True), gate.requires_grad_(True)
+    h, last = ops.gated_scan(gate, value)
+    assert torch.equal(h[-1, -3:-1], tail[:2]) and torch.equal(h[-1, -1], tail[2] + tail[1] / 2) and torch.equal(last[-1], h[-1, -1].float())
+    assert h.detach()[-1, :-3].eq(0).all() and h.detach()[:-1].eq(0).all()
+    d_h = big((B, T, D), torch.bfloat16)
+    g = torch.randint(-8, 9, (2, D), device=DEV).bfloat16()
+    d_h[-1, -2:] = g
+    d_gate, d_value = torch.autograd.grad(h, (gate, value), d_h)
+    assert torch.equal(d_value[-1, -1], g[1]) and torch.equal(d_value[-1, -2], g[0] + g[1] / 2)
+    assert d_value[-1, :-2].eq(0).all() and d_value[:-1].eq(0).all()
+    want = (g[1].double() * tail[1].double()).sum()                        # whole numbers: exact until the one rounding
+    assert d_gate[-1, -1, 0].double() == want.bfloat16().double()
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------------
 
 def test_refusals():
@@ -582,7 +658,7 @@ def test_refusals():
     v = torch.zeros(4, 5, 8, device=DEV)
     for err, call in (
             (TypeError, lambda: ops.group_rows(f, 2)), (ValueError, lambda: ops.group_rows(i[None], 2)), (ValueError, lambda: ops.group_rows(i, 0)),
-            (ValueError, lambda: ops.group_rows(i, 2 ** 25)), (TypeError, lambda: ops.row_groups(f[0], 4)), (ValueError, lambda: ops.row_groups(i[:1], 4)),
+            (ValueError, lambda: ops.group_rows(i, 2 ** 25)), (TypeError, lambda: ops.group_rows(i, 2.5)), (TypeError, lambda: ops.row_groups(i, 4.0)), (TypeError, lambda: ops.row_groups(f[0], 4)), (ValueError, lambda: ops.row_groups(i[:1], 4)),
             (ValueError, lambda: ops.row_groups(i, -1)),
             (TypeError, lambda: ops.embed_rows(f, f)), (TypeError, lambda: ops.embed_rows(i, i)), (TypeError, lambda: ops.embed_rows(i, f.double())),
             (ValueError, lambda: ops.embed_rows(i, f[0])), (ValueError, lambda: ops.embed_rows(i, f[:0])), (ValueError, lambda: ops.embed_rows(i, f[:, :0])),
