@@ -408,15 +408,17 @@ int nerf_embed_bwd(int64_t n, const void *ids, int id_bytes, int64_t rows, int64
  *   nerf_grouped_bwd_weights: d_weight[g] = sum d_z[i] x[i]^T, d_bias[g] (nullable) = sum d_z[i] over the rows of g; written,
  *                             zeros for a group without rows; fixed order of summation, no atomics
  * Products are summed in fp32 (fp32 operands: exact products).  n_groups <= 65535, K and N <= 65536.  *_ld: elements
- * between rows.  workspace 256-byte aligned. */
+ * between rows.  workspace 256-byte aligned; nerf_grouped_workspace_bytes is for the forward and (backward = 1) the data
+ * gradient and may be 0 (workspace nullable then): operands whose rows are not whole 16-byte pieces are copied there when the products are large. */
+int64_t nerf_grouped_workspace_bytes(int64_t n, int64_t n_groups, int K, int N, int backward, int precision);
 int nerf_grouped_fwd(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets, const int32_t *tile_base,
                      int K, int N, const void *x, int64_t x_ld, const void *weight, const void *bias, int relu,
-                     int precision, void *y, void *stream);
+                     int precision, void *y, void *workspace, int64_t workspace_bytes, void *stream);
 int nerf_relu_bwd(int64_t n, int N, const void *d_y, int64_t d_y_ld, const void *y, int precision, void *d_z, void *stream);
 int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets, const int32_t *tile_base,
                           int K, int N, const void *d_z, int64_t d_z_ld, const void *weight, int precision, void *d_x,
-                          void *stream);
-int64_t nerf_grouped_bwd_weights_workspace_bytes(int64_t n, int64_t n_groups, int K, int N);
+                          void *workspace, int64_t workspace_bytes, void *stream);
+int64_t nerf_grouped_bwd_weights_workspace_bytes(int64_t n, int64_t n_groups, int K, int N, int precision);
 int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32_t *order, const int32_t *offsets,
                              const int32_t *tile_base, int K, int N, const void *d_z, int64_t d_z_ld, const void *x,
                              int64_t x_ld, int precision, void *d_weight, void *d_bias, void *workspace,

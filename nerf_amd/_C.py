@@ -73,10 +73,11 @@ _SIGS = {
     "nerf_embed_fwd": (c_int, [c_int64, P, c_int, c_int64, c_int64, P, c_int64, c_float, c_int, P, P]),
     "nerf_embed_bwd_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
     "nerf_embed_bwd": (c_int, [c_int64, P, c_int, c_int64, c_int64, P, c_int64, c_float, c_int, P, P, c_int64, P]),
-    "nerf_grouped_fwd": (c_int, [c_int64, c_int64, P, P, P, c_int, c_int, P, c_int64, P, P, c_int, c_int, P, P]),
+    "nerf_grouped_workspace_bytes": (c_int64, [c_int64, c_int64, c_int, c_int, c_int, c_int]),
+    "nerf_grouped_fwd": (c_int, [c_int64, c_int64, P, P, P, c_int, c_int, P, c_int64, P, P, c_int, c_int, P, P, c_int64, P]),
     "nerf_relu_bwd": (c_int, [c_int64, c_int, P, c_int64, P, c_int, P, P]),
-    "nerf_grouped_bwd_data": (c_int, [c_int64, c_int64, P, P, P, c_int, c_int, P, c_int64, P, c_int, P, P]),
-    "nerf_grouped_bwd_weights_workspace_bytes": (c_int64, [c_int64, c_int64, c_int, c_int]),
+    "nerf_grouped_bwd_data": (c_int, [c_int64, c_int64, P, P, P, c_int, c_int, P, c_int64, P, c_int, P, P, c_int64, P]),
+    "nerf_grouped_bwd_weights_workspace_bytes": (c_int64, [c_int64, c_int64, c_int, c_int, c_int]),
     "nerf_grouped_bwd_weights": (c_int, [c_int64, c_int64, P, P, P, c_int, c_int, P, c_int64, P, c_int64, c_int, P, P, P, c_int64, P]),
     "nerf_scan_states_floats": (c_int64, [c_int64, c_int64, c_int64, c_int]),
     "nerf_scan_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),

@@ -192,6 +192,8 @@ struct LinArgs {
     Rows rows;
     int C, O, tiles_o;           // contraction length, outputs, output tiles
     int64_t a_ld;
+    int64_t w_ld, w_gs;          // elements between rows and between groups of w
+    int w_rows;                  // rows of w where they are the contraction index (C is a whole number of pieces)
     const void *a, *w, *bias;
     int relu;
     void* out;
@@ -238,7 +240,7 @@ struct Tables {
     }
 };
 
-// ---- streaming form: operands in whole aligned 16-byte pieces ------------------------------------------------------
+// ---- streaming form: operands in whole aligned 16-byte pieces, outputs at any alignment ------------------------------------------------------
 // out[row][o] = sum_c a[row][c] w_g(o, c).  WT = false: w_g is [O][C] (the layer); WT = true: w_g is [C][O] (its data
 // gradient).  One workgroup of eight waves per compute unit for the whole call.  It owns a run of consecutive items (128
 // rows x BN outputs) and streams their contraction steps without a gap between items: the memory system copies step s + 2
@@ -246,14 +248,22 @@ struct Tables {
 //
 // vmcnt counts copies and stores in the order they were issued, so a step waits for its own copies only, with the number
 // of younger copies and stores left outstanding.  For that count to be known, every wave issues the same stores for every
-// item: a position behind a tile's rows repeats the tile's last row, outputs behind the last piece repeat that piece, and
-// what they store is what is there already.  LDS is read by inline asm (reads and their wait in one block), because the
+// item: a position behind a tile's rows repeats the tile's last row, outputs behind the last piece repeat that piece
+// (out_of), and what they store is what is there already.  LDS is read by inline asm (reads and their wait in one block), because the
 // compiler would wait for every copy in flight in front of a read it can see.
 //
 // The accumulators hold outputs down and rows across: a lane's four consecutive registers are consecutive outputs of one
 // row, and one exchange between the wave's halves (v_permlane32_swap) makes them eight, a 16-byte store.
 constexpr int ST_THREADS = 512;
 constexpr int ST_ITEMS = 12;            // items whose rows and bias are in LDS at a time
+
+// Output number of place o.  The last piece of a row ends where the row does, so it may repeat outputs of the one before, and
+// places behind it repeat it: the same values are stored again.
+template <int E>
+__device__ __forceinline__ int out_of(int o, int O) {
+    const int first = o / E * E;
+    return first + E <= O ? o : O - E + (o - first);
+}
 
 template <int N>
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -506,7 +516,7 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
 #pragma unroll 3
             for (int j = tid; j < items * BN; j += ST_THREADS) {
                 const int i = j / BN, o = d_o0[i] + j % BN, g = min(d_grp[i], G - 1);
-                bias_tab[0][j] = ((const T*)p.bias)[(int64_t)g * O + (o < O ? o : O - E + o % E)];
+                bias_tab[0][j] = ((const T*)p.bias)[(int64_t)g * O + out_of<E>(o, O)];
             }
         } else {
             for (int j = tid; j < items * BN; j += ST_THREADS) bias_tab[0][j] = (T)0.0f;
@@ -515,12 +525,12 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
         int real = items;                                                   // the rows of no group come last
         while (real > 0 && d_grp[real - 1] == G) --real;
         for (int i = real; i < items; ++i) {
-            const int o0 = d_o0[i], pieces = (O - o0 < BN ? O - o0 : BN) / E;
+            const int o0 = d_o0[i], pieces = ((O - o0 < BN ? O - o0 : BN) + E - 1) / E;
             Pack<T, E> zero;
 #pragma unroll
             for (int e = 0; e < E; ++e) zero.v[e] = (T)0.0f;
             for (int j = tid; j < d_cnt[i] * pieces; j += ST_THREADS)
-                store_pack<T, E>(out + (int64_t)row_tab[i][j / pieces] * O + o0 + (j % pieces) * E, zero);
+                store_any<T, E>(out + (int64_t)row_tab[i][j / pieces] * O + out_of<E>(o0 + (j % pieces) * E, O), zero);
         }
         const int steps = real * nk;
         if (steps == 0) continue;
@@ -537,22 +547,21 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
                     const int64_t row = lds_int(rows0 + (c_item * TILE_ROWS + a_row[i]) * 4);
                     pa[i] = (const T*)p.a + row * p.a_ld + a_q[i] * E;
                 }
-                const T* w = (const T*)p.w + (int64_t)g * O * C;
+                const T* w = (const T*)p.w + g * p.w_gs;
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
                     if constexpr (WT) {
                         const int o = o0 + b_q[i] * E;
-                        pb[i] = w + (int64_t)b_row[i] * O + (o < O ? o : O - E);
+                        pb[i] = w + b_row[i] * p.w_ld + (o < p.w_ld ? o : p.w_ld - E);
                     } else {
-                        const int o = o0 + b_row[i];
-                        pb[i] = w + (int64_t)(o < O ? o : O - E + o % E) * C + b_q[i] * E;
+                        pb[i] = w + out_of<E>(o0 + b_row[i], O) * p.w_ld + b_q[i] * E;
                     }
                 }
             }
             char* const to = lds + c_buf * STAGE + wave * (NA * 1024);
             char* const to_b = lds + c_buf * STAGE + A_BYTES + wave * (NB * 1024);
             const int k0 = c_k * BK;
-            if (k0 + BK <= C) {
+            if (k0 + BK <= (WT ? p.w_rows : C)) {
 #pragma unroll
                 for (int i = 0; i < NA; ++i) copy_piece(pa[i], to + i * 1024);
 #pragma unroll
@@ -562,13 +571,13 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
                 for (int i = 0; i < NA; ++i) copy_piece(k0 + a_q[i] * E < C ? (const void*)pa[i] : (const void*)&ZERO_PIECE, to + i * 1024);
 #pragma unroll
                 for (int i = 0; i < NB; ++i)
-                    copy_piece(k0 + (WT ? b_row[i] : b_q[i] * E) < C ? (const void*)pb[i] : (const void*)&ZERO_PIECE, to_b + i * 1024);
+                    copy_piece((WT ? k0 + b_row[i] < p.w_rows : k0 + b_q[i] * E < C) ? (const void*)pb[i] : (const void*)&ZERO_PIECE, to_b + i * 1024);
             }
             if (c_item * nk + c_k + 1 < steps) {
 #pragma unroll
                 for (int i = 0; i < NA; ++i) pa[i] += BK;
 #pragma unroll
-                for (int i = 0; i < NB; ++i) pb[i] += WT ? (int64_t)BK * O : BK;
+                for (int i = 0; i < NB; ++i) pb[i] += WT ? BK * p.w_ld : BK;
             }
             // behind the last step the last one is copied again, into a buffer that nothing reads any more
             if (c_item * nk + c_k + 1 < steps && ++c_k == nk) { c_k = 0; ++c_item; }
@@ -625,16 +634,14 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
                                 x[e] = sw[0];
                                 y[e] = sw[1];
                             }
-                            int o = o0 + 32 * j + 8 * h + 8 * (lane >> 5);
-                            o = o < O ? o : O - E;
-                            *reinterpret_cast<uint4*>(out + row * O + o) = make_uint4(x[0], x[1], y[0], y[1]);
+                            const uint4 q = make_uint4(x[0], x[1], y[0], y[1]);
+                            store_any<T, E>(out + row * O + out_of<E>(o0 + 32 * j + 8 * h + 8 * (lane >> 5), O), __builtin_bit_cast(Pack<T, E>, q));
                         }
                     } else {
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
-                            int o = o0 + 32 * j + 8 * h + 4 * (lane >> 5);
-                            o = o < O ? o : O - E;
-                            *reinterpret_cast<float4*>(out + row * O + o) = make_float4(z[4 * h], z[4 * h + 1], z[4 * h + 2], z[4 * h + 3]);
+                            const float4 q = make_float4(z[4 * h], z[4 * h + 1], z[4 * h + 2], z[4 * h + 3]);
+                            store_any<T, E>(out + row * O + out_of<E>(o0 + 32 * j + 8 * h + 4 * (lane >> 5), O), __builtin_bit_cast(Pack<T, E>, q));
                         }
                     }
                 }
@@ -698,8 +705,8 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
 }
 
 // ---- through registers: any row length, any alignment ------------------------------------------------------------
-// The same product, one workgroup of four waves per tile of 128 rows x BN outputs.  Pieces are put together element by
-// element; a step is requested before the products of the one before it.
+// The same product, one workgroup of four waves per tile of 128 rows x BN outputs; a step is requested before the products of
+// the one before it (65 536 rows, 67 -> 256 bf16: forward 29 us, data gradient 40; in whole pieces, 64 -> 256, 18 and 20).
 template <typename T, bool WT, int BN>
 __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();
@@ -854,6 +861,7 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
 struct WgradArgs {
     Rows rows;
     int K, N, tiles_k, tiles_n;
+    int Kp, Np;                      // columns of x and dy that can be read (streaming form: whole pieces)
     int chunk;                       // tiles of one workgroup
     int64_t x_ld, dy_ld;
     const void *x, *dy;
@@ -941,14 +949,14 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
         const int slot = (wave * ND + i) * 64 + lane;
         d_row[i] = slot / DPR;
         const int col = n0 + ((slot % DPR) ^ tr_swap<T, BD>(d_row[i])) * E;
-        d_col[i] = col < N ? col : N - E;                                   // columns behind the last are not stored
+        d_col[i] = col < p.Np ? col : p.Np - E;                             // columns behind the last are not stored
     }
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
         const int slot = (wave * NX + i) * 64 + lane;
         x_row[i] = slot / XPR;
         const int col = k0 + ((slot % XPR) ^ tr_swap<T, BX>(x_row[i])) * E;
-        x_col[i] = col < K ? col : K - E;
+        x_col[i] = col < p.Kp ? col : p.Kp - E;
     }
     unsigned fd[S][MI], fx[S][NJ];
 #pragma unroll
@@ -1130,11 +1138,7 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
     }
 }
 
-// dW[n][k] = sum over rows dZ[row][n] x[row][k].  A workgroup owns one BT x BT block of every dW it meets and walks
-// `chunk` consecutive tiles of the flat tile list, whatever groups they belong to, so all workgroups have equal work
-// however uneven the groups are.  A group that lies inside one chunk is finished here; the pieces of a longer one go to
-// the workspace and are added up in order by wgrad_join_kernel (no atomics: the result does not depend on timing).
-// The same through registers: any row length, any alignment.
+// The same through registers, four waves per BT x BT block: any row length, any alignment (65 536 rows, 67 -> 256 bf16, 43 us).
 template <typename T, int BT>
 __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();                       // rows of one step
@@ -1312,6 +1316,21 @@ __global__ __launch_bounds__(THREADS) void wgrad_join_kernel(WgradArgs p) {
     else ((T*)p.db)[(int64_t)g * p.N + (i - NK)] = (T)sum;
 }
 
+// Rows that are not whole pieces, copied to rows that are, for the streaming forms: with zeros behind the last column, or
+// (SHIFT) the last piece ending where the row does, as out_of() has it.
+template <typename T, bool SHIFT>
+__global__ __launch_bounds__(THREADS) void pad_kernel(int64_t rows, int cols, const T* src, int64_t ld, T* dst) {
+    constexpr int E = piece<T>();
+    const int pieces = (cols + E - 1) / E;
+    const int64_t total = rows * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * THREADS) {
+        const int64_t row = total <= 0x7fffffff ? (int)i / pieces : i / pieces;
+        const int c = (int)(i - row * pieces) * E;
+        const T* from = src + row * ld;
+        store_pack<T, E>(dst + i * E, SHIFT ? load_any<T, E>(from + min(c, cols - E)) : load_piece<T>(from, c, cols, true));
+    }
+}
+
 // dZ = dY where the ReLU let something through.  Memory bound: 196 608 x 256 bf16 in 51 us, 5.9 TB/s.  Written out once, because
 // the gate inside the two products costs more: their tiles are bound by what they copy into LDS, and the gate is a third
 // operand (in the same shape, data gradient 125 us gated and 59 not, weight gradient 116 and 66).
@@ -1333,6 +1352,48 @@ static inline bool sizes_ok(int64_t n, int64_t n_groups, int K, int N) {
     return n >= 0 && n <= grp::MAX_ROWS && n_groups >= 1 && n_groups <= 65535 && K >= 1 && K <= 65536 && N >= 1 && N <= 65536;
 }
 static inline int64_t max_tiles(int64_t n, int64_t n_groups) { return n / TILE_ROWS + n_groups + 1; }
+
+// Operands whose rows are not whole pieces are copied to rows that are, and streamed, where that pays; a copy and its launch
+// cost 5 us and up.  Measured, register form against copy and streaming form:
+//   fp32, always from 2^28 products: 65 536 rows 63 -> 256 forward 80 / 47 us, data gradient 53 / 40, weight gradient 97 / 71
+//   16 bits, forward: not (65 536 rows 67 -> 256 24 / 32, 196 608 rows 255 -> 257 126 / 150)
+//   data gradient, weights alone: from 2^26 (4096 rows 67 -> 256 15 / 9.5, 65 536 rows 39 / 24); with dZ: from 2^31 (16 384 rows
+//     250 -> 131 14 / 20, 65 536 rows 43 / 35, 196 608 rows 255 -> 257 155 / 120)
+//   weight gradient, one operand: from 2^26 (65 536 rows 67 -> 256 44 / 30); both: from 2^31 (16 384 rows 250 -> 131 30 / 36,
+//     65 536 rows 55 / 53, 196 608 rows 255 -> 257 302 / 183); not up to 64 x 64 (65 536 rows 63 -> 64 20 / 26)
+struct PadPlan {
+    bool fwd, data, weights;
+    int Kp, Np;                                                             // whole pieces
+};
+static PadPlan pad_plan(int64_t n, int64_t n_groups, int K, int N, int precision) {
+    const int E = 16 / elem_bytes(precision);
+    PadPlan p = {};
+    p.Kp = (K + E - 1) / E * E;
+    p.Np = (N + E - 1) / E * E;
+    const bool odd_k = K % E != 0, odd_n = N % E != 0, fp32 = precision == NERF_PREC_FP32;
+    if (K < E || N < E || (K <= 64 && N <= 64) || n_groups * K * N > 4 * n * (K + N)) return p;
+    const double products = (double)n * K * N;                              // n K N may pass 64 bits
+    const double one = fp32 ? 0x1p28 : 0x1p26, two = fp32 ? 0x1p28 : 0x1p31;
+    p.fwd = odd_k && fp32 && products >= one;
+    p.data = (odd_k || odd_n) && products >= (odd_n ? two : one);
+    p.weights = (odd_k || odd_n) && products >= (odd_k && odd_n ? two : one);
+    return p;
+}
+static inline int64_t elems256(int64_t elems, int precision) { return (elems * elem_bytes(precision) + 255) / 256 * 256; }
+
+static int pad_rows(int64_t rows, int cols, const void* src, int64_t ld, void* dst, bool shift, int precision, void* stream) {
+    const int E = 16 / elem_bytes(precision);
+    const int64_t blocks = (rows * ((cols + E - 1) / E) + THREADS - 1) / THREADS, most = (int64_t)1 << 22;
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+#define NERF_CALL(T)                                                                                                                       \
+    do {                                                                                                                                   \
+        if (shift) hipLaunchKernelGGL((pad_kernel<T, true>), grid, dim3(THREADS), 0, (hipStream_t)stream, rows, cols, (const T*)src, ld, (T*)dst); \
+        else hipLaunchKernelGGL((pad_kernel<T, false>), grid, dim3(THREADS), 0, (hipStream_t)stream, rows, cols, (const T*)src, ld, (T*)dst);      \
+    } while (0)
+    NERF_ELEM_DISPATCH(precision, NERF_CALL);
+#undef NERF_CALL
+    return nerf_launch_status();
+}
 
 // workgroups of a grid whose kernel spreads `work` over the eight XCDs in runs of `unit`
 static inline int64_t xcd_grid(int64_t work, int64_t unit) { return ((work + unit - 1) / unit + 7) / 8 * unit * 8; }
@@ -1412,22 +1473,41 @@ static int launch_linear(const LinArgs& args, int precision, bool wide, void* st
 }  // namespace gl
 }  // namespace nerf
 
+extern "C" int64_t nerf_grouped_workspace_bytes(int64_t n, int64_t n_groups, int K, int N, int backward, int precision) {
+    using namespace nerf;
+    if (!gl::sizes_ok(n, n_groups, K, N)) return NERF_E_SHAPE;
+    if (!elem_ok(precision)) return NERF_E_DTYPE;
+    const gl::PadPlan p = gl::pad_plan(n, n_groups, K, N, precision);
+    if (!(backward ? p.data : p.fwd)) return 0;
+    return gl::elems256(n * (backward ? p.Np : p.Kp), precision) + gl::elems256(n_groups * N * p.Kp, precision);
+}
+
 extern "C" int nerf_grouped_fwd(int64_t n, int64_t n_groups, const int32_t* order, const int32_t* offsets, const int32_t* tile_base,
                                 int K, int N, const void* x, int64_t x_ld, const void* weight, const void* bias, int relu,
-                                int precision, void* y, void* stream) {
+                                int precision, void* y, void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace nerf;
     NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && x_ld >= K, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(order && offsets && tile_base && x && weight && y, NERF_E_NULL);
+    const gl::PadPlan pad = gl::pad_plan(n, n_groups, K, N, precision);
+    NERF_REQUIRE(order && offsets && tile_base && x && weight && y && (workspace || !pad.fwd), NERF_E_NULL);
     const int es = elem_bytes(precision), E = 16 / es;
     NERF_REQUIRE(nerf_aligned(x, (uintptr_t)es) && nerf_aligned(weight, (uintptr_t)es) && nerf_aligned(y, (uintptr_t)es) &&
-                 nerf_aligned(bias, (uintptr_t)es), NERF_E_ALIGN);
-    const bool wide = K % E == 0 && N % E == 0 && x_ld % E == 0 && nerf_aligned(x, 16) && nerf_aligned(weight, 16) && nerf_aligned(y, 16);
+                 nerf_aligned(bias, (uintptr_t)es) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
+    NERF_REQUIRE(workspace_bytes >= nerf_grouped_workspace_bytes(n, n_groups, K, N, 0, precision), NERF_E_WORKSPACE);
     gl::LinArgs p = {};
     p.rows = {n, (int)n_groups, order, offsets, tile_base};
-    p.C = K; p.O = N; p.a = x; p.a_ld = x_ld; p.w = weight; p.bias = bias; p.relu = relu ? 1 : 0; p.out = y;
-    return gl::launch_linear<false>(p, precision, wide, stream);
+    p.C = K; p.O = N; p.a = x; p.a_ld = x_ld; p.w = weight; p.w_ld = K; p.w_gs = (int64_t)N * K; p.bias = bias; p.relu = relu ? 1 : 0; p.out = y;
+    const bool whole = K % E == 0 && x_ld % E == 0 && nerf_aligned(x, 16) && nerf_aligned(weight, 16) && N >= E;
+    if (pad.fwd) {
+        void *a = workspace, *w = (char*)workspace + gl::elems256(n * pad.Kp, precision);
+        int rc = gl::pad_rows(n, K, x, x_ld, a, false, precision, stream);
+        if (rc == NERF_OK) rc = gl::pad_rows(n_groups * N, K, weight, K, w, false, precision, stream);
+        if (rc != NERF_OK) return rc;
+        p.C = pad.Kp; p.a = a; p.a_ld = pad.Kp; p.w = w; p.w_ld = pad.Kp; p.w_gs = (int64_t)N * pad.Kp;
+        return gl::launch_linear<false>(p, precision, true, stream);
+    }
+    return gl::launch_linear<false>(p, precision, whole, stream);
 }
 
 extern "C" int nerf_relu_bwd(int64_t n, int N, const void* d_y, int64_t d_y_ld, const void* y, int precision, void* d_z, void* stream) {
@@ -1449,30 +1529,54 @@ extern "C" int nerf_relu_bwd(int64_t n, int N, const void* d_y, int64_t d_y_ld, 
 
 extern "C" int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t* order, const int32_t* offsets, const int32_t* tile_base,
                                      int K, int N, const void* d_z, int64_t d_z_ld, const void* weight, int precision, void* d_x,
-                                     void* stream) {
+                                     void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace nerf;
     NERF_REQUIRE(gl::sizes_ok(n, n_groups, K, N) && d_z_ld >= N, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(order && offsets && tile_base && d_z && weight && d_x, NERF_E_NULL);
+    const gl::PadPlan pad = gl::pad_plan(n, n_groups, K, N, precision);
+    NERF_REQUIRE(order && offsets && tile_base && d_z && weight && d_x && (workspace || !pad.data), NERF_E_NULL);
     const int es = elem_bytes(precision), E = 16 / es;
-    NERF_REQUIRE(nerf_aligned(d_z, (uintptr_t)es) && nerf_aligned(weight, (uintptr_t)es) && nerf_aligned(d_x, (uintptr_t)es), NERF_E_ALIGN);
-    const bool wide = K % E == 0 && N % E == 0 && d_z_ld % E == 0 && nerf_aligned(d_z, 16) && nerf_aligned(weight, 16) && nerf_aligned(d_x, 16);
+    NERF_REQUIRE(nerf_aligned(d_z, (uintptr_t)es) && nerf_aligned(weight, (uintptr_t)es) && nerf_aligned(d_x, (uintptr_t)es) &&
+                 nerf_aligned(workspace, 256), NERF_E_ALIGN);
+    NERF_REQUIRE(workspace_bytes >= nerf_grouped_workspace_bytes(n, n_groups, K, N, 1, precision), NERF_E_WORKSPACE);
     gl::LinArgs p = {};
     p.rows = {n, (int)n_groups, order, offsets, tile_base};
-    p.C = N; p.O = K; p.a = d_z; p.a_ld = d_z_ld; p.w = weight; p.out = d_x;
-    return gl::launch_linear<true>(p, precision, wide, stream);
+    p.C = N; p.O = K; p.a = d_z; p.a_ld = d_z_ld; p.w = weight; p.w_ld = K; p.w_gs = (int64_t)N * K; p.w_rows = N; p.out = d_x;
+    bool a_whole = N % E == 0 && d_z_ld % E == 0 && nerf_aligned(d_z, 16), w_whole = K % E == 0 && nerf_aligned(weight, 16);
+    if (pad.data && (a_whole || N % E) && (w_whole || K % E)) {
+        if (!a_whole) {
+            const int rc = gl::pad_rows(n, N, d_z, d_z_ld, workspace, false, precision, stream);
+            if (rc != NERF_OK) return rc;
+            p.C = pad.Np; p.a = workspace; p.a_ld = pad.Np;
+        }
+        if (!w_whole) {
+            void* w = (char*)workspace + gl::elems256(n * pad.Np, precision);
+            const int rc = gl::pad_rows(n_groups * N, K, weight, K, w, true, precision, stream);
+            if (rc != NERF_OK) return rc;
+            p.w = w; p.w_ld = pad.Kp; p.w_gs = (int64_t)N * pad.Kp;
+        }
+        a_whole = w_whole = true;
+    }
+    return gl::launch_linear<true>(p, precision, a_whole && w_whole, stream);
 }
 
-extern "C" int64_t nerf_grouped_bwd_weights_workspace_bytes(int64_t n, int64_t n_groups, int K, int N) {
-    if (!nerf::gl::sizes_ok(n, n_groups, K, N)) return NERF_E_SHAPE;
-    // what alignment and type lead to differs in the number of chunks: enough for any of them
-    int64_t most = 0;
-    for (int way = 0; way < 3; ++way) {
-        const int64_t b = nerf::gl::wgrad_plan(n, n_groups, K, N, way > 0, way > 1 ? NERF_PREC_FP32 : NERF_PREC_BF16).bytes;
-        if (b > most) most = b;
-    }
-    return most;
+namespace nerf {
+namespace gl {
+// for the pieces of dW: alignment decides the form, and with it the number of chunks; enough for either
+static int64_t wgrad_bytes(int64_t n, int64_t n_groups, int K, int N, int precision) {
+    const int64_t a = wgrad_plan(n, n_groups, K, N, false, precision).bytes, b = wgrad_plan(n, n_groups, K, N, true, precision).bytes;
+    return ((a > b ? a : b) + 255) / 256 * 256;
+}
+}  // namespace gl
+}  // namespace nerf
+
+extern "C" int64_t nerf_grouped_bwd_weights_workspace_bytes(int64_t n, int64_t n_groups, int K, int N, int precision) {
+    using namespace nerf;
+    if (!gl::sizes_ok(n, n_groups, K, N)) return NERF_E_SHAPE;
+    if (!elem_ok(precision)) return NERF_E_DTYPE;
+    const gl::PadPlan pad = gl::pad_plan(n, n_groups, K, N, precision);
+    return gl::wgrad_bytes(n, n_groups, K, N, precision) + (pad.weights ? gl::elems256(n * pad.Kp, precision) + gl::elems256(n * pad.Np, precision) : 0);
 }
 
 extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32_t* order, const int32_t* offsets,
@@ -1487,15 +1591,32 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
     const int es = elem_bytes(precision), E = 16 / es;
     NERF_REQUIRE(nerf_aligned(d_z, (uintptr_t)es) && nerf_aligned(x, (uintptr_t)es) && nerf_aligned(d_weight, (uintptr_t)es) &&
                  nerf_aligned(d_bias, (uintptr_t)es) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
-    NERF_REQUIRE(workspace_bytes >= nerf_grouped_bwd_weights_workspace_bytes(n, n_groups, K, N), NERF_E_WORKSPACE);
+    NERF_REQUIRE(workspace_bytes >= nerf_grouped_bwd_weights_workspace_bytes(n, n_groups, K, N, precision), NERF_E_WORKSPACE);
     // Up to 64 x 64 the register form has blocks of that size, a quarter of the streaming form's products: 64 -> 64 fp32 53 us
     // against 89 (196 608 rows) and 12.5 against 19.5 (1024); bf16 12.5 against 16 at 16 384 rows, but 31 against 26.5 at 196 608.
     const bool small = K <= 64 && N <= 64 && (precision == NERF_PREC_FP32 || n < 65536);
-    const bool wide = !small && K % E == 0 && N % E == 0 && d_z_ld % E == 0 && x_ld % E == 0 && nerf_aligned(d_z, 16) && nerf_aligned(x, 16);
+    const gl::PadPlan pad = gl::pad_plan(n, n_groups, K, N, precision);
+    bool d_whole = N % E == 0 && d_z_ld % E == 0 && nerf_aligned(d_z, 16), x_whole = K % E == 0 && x_ld % E == 0 && nerf_aligned(x, 16);
+    if (pad.weights && (d_whole || N % E) && (x_whole || K % E)) {
+        char* at = (char*)workspace + gl::wgrad_bytes(n, n_groups, K, N, precision);
+        if (!x_whole) {
+            const int rc = gl::pad_rows(n, K, x, x_ld, at, false, precision, stream);
+            if (rc != NERF_OK) return rc;
+            x = at; x_ld = pad.Kp;
+        }
+        if (!d_whole) {
+            at += gl::elems256(n * pad.Kp, precision);
+            const int rc = gl::pad_rows(n, N, d_z, d_z_ld, at, false, precision, stream);
+            if (rc != NERF_OK) return rc;
+            d_z = at; d_z_ld = pad.Np;
+        }
+        d_whole = x_whole = true;
+    }
+    const bool wide = !small && d_whole && x_whole;
     const gl::WgradPlan w = gl::wgrad_plan(n, n_groups, K, N, wide, precision);
     gl::WgradArgs p = {};
     p.rows = {n, (int)n_groups, order, offsets, tile_base};
-    p.K = K; p.N = N; p.tiles_k = w.tiles_k; p.tiles_n = w.tiles_n; p.chunk = w.chunk;
+    p.K = K; p.N = N; p.Kp = pad.Kp; p.Np = pad.Np; p.tiles_k = w.tiles_k; p.tiles_n = w.tiles_n; p.chunk = w.chunk;
     p.x_ld = x_ld; p.dy_ld = d_z_ld; p.x = x; p.dy = d_z; p.dw = d_weight; p.db = d_bias;
     p.part_w = (float*)((char*)workspace + w.part_w);
     p.part_b = (float*)((char*)workspace + w.part_b);

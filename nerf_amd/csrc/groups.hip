@@ -1,6 +1,6 @@
 // Grouping of rows by an integer id: the stable order that puts the rows of one group next to each other, where each
 // group begins, and how many 128-row tiles the groups before it hold.  The reference has no sub-networks; this is what
-// hands sample points to them (nerf_grouped_linear) and what the gradient of a row look-up sums by (nerf_embed_bwd).
+// hands sample points to them (nerf_grouped_fwd) and what the gradient of a row look-up sums by (nerf_embed_bwd).
 //
 // An LSD radix sort of (id, position); ids outside [0, n_groups) take the key n_groups and come last.  For a digit every
 // wave owns a run of consecutive positions.  The lanes of one 64-element round that hold the same digit find each other

@@ -896,6 +896,13 @@ def embed_rows(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> to
     return _embed_fwd(ids, table, float(scale))
 
 
+def _grouped_work(n, G, K, N, backward, prec, dev):
+    """The workspace of the forward or the data gradient, as (tensor to keep, pointer, bytes); most sizes need none."""
+    nbytes = _size("nerf_grouped_workspace_bytes", n, G, K, N, backward, prec)
+    work = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+    return work, _ptr(work), nbytes
+
+
 def _grouped_fwd(x, weight, bias, groups, relu):
     """(y, x as it was read, weight as it was read)"""
     n, dev = groups.n_rows, x.device
@@ -904,8 +911,9 @@ def _grouped_fwd(x, weight, bias, groups, relu):
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     y = torch.empty((n, N), dtype=x.dtype, device=dev)
+    work, at, nbytes = _grouped_work(n, G, K, N, 0, _ELEM[x.dtype], dev)
     _call("nerf_grouped_fwd", "grouped_fwd", dev, n, n, G, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N,
-          x.data_ptr(), ld, weight.data_ptr(), _ptr(bias), int(relu), _ELEM[x.dtype], y.data_ptr())
+          x.data_ptr(), ld, weight.data_ptr(), _ptr(bias), int(relu), _ELEM[x.dtype], y.data_ptr(), at, nbytes)
     return y, x, weight
 
 
@@ -938,12 +946,13 @@ class _GroupedLinear(torch.autograd.Function):
         at = (n, G, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N, g.data_ptr(), ld)
         if need_x:
             dx = torch.empty((n, K), dtype=g.dtype, device=dev)
-            _call("nerf_grouped_bwd_data", "grouped_bwd_data", dev, n, *at, weight.data_ptr(), prec, dx.data_ptr())
+            work, place, nbytes = _grouped_work(n, G, K, N, 1, prec, dev)
+            _call("nerf_grouped_bwd_data", "grouped_bwd_data", dev, n, *at, weight.data_ptr(), prec, dx.data_ptr(), place, nbytes)
         if need_w or need_b:
             dw = torch.empty((G, N, K), dtype=g.dtype, device=dev)
             db = torch.empty((G, N), dtype=g.dtype, device=dev) if need_b else None
             x, x_ld = _row_major(x)
-            nbytes = _size("nerf_grouped_bwd_weights_workspace_bytes", n, G, K, N)
+            nbytes = _size("nerf_grouped_bwd_weights_workspace_bytes", n, G, K, N, prec)
             work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
             _call("nerf_grouped_bwd_weights", "grouped_bwd_weights", dev, n, *at, x.data_ptr(), x_ld, prec, dw.data_ptr(), _ptr(db),
                   work.data_ptr(), nbytes)

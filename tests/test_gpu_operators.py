@@ -223,7 +223,7 @@ def test_grouped_linear(n, G, K, N, kind, relu, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("K,N,relu", [(256, 256, True), (248, 232, False), (40, 1000, False), (1000, 24, True)])
+@pytest.mark.parametrize("K,N,relu", [(256, 256, True), (248, 232, False), (40, 1000, False), (1000, 24, True), (67, 256, True), (256, 67, False), (131, 250, True), (9, 1001, False), (1001, 11, True)])
 def test_grouped_linear_many_rows(K, N, relu, dtype):
     """enough tiles for the widest output tiles, several tiles per workgroup, some with a ragged last step or last tile"""
     from nerf_amd import ops

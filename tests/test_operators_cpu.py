@@ -69,21 +69,32 @@ def test_cabi_refuses_bad_table_arguments(lib):
 
 def test_cabi_refuses_bad_grouped_layer_arguments(lib):
     f, d, w = lib.nerf_grouped_fwd, lib.nerf_grouped_bwd_data, lib.nerf_grouped_bwd_weights
-    need = lib.nerf_grouped_bwd_weights_workspace_bytes(5000, 3, 40, 24)
+    need = lib.nerf_grouped_bwd_weights_workspace_bytes(5000, 3, 40, 24, 0)
+    none = (None, 0, None)                                                     # no workspace, stream
     for G, K, N in ((0, 40, 24), (65536, 40, 24), (3, 0, 24), (3, 40, 0), (3, 65537, 24), (3, 40, 65537)):
-        assert f(5000, G, P, P, P, K, N, P, 70000, P, P, 0, 0, P, None) == SHAPE
-        assert d(5000, G, P, P, P, K, N, P, 70000, P, 0, P, None) == SHAPE
-        assert lib.nerf_grouped_bwd_weights_workspace_bytes(5000, G, K, N) == SHAPE
+        assert f(5000, G, P, P, P, K, N, P, 70000, P, P, 0, 0, P, *none) == SHAPE
+        assert d(5000, G, P, P, P, K, N, P, 70000, P, 0, P, *none) == SHAPE
+        assert lib.nerf_grouped_bwd_weights_workspace_bytes(5000, G, K, N, 0) == SHAPE == lib.nerf_grouped_workspace_bytes(5000, G, K, N, 0, 0)
         assert w(5000, G, P, P, P, K, N, P, 70000, P, 70000, 0, P, P, P, need, None) == SHAPE
-    assert f(5000, 3, P, P, P, 40, 24, P, 39, P, P, 0, 0, P, None) == SHAPE and d(5000, 3, P, P, P, 40, 24, P, 23, P, 0, P, None) == SHAPE
-    assert f(5000, 3, P, P, P, 40, 24, P, 40, P, P, 0, 3, P, None) == DTYPE and d(5000, 3, P, P, P, 40, 24, P, 24, P, -1, P, None) == DTYPE
-    assert f(5000, 3, None, P, P, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL
-    assert f(5000, 3, P, None, P, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL and f(5000, 3, P, P, None, 40, 24, P, 40, P, P, 0, 0, P, None) == NULL
-    assert f(5000, 3, P, P, P, 40, 24, P + 1, 40, P, P, 0, 0, P, None) == ALIGN and d(5000, 3, P, P, P, 40, 24, P, 24, P + 2, 2, P, None) == ALIGN
+    assert lib.nerf_grouped_bwd_weights_workspace_bytes(5000, 3, 40, 24, 3) == DTYPE == lib.nerf_grouped_workspace_bytes(5000, 3, 40, 24, 1, -1)
+    assert f(5000, 3, P, P, P, 40, 24, P, 39, P, P, 0, 0, P, *none) == SHAPE and d(5000, 3, P, P, P, 40, 24, P, 23, P, 0, P, *none) == SHAPE
+    assert f(5000, 3, P, P, P, 40, 24, P, 40, P, P, 0, 3, P, *none) == DTYPE and d(5000, 3, P, P, P, 40, 24, P, 24, P, -1, P, *none) == DTYPE
+    assert f(5000, 3, None, P, P, 40, 24, P, 40, P, P, 0, 0, P, *none) == NULL
+    assert f(5000, 3, P, None, P, 40, 24, P, 40, P, P, 0, 0, P, *none) == NULL and f(5000, 3, P, P, None, 40, 24, P, 40, P, P, 0, 0, P, *none) == NULL
+    assert f(5000, 3, P, P, P, 40, 24, P + 1, 40, P, P, 0, 0, P, *none) == ALIGN and d(5000, 3, P, P, P, 40, 24, P, 24, P + 2, 2, P, *none) == ALIGN
     assert w(5000, 3, P, P, P, 40, 24, P, 24, P, 40, 0, P, P, P, need - 1, None) == WORK
     assert w(5000, 3, P, P, P, 40, 24, P, 24, P, 40, 0, P, P, P + 8, need, None) == ALIGN
     assert w(5000, 3, P, P, P, 40, 24, P, 24, P, 40, 0, None, P, P, need, None) == NULL
-    assert f(0, 3, None, None, None, 40, 24, None, 40, None, None, 0, 0, None, None) == OK
+    assert f(0, 3, None, None, None, 40, 24, None, 40, None, None, 0, 0, None, *none) == OK
+    # large products of rows that are not whole pieces need room for copies of them, small ones and whole rows none
+    room = lib.nerf_grouped_workspace_bytes
+    assert room(500, 3, 41, 24, 1, 2) == room(10 ** 6, 3, 256, 256, 0, 2) == room(10 ** 6, 3, 256, 256, 1, 0) == 0
+    fwd, bwd = room(10 ** 6, 3, 67, 250, 0, 2), room(10 ** 6, 3, 67, 250, 1, 2)
+    assert 4 * 10 ** 6 * 68 <= fwd <= 4 * (10 ** 6 + 3 * 250) * 68 + 1024 and 4 * 10 ** 6 * 252 <= bwd <= 4 * (10 ** 6 * 252 + 3 * 250 * 68) + 1024
+    assert f(10 ** 6, 3, P, P, P, 67, 250, P, 67, P, P, 0, 2, P, P, fwd - 1, None) == WORK
+    assert d(10 ** 6, 3, P, P, P, 67, 250, P, 250, P, 2, P, P, bwd - 1, None) == WORK
+    assert f(10 ** 6, 3, P, P, P, 67, 250, P, 67, P, P, 0, 2, P, None, fwd, None) == NULL
+    assert d(10 ** 6, 3, P, P, P, 67, 250, P, 250, P, 2, P, P + 64, bwd, None) == ALIGN
     r = lib.nerf_relu_bwd
     assert r(-1, 24, P, 24, P, 0, P, None) == r(50, 0, P, 24, P, 0, P, None) == r(50, 24, P, 23, P, 0, P, None) == SHAPE
     assert r(50, 24, P, 24, P, 3, P, None) == DTYPE and r(50, 24, P, 24, P + 1, 0, P, None) == r(50, 24, P, 24, P, 2, P + 2, None) == ALIGN
@@ -123,9 +134,12 @@ def test_plans_are_sound_over_the_range_of_sizes(lib):
                 assert 256 <= lib.nerf_embed_bwd_workspace_bytes(n, g, dim) <= 2048 + 28 * n + 4 * g + 2 ** 20 + 8 * 1024 * (n // 1024 + 2) + 8 * dim * (n // 8 + 1)
             if g <= 65535:
                 for K, N in ((1, 1), (63, 256), (256, 256), (1024, 1024), (4, 2000), (65536, 65536)):
-                    b = lib.nerf_grouped_bwd_weights_workspace_bytes(n, g, K, N)
                     chunks = max(512, (n // 128 + g + 1) // 256 + 1)
-                    assert 256 <= b <= 1024 + 8 * chunks * (N * K + N)
+                    for prec in (0, 1, 2):
+                        b = lib.nerf_grouped_bwd_weights_workspace_bytes(n, g, K, N, prec)
+                        a = max(lib.nerf_grouped_workspace_bytes(n, g, K, N, way, prec) for way in (0, 1))
+                        assert 256 <= b <= 2048 + 8 * chunks * (N * K + N) + 4 * n * (N + K + 14)
+                        assert 0 <= a <= 1024 + 4 * (n + g * N) * (max(K, N) + 7)
     for B in (1, 2, 1000, 10 ** 6):
         for T in (0, 1, 2, 63, 64, 1000, 10 ** 6):
             for D in (1, 3, 64, 67, 256, 4096):
