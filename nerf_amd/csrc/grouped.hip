@@ -11,10 +11,11 @@
 // Operands in whole aligned 16-byte pieces are copied into a ring of LDS buffers by the memory system itself
 // (global_load_lds, 16 bytes per lane) and multiplied by persistent workgroups, one per compute unit (stream_kernel,
 // wgrad_stream_kernel): v_mfma_f32_32x32x16_{bf16,f16} or, in fp32, v_mfma_f32_32x32x2_f32 (exact products, fp32 sums).
-// Anything else goes through registers, one workgroup per tile (linear_kernel, wgrad_kernel).
+// Anything else goes through registers, one workgroup per tile (linear_kernel, wgrad_kernel), or is copied to whole pieces
+// first (pad_plan).
 //
 // Bounds: 256 -> 256 features move 1 KiB per row for 128 kflop, memory at 16 bits (floor 39 us for 196 608 rows; 57 forward,
-// 59 data gradient, 65 weight gradient) and the fp32 matrix instructions at 32 (65 536 rows: 56 us; 107, 108, 122).  1024 ->
+// 59 data gradient, 65 weight gradient) and the fp32 matrix instructions at 32 (65 536 rows: 56 us; 102, 110, 113).  1024 ->
 // 1024 features are bound by the copies into LDS, 29 bytes per ns and compute unit (65 536 rows fp16, 64 uneven groups: 220 to
 // 239 us; one group 170 us, 0.81 PFLOP/s, where a large library product reaches 1.06).
 //
@@ -255,7 +256,9 @@ struct Tables {
 // The accumulators hold outputs down and rows across: a lane's four consecutive registers are consecutive outputs of one
 // row, and one exchange between the wave's halves (v_permlane32_swap) makes them eight, a 16-byte store.
 constexpr int ST_THREADS = 512;
-constexpr int ST_ITEMS = 12;            // items whose rows and bias are in LDS at a time
+// items whose rows and bias are in LDS at a time; 64 outputs leave room for two workgroups in a compute unit's LDS
+// (65 536 rows 256 -> 256 fp32: 102 us with two, 111 with one)
+template <int BN> constexpr int st_items() { return BN == 64 ? 8 : 12; }
 
 // Output number of place o.  The last piece of a row ends where the row does, so it may repeat outputs of the one before, and
 // places behind it repeat it: the same values are stored again.
@@ -447,12 +450,13 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
     constexpr int A_BYTES = TILE_ROWS * 128, B_BYTES = WT ? tr_bytes<T, BN>() : BN * 128, STAGE = A_BYTES + B_BYTES;
     constexpr int NA = A_BYTES / 1024 / WAVES, NB = B_BYTES / 1024 / WAVES; // copies of a wave per step
     constexpr int COPIES = NA + NB;
+    constexpr int ITEMS = st_items<BN>();
     constexpr int STORES = MI * NJ * (sizeof(T) == 2 ? 2 : 4);              // stores of a wave per item
     static_assert(COPIES + 2 * STORES < 64, "vmcnt counts to 63");
     __shared__ __attribute__((aligned(1024))) char lds[3 * STAGE];
-    __shared__ int row_tab[ST_ITEMS][TILE_ROWS];
-    __shared__ __attribute__((aligned(16))) T bias_tab[ST_ITEMS][BN];
-    __shared__ int d_grp[ST_ITEMS], d_o0[ST_ITEMS], d_cnt[ST_ITEMS], d_pos[ST_ITEMS];
+    __shared__ int row_tab[ITEMS][TILE_ROWS];
+    __shared__ __attribute__((aligned(16))) T bias_tab[ITEMS][BN];
+    __shared__ int d_grp[ITEMS], d_o0[ITEMS], d_cnt[ITEMS], d_pos[ITEMS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m_off = (wave % WM) * (MI * 32), o_off = (wave / WM) * (NJ * 32);
     const int G = p.rows.n_groups, O = p.O, C = p.C;
@@ -498,9 +502,9 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
         }
     }
 
-    for (int64_t first = begin; first < finish; first += ST_ITEMS * stride) {
+    for (int64_t first = begin; first < finish; first += ITEMS * stride) {
         const int64_t left = (finish - first + stride - 1) / stride;
-        const int items = (int)(left < ST_ITEMS ? left : ST_ITEMS);
+        const int items = (int)(left < ITEMS ? left : ITEMS);
         __syncthreads();
         for (int i = wave; i < items; i += WAVES) {
             const Tile t = tables.tile(p.rows, first + i * stride, p.tiles_o, BN);
@@ -706,7 +710,7 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
 
 // ---- through registers: any row length, any alignment ------------------------------------------------------------
 // The same product, one workgroup of four waves per tile of 128 rows x BN outputs; a step is requested before the products of
-// the one before it (65 536 rows, 67 -> 256 bf16: forward 29 us, data gradient 40; in whole pieces, 64 -> 256, 18 and 20).
+// the one before it (65 536 rows, 67 -> 256 bf16: forward 24 us, data gradient 39; in whole pieces, 64 -> 256, 19 and 14).
 template <typename T, bool WT, int BN>
 __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();
@@ -911,10 +915,30 @@ NERF_WG_BLOCK(__bf16, "v_mfma_f32_32x32x16_bf16")
 NERF_WG_BLOCK(_Float16, "v_mfma_f32_32x32x16_f16")
 #undef NERF_WG_BLOCK
 
+// fp32: one block per 32 x 32 sums, four products each
+#define NERF_READ_F4(n, at) "ds_read_b32 %[" n "0], %[" at "]\n\tds_read_b32 %[" n "1], %[" at "] offset:%[row1]\n\tds_read_b32 %[" n "2], %[" at "] offset:%[row2]\n\tds_read_b32 %[" n "3], %[" at "] offset:%[row3]\n\t"
+#define NERF_MFMA32_W NERF_MFMA(NERF_OP32, "c", "e0", "f0") NERF_MFMA(NERF_OP32, "c", "e1", "f1") NERF_MFMA(NERF_OP32, "c", "e2", "f2") NERF_MFMA(NERF_OP32, "c", "e3", "f3")
+template <int PD, int PX, int NJ, typename F>
+__device__ __forceinline__ void block_wgrad(float, f32x16 (&c)[2][NJ], F (&d)[2], F (&x)[NJ], unsigned d0, unsigned d1, unsigned x0, unsigned) {
+    static_assert(NJ == 1 && PD == PX, "fp32 blocks are 128 x 128");
+    float a[4], b[4], w[4];
+    asm volatile(NERF_BLOCK_HEAD NERF_READ_F4("n", "at") NERF_READ_F4("m", "to") NERF_MFMA32_W NERF_BLOCK_TAIL
+                 : [c] "+v"(c[0][0]), [n0] "=&v"(a[0]), [n1] "=&v"(a[1]), [n2] "=&v"(a[2]), [n3] "=&v"(a[3]), [m0] "=&v"(w[0]), [m1] "=&v"(w[1]),
+                   [m2] "=&v"(w[2]), [m3] "=&v"(w[3])
+                 : NERF_IN4(e, d[0]), NERF_IN4(f, x[0]), [at] "v"(d0), [to] "v"(x0), [row1] "n"(PD), [row2] "n"(2 * PD), [row3] "n"(3 * PD)
+                 : "memory");
+    asm volatile(NERF_BLOCK_HEAD NERF_READ_F4("n", "at") NERF_MFMA32_W NERF_BLOCK_TAIL
+                 : [c] "+v"(c[1][0]), [n0] "=&v"(b[0]), [n1] "=&v"(b[1]), [n2] "=&v"(b[2]), [n3] "=&v"(b[3])
+                 : NERF_IN4(e, d[1]), NERF_IN4(f, x[0]), [at] "v"(d1), [row1] "n"(PD), [row2] "n"(2 * PD), [row3] "n"(3 * PD)
+                 : "memory");
+    d[0] = F{a[0], a[1], a[2], a[3]};
+    d[1] = F{b[0], b[1], b[2], b[3]};
+    x[0] = F{w[0], w[1], w[2], w[3]};
+}
+
 template <typename T, int BX>
 __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>(), WAVES = ST_THREADS / 64, BD = 128;
-    constexpr bool AHEAD = sizeof(T) == 2;                                  // fragments read one product step ahead
     constexpr int PER_TILE = TILE_ROWS / BK, S = ROW_PIECES / 2;
     constexpr int MI = 2, NJ = BX / 4 / 32;                                 // waves: 2 along n, 4 along k
     constexpr int D_BYTES = tr_bytes<T, BD>(), X_BYTES = tr_bytes<T, BX>(), STAGE = D_BYTES + X_BYTES;
@@ -930,12 +954,12 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
     typedef __attribute__((address_space(3))) char* lds_ptr;
     const unsigned lds0 = (unsigned)(uintptr_t)(lds_ptr)lds, rows0 = (unsigned)(uintptr_t)(lds_ptr)row_tab, grp0 = (unsigned)(uintptr_t)(lds_ptr)tile_grp;
 
-    // the blocks of one chunk next to each other on one XCD: they read the same rows
+    // the blocks of one chunk next to each other, on one XCD where there are eight chunks or more: they read the same rows
     const int G = p.rows.n_groups, K = p.K, N = p.N;
     const int tiles = p.rows.tile_base[G];                                  // the rows of no group stay out
     const int blocks = p.tiles_n * p.tiles_k;
     const int64_t chunks = (tiles + p.chunk - 1) / p.chunk;
-    const int64_t per_xcd = (chunks + 7) / 8 * blocks, local = blockIdx.x >> 3;
+    const int64_t per_xcd = (chunks * blocks + 7) / 8, local = blockIdx.x >> 3;
     const int64_t at = (blockIdx.x & 7) * per_xcd + local;
     if (local >= per_xcd || at >= chunks * blocks) return;
     const int c = (int)(at / blocks), blk = (int)(at % blocks);
@@ -1078,7 +1102,7 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
             const int i = s / PER_TILE;
             const int g = __builtin_amdgcn_readfirstlane(lds_int(grp0 + i * 4)), next = __builtin_amdgcn_readfirstlane(lds_int(grp0 + i * 4 + 4));
             if (g != next) {
-                if constexpr (AHEAD) settle<T, MI, NJ>(acc);
+                settle<T, MI, NJ>(acc);
                 flush(g);
                 clear();
             }
@@ -1088,57 +1112,34 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
         copy_step();
         int buf = 0;
         typename El<T>::frag d[MI], x[NJ];
-        if constexpr (AHEAD) {
-            copy_step();
-            wait_copies<2 * COPIES>();
-            __builtin_amdgcn_s_barrier();
+        copy_step();
+        wait_copies<2 * COPIES>();
+        __builtin_amdgcn_s_barrier();
 #pragma unroll
-            for (int i = 0; i < MI; ++i) d[i] = read_tr<T, BD * (int)sizeof(T)>(fd[0][i]);
+        for (int i = 0; i < MI; ++i) d[i] = read_tr<T, BD * (int)sizeof(T)>(fd[0][i]);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) x[j] = read_tr<T, BX * (int)sizeof(T)>(fx[0][j]);
-            for (int s = 0; s < steps; ++s) {
+        for (int j = 0; j < NJ; ++j) x[j] = read_tr<T, BX * (int)sizeof(T)>(fx[0][j]);
+        for (int s = 0; s < steps; ++s) {
 #pragma unroll
-                for (int u = 0; u < S; ++u) {
-                    add_rows(d, u);
-                    if (u == S - 1) {
-                        wait_copies<COPIES>();
-                        __builtin_amdgcn_s_barrier();
-                        buf = buf == 2 ? 0 : buf + 1;
-                    }
-                    const int n = (u + 1) % S;
-                    const unsigned stage = buf * STAGE;
-                    block_wgrad<BD * 2, BX * 2, NJ>(T(), acc, d, x, fd[n][0] + stage, fd[n][1] + stage, fx[n][0] + stage, fx[n][NJ - 1] + stage);
+            for (int u = 0; u < S; ++u) {
+                add_rows(d, u);
+                if (u == S - 1) {
+                    wait_copies<COPIES>();
+                    __builtin_amdgcn_s_barrier();
+                    buf = buf == 2 ? 0 : buf + 1;
                 }
-                copy_step();
-                end_step(s);
-            }
-        } else {
-            for (int s = 0; s < steps; ++s) {
-                wait_copies<COPIES>();
-                __builtin_amdgcn_s_barrier();
-                copy_step();
+                const int n = (u + 1) % S;
                 const unsigned stage = buf * STAGE;
-#pragma unroll
-                for (int u = 0; u < S; ++u) {
-#pragma unroll
-                    for (int i = 0; i < MI; ++i) d[i] = read_tr<T, BD * (int)sizeof(T)>(fd[u][i] + stage);
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) x[j] = read_tr<T, BX * (int)sizeof(T)>(fx[u][j] + stage);
-#pragma unroll
-                    for (int i = 0; i < MI; ++i)
-#pragma unroll
-                        for (int j = 0; j < NJ; ++j) acc[i][j] = El<T>::mfma(d[i], x[j], acc[i][j]);
-                    add_rows(d, u);
-                }
-                end_step(s);
-                buf = buf == 2 ? 0 : buf + 1;
+                block_wgrad<BD * (int)sizeof(T), BX * (int)sizeof(T), NJ>(T(), acc, d, x, fd[n][0] + stage, fd[n][1] + stage, fx[n][0] + stage, fx[n][NJ - 1] + stage);
             }
+            copy_step();
+            end_step(s);
         }
         wait_copies<0>();                                                   // nothing may land once the rows are written anew
     }
 }
 
-// The same through registers, four waves per BT x BT block: any row length, any alignment (65 536 rows, 67 -> 256 bf16, 43 us).
+// The same through registers, four waves per BT x BT block: any row length, any alignment (65 536 rows, 67 -> 256 bf16, 44 us).
 template <typename T, int BT>
 __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();                       // rows of one step
@@ -1149,12 +1150,12 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n_off = (wave & 1) * (BT / 2), k_off = (wave >> 1) * (BT / 2);
 
-    // the blocks of one chunk next to each other on one XCD: they read the same rows
+    // the blocks of one chunk next to each other, on one XCD where there are eight chunks or more: they read the same rows
     const int G = p.rows.n_groups;
     const int tiles = p.rows.tile_base[G];                                  // the rows of no group stay out
     const int blocks = p.tiles_n * p.tiles_k;
     const int64_t work = (int64_t)((tiles + p.chunk - 1) / p.chunk) * blocks;
-    const int64_t per_xcd = ((work + blocks - 1) / blocks + 7) / 8 * blocks;
+    const int64_t per_xcd = (work + 7) / 8;
     const int64_t local = blockIdx.x >> 3;
     const int64_t at = (blockIdx.x & 7) * per_xcd + local;
     if (local >= per_xcd || at >= work) return;
@@ -1395,8 +1396,8 @@ static int pad_rows(int64_t rows, int cols, const void* src, int64_t ld, void* d
     return nerf_launch_status();
 }
 
-// workgroups of a grid whose kernel spreads `work` over the eight XCDs in runs of `unit`
-static inline int64_t xcd_grid(int64_t work, int64_t unit) { return ((work + unit - 1) / unit + 7) / 8 * unit * 8; }
+// workgroups of a grid whose kernel gives each of the eight XCDs an equal run of `work`
+static inline int64_t xcd_grid(int64_t work) { return (work + 7) / 8 * 8; }
 
 struct WgradPlan {
     int bd, bx, tiles_n, tiles_k, chunk;
@@ -1442,7 +1443,7 @@ static int launch_linear(const LinArgs& args, int precision, bool wide, void* st
         }
         p.tiles_o = (p.O + bn - 1) / bn;
         int64_t grid = (tiles * p.tiles_o + 7) / 8 * 8;
-        if (grid > 256) grid = 256;
+        if (grid > (bn == 64 ? 512 : 256)) grid = bn == 64 ? 512 : 256;
 #define NERF_ST(T, BN) hipLaunchKernelGGL((stream_kernel<T, WT, BN>), dim3((unsigned)grid), dim3(ST_THREADS), 0, st, p)
 #define NERF_CALL(T)                                                \
     do {                                                            \
@@ -1458,7 +1459,7 @@ static int launch_linear(const LinArgs& args, int precision, bool wide, void* st
     }
     const int bn = p.O <= 64 ? 64 : 128;
     p.tiles_o = (p.O + bn - 1) / bn;
-    const int64_t grid = xcd_grid(tiles * p.tiles_o, 1);
+    const int64_t grid = xcd_grid(tiles * p.tiles_o);
     NERF_REQUIRE(grid < ((int64_t)1 << 31), NERF_E_SHAPE);
 #define NERF_CALL(T)                                                                                                           \
     do {                                                                                                                       \
@@ -1621,7 +1622,7 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
     p.part_w = (float*)((char*)workspace + w.part_w);
     p.part_b = (float*)((char*)workspace + w.part_b);
     const int64_t blocks = (int64_t)w.tiles_n * w.tiles_k;
-    const int64_t grid = gl::xcd_grid(w.chunks * blocks, blocks);
+    const int64_t grid = gl::xcd_grid(w.chunks * blocks);
     NERF_REQUIRE(grid < ((int64_t)1 << 31), NERF_E_SHAPE);
     hipStream_t st = (hipStream_t)stream;
     const dim3 join((unsigned)(((int64_t)N * K + N + gl::THREADS - 1) / gl::THREADS), (unsigned)n_groups);
