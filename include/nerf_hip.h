@@ -392,7 +392,7 @@ int nerf_group_offsets(int64_t n, int64_t n_groups, const int32_t *offsets_in, i
 int nerf_embed_fwd(int64_t n, const void *ids, int id_bytes, int64_t rows, int64_t dim, const void *table, int64_t table_ld,
                    float scale, int precision, void *out, void *stream);
 /* d_table [rows, dim] (written, not accumulated) = scale * the sum of d_out's rows by id.  fp32 sums in a fixed order (the
- * rows are grouped by id first), no atomics.  dim <= 2^20; rows, n as for nerf_group_rows; workspace 256-byte aligned. */
+ * rows are grouped by id first), no atomics.  dim <= 2^20; rows, n as for nerf_group_rows; workspace 256-byte aligned, of few positions and rows 0 bytes (nullable then). */
 int64_t nerf_embed_bwd_workspace_bytes(int64_t n, int64_t rows, int64_t dim);
 int nerf_embed_bwd(int64_t n, const void *ids, int id_bytes, int64_t rows, int64_t dim, const void *d_out, int64_t d_out_ld,
                    float scale, int precision, void *d_table, void *workspace, int64_t workspace_bytes, void *stream);

@@ -433,7 +433,7 @@ static BwdPlan bwd_plan(int64_t n, int64_t rows, int64_t dim) {
 
 extern "C" int64_t nerf_embed_bwd_workspace_bytes(int64_t n, int64_t rows, int64_t dim) {
     if (!nerf::emb::sizes_ok(n, rows, dim)) return NERF_E_SHAPE;
-    return nerf::emb::bwd_plan(n, rows, dim).bytes;
+    return nerf::emb::small_call(n, rows) ? 0 : nerf::emb::bwd_plan(n, rows, dim).bytes;
 }
 
 extern "C" int nerf_embed_bwd(int64_t n, const void* ids, int id_bytes, int64_t rows, int64_t dim, const void* d_out, int64_t d_out_ld,
@@ -442,18 +442,19 @@ extern "C" int nerf_embed_bwd(int64_t n, const void* ids, int id_bytes, int64_t 
     NERF_REQUIRE(emb::sizes_ok(n, rows, dim) && d_out_ld >= dim, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision) && (id_bytes == 4 || id_bytes == 8), NERF_E_DTYPE);
     if (n == 0) return NERF_OK;
-    NERF_REQUIRE(ids && d_out && d_table && workspace, NERF_E_NULL);
+    const bool small = emb::small_call(n, rows);
+    NERF_REQUIRE(ids && d_out && d_table && (workspace || small), NERF_E_NULL);
     const int es = elem_bytes(precision), full = 16 / es;
     NERF_REQUIRE(nerf_aligned(ids, (uintptr_t)id_bytes) && nerf_aligned(d_out, (uintptr_t)es) && nerf_aligned(d_table, (uintptr_t)es) &&
                  nerf_aligned(workspace, 256), NERF_E_ALIGN);
     const emb::BwdPlan plan = emb::bwd_plan(n, rows, dim);
-    NERF_REQUIRE(workspace_bytes >= plan.bytes, NERF_E_WORKSPACE);
+    NERF_REQUIRE(small || workspace_bytes >= plan.bytes, NERF_E_WORKSPACE);
     char* ws = (char*)workspace;
     hipStream_t st = (hipStream_t)stream;
     int32_t *order = (int32_t*)(ws + plan.order), *offsets = (int32_t*)(ws + plan.offsets), *keys = (int32_t*)(ws + plan.keys);
     const bool wide = dim >= full;
     const int vec = wide ? full : 1, lpr = emb::lanes_per_row(dim, vec);
-    if (emb::small_call(n, rows)) {
+    if (small) {
 #define NERF_SMALL(T, V, ID)                                                                                                      \
     hipLaunchKernelGGL((emb::bwd_small_kernel<T, V, ID>), dim3((unsigned)rows), dim3(emb::THREADS), 0, st, (int)n, (const ID*)ids, (int)dim, \
                        lpr, (const T*)d_out, d_out_ld, scale, (T*)d_table)

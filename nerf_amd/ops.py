@@ -778,6 +778,17 @@ def _row_major(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
 
 
+def _first_order(backward):
+    """``once_differentiable`` for the backward of a short call: its detour is taken only where a graph of the gradients is
+    asked for."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
 class RowGroups:
     """Rows dealt out to groups: what ``group_rows`` and ``row_groups`` return and ``grouped_linear`` takes.
 
@@ -860,19 +871,19 @@ class _EmbedRows(torch.autograd.Function):
         return _embed_fwd(ids, table, scale)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, d_out):
         (ids,) = ctx.saved_tensors
         rows, dim = ctx.sizes
         n, dev = ids.numel(), d_out.device
         if n == 0:
             return None, torch.zeros((rows, dim), dtype=d_out.dtype, device=dev), None
-        g, ld = _row_major(d_out.reshape(n, dim))
+        g, ld = _row_major(d_out if d_out.dim() == 2 else d_out.reshape(n, dim))
         d_table = torch.empty((rows, dim), dtype=g.dtype, device=dev)
         nbytes = _size("nerf_embed_bwd_workspace_bytes", n, rows, dim)
-        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        work = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
         _call("nerf_embed_bwd", "embed_bwd", dev, n, n, ids.data_ptr(), ids.element_size(), rows, dim, g.data_ptr(), ld, ctx.scale,
-              _ELEM[g.dtype], d_table.data_ptr(), work.data_ptr(), nbytes)
+              _ELEM[g.dtype], d_table.data_ptr(), _ptr(work), nbytes)
         return None, d_table, None
 
 
@@ -928,7 +939,7 @@ class _GroupedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, d_y):
         x, weight, y = ctx.saved_tensors
         groups, dev = ctx.groups, d_y.device
@@ -1039,7 +1050,7 @@ class _GatedScan(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, d_h, d_last):
         if d_h is None and d_last is None:
             return None, None, None, None
