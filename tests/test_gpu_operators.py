@@ -61,8 +61,9 @@ def make_ids(n, groups, kind, g, dtype=torch.int64):
 # ---- grouping ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
-@pytest.mark.parametrize("n,groups", [(1, 1), (2, 1), (63, 2), (64, 3), (65, 255), (1000, 256), (1025, 257), (2048, 8), (2048, 5000), (2049, 8), (2049, 300), (300001, 3000), (4096, 8), (4096, 5000), (4097, 8),
-                                      (4097, 255), (8192, 256), (12289, 70000), (100003, 64), (300000, 1), (50000, 65535)])
+@pytest.mark.parametrize("n,groups", [(1, 1), (2, 1), (63, 2), (64, 3), (65, 255), (1000, 256), (1025, 257), (2048, 8), (2048, 5000), (2049, 8),
+                                      (2049, 300), (300001, 3000), (1100000, 7), (3000001, 5000), (4096, 8), (4096, 5000), (4097, 8), (4097, 255),
+                                      (8192, 256), (12289, 70000), (100003, 64), (300000, 1), (50000, 65535)])
 def test_group_rows(n, groups, dtype):
     from nerf_amd import ops
     for kind in ("random", "skewed", "one", "none"):
