@@ -49,6 +49,7 @@ struct In {
 
 struct Args {
     Geo g;
+    int64_t block0;         // blocks of sequences that earlier launches of the call have taken
     In gate, value;
     const float* state;     // [B][D] or NULL
     int reverse;
@@ -73,7 +74,7 @@ struct Place {
 };
 
 template <int V>
-__device__ __forceinline__ Place place(const Geo& g) {
+__device__ __forceinline__ Place place(const Geo& g, int64_t block0) {
     Place p;
     p.lane = threadIdx.x & 63;
     p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -84,7 +85,7 @@ __device__ __forceinline__ Place place(const Geo& g) {
     p.tgi = p.unit % g.tg;
     p.wd = g.tg < in_wave ? g.tg : in_wave;       // threads of the tile in this wave
     p.u = p.tgi & (p.wd - 1);
-    p.b = (int64_t)blockIdx.x * g.seqs + p.seq_in;
+    p.b = (block0 + blockIdx.x) * g.seqs + p.seq_in;
     const int ch = ((int)blockIdx.y << g.cgl) * V + p.cg * V;
     p.on = p.b < g.B && ch < g.D;
     p.ch = min(ch, g.D - V);
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(THREADS) void fwd_kernel(Args a) {
     constexpr int VA = SHARED ? 1 : V, L = max_len<V>();
     __shared__ float sm[WAVES * 64 * (V + VA)];
     const Geo& g = a.g;
-    const Place p = place<V>(g);
+    const Place p = place<V>(g, a.block0);
     // the main pass begins with the segments that the first one read last: they are still in the last-level cache
     const int64_t seg = AGG ? blockIdx.z : g.segs - 1 - blockIdx.z;
     const int64_t first = seg * g.per_seg, stop = first + g.per_seg < g.tiles ? first + g.per_seg : g.tiles;
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(THREADS, 2) void bwd_kernel(Args a) {
     constexpr bool AHEAD = AGG || SHARED || V != 4;
     __shared__ float sm[WAVES * 64 * (V + VA)];
     const Geo& g = a.g;
-    const Place p = place<V>(g);
+    const Place p = place<V>(g, a.block0);
     // the main pass begins with the segments that the first one read last: they are still in the last-level cache
     const int64_t seg = AGG ? blockIdx.z : g.segs - 1 - blockIdx.z;
     const int64_t first = seg * g.per_seg, stop = first + g.per_seg < g.tiles ? first + g.per_seg : g.tiles;
@@ -442,6 +443,7 @@ __global__ __launch_bounds__(THREADS, 2) void bwd_kernel(Args a) {
 // per run of at most PER consecutive segments, whose maps it requests all at once (2 x 262 144 x 64 fp32, 512 segments: the whole
 // forward 127 -> 124 us, backward 173 -> 170).
 constexpr int MAX_SEGS = 64 * 16;
+constexpr int64_t MAX_BLOCKS = (int64_t)1 << 23;        // blocks of sequences of one launch
 template <bool DOWN, int PER>
 __device__ __forceinline__ void run_segments(int64_t segs, int64_t D, int64_t base, int lane, const float* start, const float* __restrict__ agg_a,
                                              const float* __restrict__ agg_h, float* __restrict__ seg_in) {
@@ -563,20 +565,26 @@ static int launch(Args& a, const Workspace& w, void* workspace, bool shared, boo
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     const int64_t seq_blocks = (g.B + g.seqs - 1) / g.seqs;
-    NERF_REQUIRE(seq_blocks < ((int64_t)1 << 31) && g.segs <= MAX_SEGS, NERF_E_SHAPE);
-    const dim3 grid((unsigned)seq_blocks, (unsigned)g.col_blocks, (unsigned)g.segs), block(THREADS);
+    NERF_REQUIRE(g.segs <= MAX_SEGS, NERF_E_SHAPE);
+    const dim3 block(THREADS);
     const int vec = vec_of(g.D, precision);
     if (g.segs > 1) {
         a.agg_a = (float*)(ws + w.agg_a); a.agg_h = (float*)(ws + w.agg_h); a.seg_in = (const float*)(ws + w.seg_in);
     }
     a.gate_part = (float*)(ws + w.gate_part);
-#define NERF_K(KERN, E, V, S, AGG) hipLaunchKernelGGL((KERN<E, V, S, AGG>), grid, block, 0, st, a)
+    // a launch has fewer than 2^32 threads in a direction; sequences beyond that go to further launches
+#define NERF_K(KERN, E, V, S, AGG)                                                                                          \
+    for (a.block0 = 0; a.block0 < seq_blocks; a.block0 += MAX_BLOCKS) {                                                     \
+        const int64_t left = seq_blocks - a.block0;                                                                         \
+        const dim3 grid((unsigned)(left < MAX_BLOCKS ? left : MAX_BLOCKS), (unsigned)g.col_blocks, (unsigned)g.segs);        \
+        hipLaunchKernelGGL((KERN<E, V, S, AGG>), grid, block, 0, st, a);                                                    \
+    }
 #define NERF_VS(KERN, E, AGG)                                                      \
     do {                                                                           \
-        if (vec > 1 && shared) NERF_K(KERN, E, full_vec<E>(), true, AGG);           \
-        else if (vec > 1) NERF_K(KERN, E, full_vec<E>(), false, AGG);               \
-        else if (shared) NERF_K(KERN, E, 1, true, AGG);                             \
-        else NERF_K(KERN, E, 1, false, AGG);                                        \
+        if (vec > 1 && shared) { NERF_K(KERN, E, full_vec<E>(), true, AGG) }        \
+        else if (vec > 1) { NERF_K(KERN, E, full_vec<E>(), false, AGG) }            \
+        else if (shared) { NERF_K(KERN, E, 1, true, AGG) }                          \
+        else { NERF_K(KERN, E, 1, false, AGG) }                                     \
     } while (0)
 #define NERF_CALL(E)                                                                                                      \
     do {                                                                                                                  \
