@@ -37,6 +37,9 @@ using grp::TILE_ROWS;
 constexpr int THREADS = 256;
 constexpr int ROW_PIECES = 8;                     // 16-byte pieces of one contraction step in a row: 128 bytes
 constexpr int MAX_CHUNK_TILES = 256;              // tiles one workgroup of the weight gradient walks
+// Workgroups in one direction of a grid: the runtime cuts off what passes 2^32 threads, without an error.  A multiple of the
+// eight XCDs that leaves room for workgroups of up to 512 threads.
+constexpr int64_t MAX_GRID = (int64_t)1 << 22;
 
 template <typename T> struct El;
 template <> struct El<__bf16> {
@@ -727,7 +730,7 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
     // consecutive tiles on one XCD (workgroups go round the eight XCDs), output tiles of the same rows next to each other
     const Tables tables(p.rows, lane);
     const int64_t work = (int64_t)tables.total * p.tiles_o;
-    const int64_t per_xcd = (work + 7) / 8, local = blockIdx.x >> 3;
+    const int64_t per_xcd = (work + 7) / 8, local = (blockIdx.x >> 3) + (int64_t)blockIdx.y * (gridDim.x >> 3);
     const int64_t at = (blockIdx.x & 7) * per_xcd + local;
     if (local >= per_xcd || at >= work) return;
     const Tile t = tables.tile(p.rows, at, p.tiles_o, BN);
@@ -1301,20 +1304,20 @@ __global__ __launch_bounds__(THREADS) void wgrad_join_kernel(WgradArgs p) {
     const int b0 = p.rows.tile_base[g], b1 = p.rows.tile_base[g + 1];
     const int c0 = b0 / p.chunk, c1 = b1 > b0 ? (b1 - 1) / p.chunk : c0;
     if (b1 > b0 && c0 == c1) return;
-    const int64_t NK = (int64_t)p.N * p.K;
-    const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-    const bool is_w = i < NK;
-    if (!is_w && !(p.db && i < NK + p.N)) return;
-    const float* part = is_w ? p.part_w + i : p.part_b + (i - NK);
-    const int64_t ld = is_w ? NK : p.N;
-    float sum = 0.0f;
-    if (b1 > b0) {
-        sum = part[(2 * (int64_t)c0 + 1) * ld];
+    const int64_t NK = (int64_t)p.N * p.K, all = p.db ? NK + p.N : NK;
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < all; i += (int64_t)gridDim.x * THREADS) {
+        const bool is_w = i < NK;
+        const float* part = is_w ? p.part_w + i : p.part_b + (i - NK);
+        const int64_t ld = is_w ? NK : p.N;
+        float sum = 0.0f;
+        if (b1 > b0) {
+            sum = part[(2 * (int64_t)c0 + 1) * ld];
 #pragma unroll 8
-        for (int c = c0 + 1; c <= c1; ++c) sum += part[2 * (int64_t)c * ld];
+            for (int c = c0 + 1; c <= c1; ++c) sum += part[2 * (int64_t)c * ld];
+        }
+        if (is_w) ((T*)p.dw)[g * NK + i] = (T)sum;
+        else ((T*)p.db)[(int64_t)g * p.N + (i - NK)] = (T)sum;
     }
-    if (is_w) ((T*)p.dw)[g * NK + i] = (T)sum;
-    else ((T*)p.db)[(int64_t)g * p.N + (i - NK)] = (T)sum;
 }
 
 // Rows that are not whole pieces, copied to rows that are, for the streaming forms: with zeros behind the last column, or
@@ -1459,12 +1462,14 @@ static int launch_linear(const LinArgs& args, int precision, bool wide, void* st
     }
     const int bn = p.O <= 64 ? 64 : 128;
     p.tiles_o = (p.O + bn - 1) / bn;
-    const int64_t grid = xcd_grid(tiles * p.tiles_o);
-    NERF_REQUIRE(grid < ((int64_t)1 << 31), NERF_E_SHAPE);
+    // many groups times many outputs: more workgroups than a direction of the grid holds threads for go to the next one
+    const int64_t work = xcd_grid(tiles * p.tiles_o), row = work < MAX_GRID ? work : MAX_GRID;
+    NERF_REQUIRE((work + row - 1) / row < 65536, NERF_E_SHAPE);
+    const dim3 grid((unsigned)row, (unsigned)((work + row - 1) / row));
 #define NERF_CALL(T)                                                                                                           \
     do {                                                                                                                       \
-        if (bn == 128) hipLaunchKernelGGL((linear_kernel<T, WT, 128>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);         \
-        else hipLaunchKernelGGL((linear_kernel<T, WT, 64>), dim3((unsigned)grid), dim3(THREADS), 0, st, p);                    \
+        if (bn == 128) hipLaunchKernelGGL((linear_kernel<T, WT, 128>), grid, dim3(THREADS), 0, st, p);                         \
+        else hipLaunchKernelGGL((linear_kernel<T, WT, 64>), grid, dim3(THREADS), 0, st, p);                                    \
     } while (0)
     NERF_ELEM_DISPATCH(precision, NERF_CALL);
 #undef NERF_CALL
@@ -1623,9 +1628,10 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
     p.part_b = (float*)((char*)workspace + w.part_b);
     const int64_t blocks = (int64_t)w.tiles_n * w.tiles_k;
     const int64_t grid = gl::xcd_grid(w.chunks * blocks);
-    NERF_REQUIRE(grid < ((int64_t)1 << 31), NERF_E_SHAPE);
+    NERF_REQUIRE(grid <= 2 * gl::MAX_GRID - 8, NERF_E_SHAPE);               // 512 threads each
     hipStream_t st = (hipStream_t)stream;
-    const dim3 join((unsigned)(((int64_t)N * K + N + gl::THREADS - 1) / gl::THREADS), (unsigned)n_groups);
+    const int64_t join_blocks = ((int64_t)N * K + N + gl::THREADS - 1) / gl::THREADS;
+    const dim3 join((unsigned)(join_blocks < gl::MAX_GRID ? join_blocks : gl::MAX_GRID), (unsigned)n_groups);
 #define NERF_WG(T, BT) hipLaunchKernelGGL((gl::wgrad_kernel<T, BT>), dim3((unsigned)grid), dim3(gl::THREADS), 0, st, p)
 #define NERF_WS(T, BX) hipLaunchKernelGGL((gl::wgrad_stream_kernel<T, BX>), dim3((unsigned)grid), dim3(gl::ST_THREADS), 0, st, p)
 #define NERF_CALL(T)                                                                                   \

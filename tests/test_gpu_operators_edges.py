@@ -17,6 +17,58 @@ def whole(g, lo, hi, *shape):
     return torch.randint(lo, hi + 1, shape, generator=g).float()
 
 
+# ---- layers of the largest sizes that the documentation allows -------------------------------------------------------
+
+def test_grouped_linear_gradient_of_the_largest_layer():
+    """65 536 x 65 536 features: more than 2^32 sums in d_weight, of a group that has rows and of one that has none"""
+    from nerf_amd import ops
+    n, F = 130, 65536
+    ids = torch.ones(n, dtype=torch.int32, device=DEV)
+    ids[3] = -1
+    x = torch.randint(-2, 3, (n, F), device=DEV, generator=torch.Generator(DEV).manual_seed(0)).bfloat16()
+    w = torch.zeros(2, F, F, dtype=torch.bfloat16, device=DEV)
+    w[1, -1, :40] = 1                                                       # one row and one column: sums of few terms
+    w[1, :, -1] = 2
+    w.requires_grad_(True)
+    bias = torch.zeros(2, F, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    y = ops.grouped_linear(x, w, ops.group_rows(ids, 2), bias=bias)
+    keep = torch.arange(n, device=DEV) != 3
+    want = (2 * x[:, -1:].float()).repeat(1, F)
+    want[:, -1] += x[:, :40].float().sum(1)
+    assert torch.equal(y.detach(), torch.where(keep[:, None], want, 0 * want).bfloat16())
+    d_y = torch.zeros(n, F, dtype=torch.bfloat16, device=DEV)
+    for i, cols in ((0, slice(0, 7)), (3, slice(0, None)), (5, slice(40000, 40100)), (129, slice(F - 3, None)), (64, slice(F - 1, None))):
+        d_y[i, cols] = torch.randint(-3, 4, d_y[i, cols].shape, device=DEV).bfloat16()
+    torch.cuda.empty_cache()
+    dirt = torch.full((2, F, F), 7.0, dtype=torch.bfloat16, device=DEV)     # what the gradient's memory held before
+    del dirt
+    dw, db = torch.autograd.grad(y, (w, bias), d_y)
+    d_y[3] = 0
+    assert torch.equal(db[1], d_y.float().sum(0).bfloat16()) and not db[0].any() and not dw[0].any()
+    for lo in range(0, F, 4096):
+        rows = d_y[:, lo:lo + 4096].float()
+        assert torch.equal(dw[1, lo:lo + 4096], (rows.t().contiguous() @ x.float()).bfloat16()), lo
+
+
+def test_grouped_linear_most_groups_times_most_outputs():
+    """65 535 groups of 65 536 outputs: more than 2^24 tiles of output, most of them of groups without rows"""
+    from nerf_amd import ops
+    n, G, N = 300, 65535, 65536
+    ids = torch.randint(0, G, (n,), device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    ids[:4] = torch.tensor([G - 1, 0, -1, G - 1], device=DEV)
+    w = torch.zeros(G, N, 1, dtype=torch.bfloat16, device=DEV)
+    w[ids.clamp_min(0)] = torch.randint(-4, 5, (n, N, 1), device=DEV).bfloat16()
+    x = torch.randint(-4, 5, (n, 1), device=DEV).bfloat16()
+    x.requires_grad_(True)
+    y = ops.grouped_linear(x, w, ops.group_rows(ids, G))
+    ok = (ids >= 0)[:, None]
+    assert torch.equal(y.detach(), torch.where(ok, x.detach() * w[ids.clamp_min(0), :, 0], torch.zeros((), device=DEV, dtype=torch.bfloat16)))
+    d_y = torch.zeros(n, N, dtype=torch.bfloat16, device=DEV)
+    d_y[:, -9:] = torch.randint(-2, 3, (n, 9), device=DEV).bfloat16()
+    dx = torch.autograd.grad(y, x, d_y)[0]
+    assert torch.equal(dx, torch.where(ok, (w[ids.clamp_min(0), -9:, 0].float() * d_y[:, -9:].float()).sum(1, keepdim=True), torch.zeros((), device=DEV)).bfloat16())
+
+
 # ---- scans of more sequences than one launch holds -------------------------------------------------------------------
 
 @pytest.mark.parametrize("B,D,dtype", [(2 ** 29 + 3, 7, torch.bfloat16), (2 ** 30 + 1, 3, torch.float16)])
