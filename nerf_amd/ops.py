@@ -11,6 +11,7 @@ import operator
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _C
@@ -778,13 +779,21 @@ def _row_major(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
 
 
+def _dual_level() -> bool:
+    """Whether inputs may carry forward-mode tangents.  Such a tensor has requires_grad False; a call has to go through its
+    autograd Function all the same, which refuses it, or the result would count as one whose derivative is zero."""
+    return forward_ad._current_level >= 0
+
+
 def _first_order(backward):
     """``once_differentiable`` for the backward of a short call: its detour is taken only where a graph of the gradients is
-    asked for."""
+    asked for.  Forward-mode tangents of the incoming gradients are refused as well."""
     recorded = once_differentiable(backward)
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        if _dual_level() and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            raise NotImplementedError("this operator has no forward-mode derivative of its gradients")
         return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
     return run
 
@@ -902,7 +911,7 @@ def embed_rows(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> to
     if table.shape[1] > 2 ** 20:
         raise ValueError(f"at most {2 ** 20} columns, got {table.shape[1]}")
     _group_sizes(ids.numel(), table.shape[0])
-    if torch.is_grad_enabled() and table.requires_grad:
+    if _dual_level() or torch.is_grad_enabled() and table.requires_grad:
         return _EmbedRows.apply(ids, table, float(scale))
     return _embed_fwd(ids, table, float(scale))
 
@@ -999,7 +1008,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
         if tuple(bias.shape) != (G, N):
             raise ValueError(f"bias must be [{G}, {N}], got {tuple(bias.shape)}")
     rows = x if x.dim() == 2 else x.reshape(-1, K)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
+    if _dual_level() or torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
         y = _GroupedLinear.apply(rows, weight, bias, groups, bool(relu))
     else:
         y = _grouped_fwd(rows, weight, bias, groups, bool(relu))[0]
@@ -1104,7 +1113,7 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: Optional[torch.Te
         return value.clone(), last
     if gate.shape[0] != B or gate.shape[1] != T:
         gate = gate.expand(B, T, gate.shape[2])
-    if torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or state is not None and state.requires_grad):
+    if _dual_level() or torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or state is not None and state.requires_grad):
         return _GatedScan.apply(gate, value, state, bool(reverse))
     return _scan_fwd(gate, value, state, bool(reverse), False)[:2]
 

@@ -17,6 +17,40 @@ def whole(g, lo, hi, *shape):
     return torch.randint(lo, hi + 1, shape, generator=g).float()
 
 
+# ---- forward-mode derivatives ----------------------------------------------------------------------------------------
+
+def test_forward_mode_is_refused_not_dropped():
+    """A tensor with a tangent has requires_grad False; a result without a tangent would count as a derivative of zero."""
+    import torch.autograd.forward_ad as fw
+    from nerf_amd import ops
+    ids = torch.tensor([0, 2, 1, 0], device=DEV)
+    table = torch.randn(3, 8, device=DEV)
+    groups = ops.group_rows(ids, 3)
+    x, w, b = torch.randn(4, 8, device=DEV), torch.randn(3, 5, 8, device=DEV), torch.randn(3, 5, device=DEV)
+    gate, value, state = torch.rand(2, 6, 8, device=DEV), torch.randn(2, 6, 8, device=DEV), torch.randn(2, 8, device=DEV)
+    calls = [(lambda t: ops.embed_rows(ids, t), table),
+             (lambda t: ops.grouped_linear(t, w, groups, bias=b, relu=True), x), (lambda t: ops.grouped_linear(x, t, groups, bias=b), w),
+             (lambda t: ops.grouped_linear(x, w, groups, bias=t), b), (lambda t: ops.grouped_linear(t, w, groups), x.view(2, 2, 8)),
+             (lambda t: ops.gated_scan(t, value), gate), (lambda t: ops.gated_scan(t, value), gate[:1, :, :1]),
+             (lambda t: ops.gated_scan(gate, t, state=state), value), (lambda t: ops.gated_scan(gate, value, state=t, reverse=True), state)]
+    for mode in (torch.enable_grad, torch.no_grad):
+        for call, t in calls:
+            with mode(), fw.dual_level(), pytest.raises(NotImplementedError):
+                call(fw.make_dual(t, torch.ones_like(t)))
+        with mode(), fw.dual_level():                                      # nothing carries a tangent: an ordinary call
+            for call, t in calls:
+                a, b2 = call(t), call(t)
+                assert all(torch.equal(p, q) for p, q in zip(a, b2))
+    for call, t in calls:
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
+        out = call(t.detach().requires_grad_(True))
+        out = out[0] if isinstance(out, tuple) else out
+        with fw.dual_level(), pytest.raises(NotImplementedError):          # nor are those of an incoming gradient
+            out.backward(fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
+        out.backward(torch.ones_like(out))
+
+
 # ---- layers of the largest sizes that the documentation allows -------------------------------------------------------
 
 def test_grouped_linear_gradient_of_the_largest_layer():
