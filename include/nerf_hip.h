@@ -443,6 +443,15 @@ int nerf_scan_bwd(int64_t B, int64_t T, int64_t D, const void *gate, int64_t gat
                   const void *value, int64_t value_sb, int64_t value_st, const float *state, const float *states,
                   const void *d_h, const float *d_last, int reverse, int precision, void *d_gate, void *d_value,
                   float *d_state, void *workspace, int64_t workspace_bytes, void *stream);
+/* The same for a gate that repeats over the sequences, the samples or both (gate_sb, gate_st 0): d_gate is the gradient of the
+ * gate itself, [B or 1, T or 1, D or 1] contiguous, summed over what it repeats over in fp32 and a fixed order and rounded once
+ * (the sum of nerf_scan_bwd's d_gate would add up rounded terms).  The workspace holds the fp32 terms. */
+int64_t nerf_scan_repeat_workspace_bytes(int64_t B, int64_t T, int64_t D, int gate_shared, int over_sequences, int over_samples,
+                                         int precision);
+int nerf_scan_bwd_repeat(int64_t B, int64_t T, int64_t D, const void* gate, int64_t gate_sb, int64_t gate_st, int gate_shared,
+                         const void* value, int64_t value_sb, int64_t value_st, const float* state, const float* states,
+                         const void* d_h, const float* d_last, int reverse, int over_sequences, int over_samples, int precision,
+                         void* d_gate, void* d_value, float* d_state, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Adam on a flat fp32 buffer -- the optimizer.step() of scripts/train_nerf.py:336
  * (torch.optim.Adam, no weight decay, no amsgrad).  step is 1-based. */

@@ -85,6 +85,9 @@ _SIGS = {
                               c_int64, P]),
     "nerf_scan_bwd": (c_int, [c_int64, c_int64, c_int64, P, c_int64, c_int64, c_int, P, c_int64, c_int64, P, P, P, P, c_int, c_int, P, P, P,
                               P, c_int64, P]),
+    "nerf_scan_repeat_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int]),
+    "nerf_scan_bwd_repeat": (c_int, [c_int64, c_int64, c_int64, P, c_int64, c_int64, c_int, P, c_int64, c_int64, P, P, P, P, c_int, c_int,
+                                     c_int, c_int, P, P, P, P, c_int64, P]),
     "nerf_adam_step": (c_int, [c_int64, P, P, P, P, c_float, c_float, c_float, c_float, c_int64, c_float, P]),
 }
 for _name, (_res, _args) in _SIGS.items():

@@ -321,8 +321,9 @@ __global__ __launch_bounds__(THREADS) void fwd_kernel(Args a) {
     }
 }
 
-// The same backwards in time.  AGG: the map of u over each segment.
-template <typename T, int V, bool SHARED, bool AGG>
+// The same backwards in time.  AGG: the map of u over each segment.  G: the type that the gate's gradient is written in, fp32
+// where it is summed over sequences or samples afterwards.
+template <typename T, int V, bool SHARED, bool AGG, typename G = T>
 __global__ __launch_bounds__(THREADS, 2) void bwd_kernel(Args a) {
     constexpr int VA = SHARED ? 1 : V, L = max_len<V>();
     // A tile is requested ahead, except where three fp32 tensors per channel would leave one wave per SIMD (or spill):
@@ -391,15 +392,15 @@ __global__ __launch_bounds__(THREADS, 2) void bwd_kernel(Args a) {
         else load_floats<V>(hs, a.states + (p.b * (g.tiles - 1) + i - 1) * g.D + p.ch, p.on);
         compose<V, VA, true>(g, p, A, U, carry, u, sm);
         compose<V, VA, false>(g, p, A2, H, hs, h, sm);
-        float G[L][V];
+        float gs[L][V];                                  // dL/dh in full
 #pragma unroll
         for (int j = L - 1; j >= 0; --j) {
             Pack<T, V> y;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                G[j][v] = (float)gr.x[j].v[v] + u[v];
-                u[v] = ga.at(j, v) * G[j][v];
-                y.v[v] = (T)G[j][v];
+                gs[j][v] = (float)gr.x[j].v[v] + u[v];
+                u[v] = ga.at(j, v) * gs[j][v];
+                y.v[v] = (T)gs[j][v];
             }
             const int64_t t = t0 + j;
             if (a.d_value && p.on && j < g.len && t < g.T)
@@ -415,17 +416,17 @@ __global__ __launch_bounds__(THREADS, 2) void bwd_kernel(Args a) {
             if constexpr (SHARED) {
                 float s = 0.0f;
 #pragma unroll
-                for (int v = 0; v < V; ++v) s += p.on && v >= p.again ? G[j][v] * h[v] : 0.0f;
+                for (int v = 0; v < V; ++v) s += p.on && v >= p.again ? gs[j][v] * h[v] : 0.0f;
                 for (int off = 1; off < (1 << g.cgl); off <<= 1) s += __shfl_xor(s, off, 64);
                 if (ok && p.cg == 0) {
-                    if (g.col_blocks == 1) ((T*)a.d_gate)[at] = (T)s;
+                    if (g.col_blocks == 1) ((G*)a.d_gate)[at] = (G)s;
                     else a.gate_part[(int64_t)blockIdx.y * g.B * g.T + at] = s;
                 }
             } else if (ok) {
-                Pack<T, V> y;
+                Pack<G, V> y;
 #pragma unroll
-                for (int v = 0; v < V; ++v) y.v[v] = (T)(G[j][v] * h[v]);
-                put<T, V>((T*)a.d_gate + at * g.D + p.ch, y);
+                for (int v = 0; v < V; ++v) y.v[v] = (G)(gs[j][v] * h[v]);
+                put<G, V>((G*)a.d_gate + at * g.D + p.ch, y);
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = fmaf(ga.at(j, v), h[v], (float)va.x[j].v[v]);
@@ -502,6 +503,33 @@ __global__ __launch_bounds__(THREADS) void gate_join_kernel(int64_t n, int parts
     }
 }
 
+// Gradient of a gate that repeats over sequences or samples: out [A][P][I] = sums of in [A][R][I] over P equal runs of R.  LX
+// threads along I, the others along R; each adds up every (256 / LX)-th term of its run, then they meet in pairs in LDS, so the
+// order is fixed and no term passes more than R / (256 / LX) + 8 additions.  Rounded to O at the store.
+template <typename O>
+__global__ __launch_bounds__(THREADS) void sum_kernel(int64_t A, int64_t R, int64_t I, int64_t P, int lx, const float* __restrict__ in,
+                                                      O* __restrict__ out) {
+    __shared__ float red[THREADS];
+    const int tx = (int)threadIdx.x & (lx - 1), ty = (int)threadIdx.x / lx, ly = THREADS / lx;
+    const int64_t cols = (I + lx - 1) / lx, per = (R + P - 1) / P;
+    for (int64_t item = blockIdx.x; item < A * P * cols; item += gridDim.x) {
+        const int64_t i = item % cols * lx + tx, ap = item / cols, a = ap / P, r0 = ap % P * per;
+        const int64_t r1 = r0 + per < R ? r0 + per : R;
+        float s = 0.0f;
+        if (i < I)
+#pragma unroll 4
+            for (int64_t r = r0 + ty; r < r1; r += ly) s += in[(a * R + r) * I + i];
+        red[threadIdx.x] = s;
+        __syncthreads();
+        for (int half = ly >> 1; half > 0; half >>= 1) {
+            if (ty < half) red[threadIdx.x] += red[threadIdx.x + half * lx];
+            __syncthreads();
+        }
+        if (ty == 0 && i < I) out[ap * I + i] = (O)red[threadIdx.x];
+        __syncthreads();
+    }
+}
+
 static inline bool sizes_ok(int64_t B, int64_t T, int64_t D) {
     return B >= 0 && T >= 0 && D >= 1 && D <= 65536 && B <= ((int64_t)1 << 31) && T <= ((int64_t)1 << 40) && B * D <= ((int64_t)1 << 40) &&
            (B == 0 || T <= ((int64_t)1 << 46) / (B * D));
@@ -560,7 +588,37 @@ static Workspace workspace(const Geo& g, bool shared_gate, bool backward) {
     return w;
 }
 
-static int launch(Args& a, const Workspace& w, void* workspace, bool shared, bool backward, int precision, void* stream) {
+// sum of the gate's gradient over sequences and / or samples: [A][R][I] in fp32, over R; P runs of R where one would leave the
+// chip short of workgroups
+struct Repeat {
+    int64_t A, R, I, P, full, part, bytes;      // full, part: byte offsets in the workspace
+    int lx;
+};
+static Repeat repeat_plan(const Geo& g, bool shared, bool over_b, bool over_t, int64_t at) {
+    const int64_t C = shared ? 1 : g.D;
+    Repeat r = {};
+    r.A = over_b ? 1 : g.B;
+    r.R = (over_b ? g.B : 1) * (over_t ? g.T : 1);
+    r.I = C * (over_t ? 1 : g.T);
+    r.lx = 1;
+    while (r.lx < THREADS && r.lx < r.I) r.lx <<= 1;
+    const int64_t blocks = r.A * ((r.I + r.lx - 1) / r.lx), runs = (r.R * r.lx + THREADS * 8 - 1) / (THREADS * 8);
+    r.P = blocks < 1024 ? (1024 + blocks - 1) / (blocks < 1 ? 1 : blocks) : 1;
+    if (r.P > runs) r.P = runs;
+    if (r.P < 1) r.P = 1;
+    r.full = at;
+    r.part = r.full + (g.B * g.T * C * 4 + 255) / 256 * 256;
+    r.bytes = r.part + (r.P > 1 ? (r.A * r.P * r.I * 4 + 255) / 256 * 256 : 0);
+    return r;
+}
+template <typename O>
+static void launch_sum(int64_t A, int64_t R, int64_t I, int64_t P, int lx, const float* in, O* out, hipStream_t st) {
+    const int64_t blocks = A * P * ((I + lx - 1) / lx), most = (int64_t)1 << 20;
+    hipLaunchKernelGGL(sum_kernel<O>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(THREADS), 0, st, A, R, I, P, lx, in, out);
+}
+
+// repeat: the gate's gradient is summed as it says (backward, with a gradient asked for), else NULL
+static int launch(Args& a, const Workspace& w, void* workspace, bool shared, bool backward, const Repeat* repeat, int precision, void* stream) {
     const Geo& g = a.g;
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
@@ -572,19 +630,28 @@ static int launch(Args& a, const Workspace& w, void* workspace, bool shared, boo
         a.agg_a = (float*)(ws + w.agg_a); a.agg_h = (float*)(ws + w.agg_h); a.seg_in = (const float*)(ws + w.seg_in);
     }
     a.gate_part = (float*)(ws + w.gate_part);
+    void* const d_gate = a.d_gate;
+    if (repeat) a.d_gate = ws + repeat->full;
     // a launch has fewer than 2^32 threads in a direction; sequences beyond that go to further launches
-#define NERF_K(KERN, E, V, S, AGG)                                                                                          \
+#define NERF_K(...)                                                                                                         \
     for (a.block0 = 0; a.block0 < seq_blocks; a.block0 += MAX_BLOCKS) {                                                     \
         const int64_t left = seq_blocks - a.block0;                                                                         \
         const dim3 grid((unsigned)(left < MAX_BLOCKS ? left : MAX_BLOCKS), (unsigned)g.col_blocks, (unsigned)g.segs);        \
-        hipLaunchKernelGGL((KERN<E, V, S, AGG>), grid, block, 0, st, a);                                                    \
+        hipLaunchKernelGGL((__VA_ARGS__), grid, block, 0, st, a);                                                           \
     }
-#define NERF_VS(KERN, E, AGG)                                                      \
-    do {                                                                           \
-        if (vec > 1 && shared) { NERF_K(KERN, E, full_vec<E>(), true, AGG) }        \
-        else if (vec > 1) { NERF_K(KERN, E, full_vec<E>(), false, AGG) }            \
-        else if (shared) { NERF_K(KERN, E, 1, true, AGG) }                          \
-        else { NERF_K(KERN, E, 1, false, AGG) }                                     \
+#define NERF_VS(KERN, E, ...)                                                              \
+    do {                                                                                   \
+        if (vec > 1 && shared) { NERF_K(KERN<E, full_vec<E>(), true, __VA_ARGS__>) }        \
+        else if (vec > 1) { NERF_K(KERN<E, full_vec<E>(), false, __VA_ARGS__>) }            \
+        else if (shared) { NERF_K(KERN<E, 1, true, __VA_ARGS__>) }                          \
+        else { NERF_K(KERN<E, 1, false, __VA_ARGS__>) }                                     \
+    } while (0)
+#define NERF_JOIN(O)                                                                                                        \
+    do {                                                                                                                    \
+        int64_t jb = (g.B * g.T + THREADS - 1) / THREADS;                                                                   \
+        if (jb > 8192) jb = 8192;                                                                                           \
+        hipLaunchKernelGGL(gate_join_kernel<O>, dim3((unsigned)jb), block, 0, st, g.B * g.T, g.col_blocks, a.gate_part,      \
+                           (O*)a.d_gate);                                                                                   \
     } while (0)
 #define NERF_CALL(E)                                                                                                      \
     do {                                                                                                                  \
@@ -597,22 +664,30 @@ static int launch(Args& a, const Workspace& w, void* workspace, bool shared, boo
             }                                                                                                             \
             NERF_VS(fwd_kernel, E, false);                                                                                \
         } else {                                                                                                          \
+            const bool join = shared && a.d_gate && g.col_blocks > 1;                                                     \
             if (g.segs > 1) {                                                                                             \
                 NERF_VS(bwd_kernel, E, true);                                                                             \
                 hipLaunchKernelGGL(segments_kernel<true>, gs, block, 0, st, g.B, g.segs, g.D, a.d_last, a.agg_a, a.agg_h, \
                                    (float*)a.seg_in);                                                                     \
             }                                                                                                             \
-            NERF_VS(bwd_kernel, E, false);                                                                                \
-            if (shared && a.d_gate && g.col_blocks > 1) {                                                                             \
-                int64_t jb = (g.B * g.T + THREADS - 1) / THREADS;                                                          \
-                if (jb > 8192) jb = 8192;                                                                                 \
-                hipLaunchKernelGGL(gate_join_kernel<E>, dim3((unsigned)jb), block, 0, st, g.B * g.T, g.col_blocks,         \
-                                   a.gate_part, (E*)a.d_gate);                                                            \
+            if (!repeat) {                                                                                                \
+                NERF_VS(bwd_kernel, E, false);                                                                            \
+                if (join) NERF_JOIN(E);                                                                                   \
+            } else {                                                                                                      \
+                NERF_VS(bwd_kernel, E, false, float);                                                                     \
+                if (join) NERF_JOIN(float);                                                                               \
+                const float* full = (const float*)a.d_gate;                                                               \
+                float* part = (float*)(ws + repeat->part);                                                                \
+                const bool two = repeat->P > 1;                                                                           \
+                if (two) launch_sum<float>(repeat->A, repeat->R, repeat->I, repeat->P, repeat->lx, full, part, st);        \
+                launch_sum<E>(repeat->A, two ? repeat->P : repeat->R, repeat->I, 1, repeat->lx, two ? part : full,         \
+                              (E*)d_gate, st);                                                                            \
             }                                                                                                             \
         }                                                                                                                 \
     } while (0)
     NERF_ELEM_DISPATCH(precision, NERF_CALL);
 #undef NERF_CALL
+#undef NERF_JOIN
 #undef NERF_VS
 #undef NERF_K
     return nerf_launch_status();
@@ -652,29 +727,63 @@ extern "C" int nerf_scan_fwd(int64_t B, int64_t T, int64_t D, const void* gate, 
     a.gate = {gate, gate_sb, gate_st};
     a.value = {value, value_sb, value_st};
     a.state = state; a.reverse = reverse ? 1 : 0; a.h = h; a.last = last; a.states = a.g.tiles > 1 ? states : nullptr;
-    return scan::launch(a, w, workspace, gate_shared != 0, false, precision, stream);
+    return scan::launch(a, w, workspace, gate_shared != 0, false, nullptr, precision, stream);
 }
 
-extern "C" int nerf_scan_bwd(int64_t B, int64_t T, int64_t D, const void* gate, int64_t gate_sb, int64_t gate_st, int gate_shared,
-                             const void* value, int64_t value_sb, int64_t value_st, const float* state, const float* states,
-                             const void* d_h, const float* d_last, int reverse, int precision, void* d_gate, void* d_value,
-                             float* d_state, void* workspace, int64_t workspace_bytes, void* stream) {
-    using namespace nerf;
-    NERF_REQUIRE(scan::sizes_ok(B, T, D) && gate_sb >= 0 && gate_st >= 0 && value_sb >= 0 && value_st >= 0, NERF_E_SHAPE);
+namespace nerf {
+namespace scan {
+
+static int backward(int64_t B, int64_t T, int64_t D, const void* gate, int64_t gate_sb, int64_t gate_st, bool shared, const void* value,
+                    int64_t value_sb, int64_t value_st, const float* state, const float* states, const void* d_h, const float* d_last,
+                    int reverse, bool over_b, bool over_t, int precision, void* d_gate, void* d_value, float* d_state, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+    NERF_REQUIRE(sizes_ok(B, T, D) && gate_sb >= 0 && gate_st >= 0 && value_sb >= 0 && value_st >= 0, NERF_E_SHAPE);
     NERF_REQUIRE(elem_ok(precision), NERF_E_DTYPE);
     if (B == 0 || T == 0) return NERF_OK;
-    scan::Args a = {};
-    a.g = scan::geometry(B, T, D, precision);
+    Args a = {};
+    a.g = geometry(B, T, D, precision);
     NERF_REQUIRE(gate && value && workspace && (states || a.g.tiles == 1), NERF_E_NULL);
     const uintptr_t es = (uintptr_t)elem_bytes(precision);
     NERF_REQUIRE(nerf_aligned(value, es) && nerf_aligned(gate, es) && nerf_aligned(d_h, es) && nerf_aligned(d_value, es) &&
                  nerf_aligned(d_gate, es) && nerf_aligned(state, 4) && nerf_aligned(states, 4) &&
                  nerf_aligned(d_last, 4) && nerf_aligned(d_state, 4) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
-    const scan::Workspace w = scan::workspace(a.g, gate_shared != 0, true);
-    NERF_REQUIRE(workspace_bytes >= w.bytes, NERF_E_WORKSPACE);
+    const Workspace w = scan::workspace(a.g, shared, true);
+    const bool sums = d_gate && (over_b || over_t);
+    const Repeat r = repeat_plan(a.g, shared, over_b, over_t, w.bytes);
+    NERF_REQUIRE(workspace_bytes >= (sums ? r.bytes : w.bytes), NERF_E_WORKSPACE);
     a.gate = {gate, gate_sb, gate_st};
     a.value = {value, value_sb, value_st};
     a.state = state; a.states = (float*)states; a.reverse = reverse ? 1 : 0;
     a.d_h = d_h; a.d_last = d_last; a.d_gate = d_gate; a.d_value = d_value; a.d_state = d_state;
-    return scan::launch(a, w, workspace, gate_shared != 0, true, precision, stream);
+    return launch(a, w, workspace, shared, true, sums ? &r : nullptr, precision, stream);
+}
+
+}  // namespace scan
+}  // namespace nerf
+
+extern "C" int nerf_scan_bwd(int64_t B, int64_t T, int64_t D, const void* gate, int64_t gate_sb, int64_t gate_st, int gate_shared,
+                             const void* value, int64_t value_sb, int64_t value_st, const float* state, const float* states,
+                             const void* d_h, const float* d_last, int reverse, int precision, void* d_gate, void* d_value,
+                             float* d_state, void* workspace, int64_t workspace_bytes, void* stream) {
+    return nerf::scan::backward(B, T, D, gate, gate_sb, gate_st, gate_shared != 0, value, value_sb, value_st, state, states, d_h, d_last,
+                                reverse, false, false, precision, d_gate, d_value, d_state, workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t nerf_scan_repeat_workspace_bytes(int64_t B, int64_t T, int64_t D, int gate_shared, int over_sequences, int over_samples,
+                                                    int precision) {
+    using namespace nerf;
+    if (!scan::sizes_ok(B, T, D)) return NERF_E_SHAPE;
+    if (!elem_ok(precision)) return NERF_E_DTYPE;
+    const scan::Geo g = scan::geometry(B, T, D, precision);
+    const int64_t at = scan::workspace(g, gate_shared != 0, true).bytes;
+    return over_sequences || over_samples ? scan::repeat_plan(g, gate_shared != 0, over_sequences != 0, over_samples != 0, at).bytes : at;
+}
+
+extern "C" int nerf_scan_bwd_repeat(int64_t B, int64_t T, int64_t D, const void* gate, int64_t gate_sb, int64_t gate_st, int gate_shared,
+                                    const void* value, int64_t value_sb, int64_t value_st, const float* state, const float* states,
+                                    const void* d_h, const float* d_last, int reverse, int over_sequences, int over_samples, int precision,
+                                    void* d_gate, void* d_value, float* d_state, void* workspace, int64_t workspace_bytes, void* stream) {
+    return nerf::scan::backward(B, T, D, gate, gate_sb, gate_st, gate_shared != 0, value, value_sb, value_st, state, states, d_h, d_last,
+                                reverse, over_sequences != 0, over_samples != 0, precision, d_gate, d_value, d_state, workspace,
+                                workspace_bytes, stream);
 }

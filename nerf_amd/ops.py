@@ -1034,6 +1034,8 @@ def _scan_fwd(gate, value, state, reverse, need):
     """(h, last, gate, value and state as they were read, the states the backward starts from)"""
     (B, T, D), dev, prec = value.shape, value.device, _ELEM[value.dtype]
     shared = gate.shape[2] == 1 and D > 1
+    if gate.shape[0] != B or gate.shape[1] != T:
+        gate = gate.expand(B, T, gate.shape[2])
     value, vsb, vst = _scan_input(value)
     gate, gsb, gst = _scan_input(gate)
     state = None if state is None else state.contiguous()
@@ -1052,6 +1054,8 @@ class _GatedScan(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gate, value, state, reverse):
+        # what the gate repeats over is summed here, in fp32: autograd would add up terms that are rounded to the gate's type
+        ctx.over = (gate.shape[0] != value.shape[0], gate.shape[1] != value.shape[1])
         h, last, gate, value, state, states = _scan_fwd(gate, value, state, reverse, True)
         ctx.save_for_backward(gate, value, state, states)
         ctx.reverse = reverse
@@ -1071,14 +1075,19 @@ class _GatedScan(torch.autograd.Function):
         value, vsb, vst = _scan_input(value)
         d_h = None if d_h is None else d_h.contiguous()
         d_last = None if d_last is None else d_last.contiguous()
-        d_gate = torch.empty((B, T, 1 if shared else D), dtype=value.dtype, device=dev) if need_gate else None
+        over_b, over_t = ctx.over
+        repeats = need_gate and (over_b or over_t)
+        d_gate = torch.empty((1 if over_b else B, 1 if over_t else T, 1 if shared else D), dtype=value.dtype, device=dev) if need_gate else None
         d_value = torch.empty((B, T, D), dtype=value.dtype, device=dev) if need_value else None
         d_state = torch.empty((B, D), dtype=torch.float32, device=dev) if need_state else None
-        nbytes = _size("nerf_scan_workspace_bytes", B, T, D, int(shared), 1, prec)
+        if repeats:
+            nbytes = _size("nerf_scan_repeat_workspace_bytes", B, T, D, int(shared), int(over_b), int(over_t), prec)
+        else:
+            nbytes = _size("nerf_scan_workspace_bytes", B, T, D, int(shared), 1, prec)
         work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-        _call("nerf_scan_bwd", "scan_bwd", dev, B * T, B, T, D, gate.data_ptr(), gsb, gst, int(shared), value.data_ptr(), vsb, vst,
-              _ptr(state), states.data_ptr(), _ptr(d_h), _ptr(d_last), int(ctx.reverse), prec, _ptr(d_gate), _ptr(d_value), _ptr(d_state),
-              work.data_ptr(), nbytes)
+        _call("nerf_scan_bwd_repeat" if repeats else "nerf_scan_bwd", "scan_bwd", dev, B * T, B, T, D, gate.data_ptr(), gsb, gst, int(shared),
+              value.data_ptr(), vsb, vst, _ptr(state), states.data_ptr(), _ptr(d_h), _ptr(d_last), int(ctx.reverse),
+              *((int(over_b), int(over_t)) if repeats else ()), prec, _ptr(d_gate), _ptr(d_value), _ptr(d_state), work.data_ptr(), nbytes)
         return d_gate, d_value, d_state, None
 
 
@@ -1086,8 +1095,9 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: Optional[torch.Te
                reverse: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """h[:, t] = gate[:, t] * h[:, t-1] + value[:, t] along the samples of each ray, from ``state`` (zeros when None):
     ``value`` [B, T, D]; ``gate`` [B, T, D], or [B, T, 1] for one gate per sample; size-1 batch and sample axes of the gate are
-    expanded.  ``reverse`` runs from the last sample to the first.  Returns (h [B, T, D] in the value's type, the state behind
-    the last step [B, D] in fp32), so that ``gated_scan(..., state=last)`` goes on with the next samples.
+    expanded, and its gradient summed over them in fp32.  ``reverse`` runs from the last sample to the first.  Returns
+    (h [B, T, D] in the value's type, the state behind the last step [B, D] in fp32), so that ``gated_scan(..., state=last)`` goes
+    on with the next samples.
 
     gate and value share one of bf16, fp16, fp32; ``state`` is fp32.  States are fp32 throughout, also in the backward pass,
     which recomputes them.  Time is cut into pieces that are composed, so the product of consecutive gates has to stay in the
@@ -1111,8 +1121,6 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: Optional[torch.Te
     if B == 0 or T == 0:
         last = value.new_zeros((B, D), dtype=torch.float32) if state is None else state.clone()
         return value.clone(), last
-    if gate.shape[0] != B or gate.shape[1] != T:
-        gate = gate.expand(B, T, gate.shape[2])
     if _dual_level() or torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or state is not None and state.requires_grad):
         return _GatedScan.apply(gate, value, state, bool(reverse))
     return _scan_fwd(gate, value, state, bool(reverse), False)[:2]

@@ -3,12 +3,14 @@
 Most operands here are small whole numbers (or halves), so that every sum is exact in fp32 in any order as long as its
 magnitude stays below 2^24 steps of its smallest term: results are compared bit for bit with the exact value rounded once,
 and a single missing, repeated or misplaced row shows."""
+import math
+
 import pytest
 import torch
 
 from util import ROOT  # noqa: F401  (puts the repository on the path)
 from oracle import operators_oracle as R
-from test_gpu_operators import DEV, DTYPES, close, gen, scan_case
+from test_gpu_operators import DEV, DTYPES, U, close, gen, scan_case
 
 pytestmark = pytest.mark.gpu
 
@@ -49,6 +51,98 @@ def test_forward_mode_is_refused_not_dropped():
         with fw.dual_level(), pytest.raises(NotImplementedError):          # nor are those of an incoming gradient
             out.backward(fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
         out.backward(torch.ones_like(out))
+
+
+# ---- gates that repeat over sequences or samples ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,D", [(3, 50, 32), (65, 3, 40), (1, 700, 9), (700, 1, 8), (5, 333, 3), (2, 4000, 130), (300, 40, 1), (2, 30, 1031)])
+def test_gated_scan_gradient_of_a_repeated_gate_is_summed_in_fp32(B, T, D, dtype):
+    """d_gate is a sum over B and / or T as well: its terms, the fp32 values of the full gate's gradient (2 (2 T + 192) + D
+    roundings, tests/test_gpu_operators.py), meet in fp32, at most one rounding per term, and are rounded to the type once"""
+    from nerf_amd import ops
+    for k, shape in enumerate(((1, T, 1), (B, 1, 1), (1, 1, 1), (1, T, D), (B, 1, D), (1, 1, D))):
+        gate, value, st, d_h, d_last = scan_case(B, T, D, shape, dtype, True)
+        ga, va, sa = (t.to(DEV).requires_grad_(True) for t in (gate, value, st))
+        runs = []
+        for _ in range(2):
+            h, last = ops.gated_scan(ga, va, state=sa, reverse=bool(k & 1))
+            runs.append(torch.autograd.grad((h, last), (ga, va, sa), (d_h.to(DEV), d_last.to(DEV))))
+        (eg, mg), (ev, mv), (es, ms) = R.gated_scan_grads(gate, value, st, bool(k & 1), d_h, d_last)
+        terms = 1
+        for ax in range(2):
+            if gate.shape[ax] != eg.shape[ax]:
+                terms *= eg.shape[ax]
+                eg, mg = eg.sum(ax, keepdim=True), mg.sum(ax, keepdim=True)
+        c = 2 * T + 192
+        got = runs[0][0]
+        assert got.dtype == dtype and got.shape == shape
+        # A sum from (2 - eps / 2) 2^e on, 2^e the type's largest power of two, is nearer to the first value behind the type's
+        # range than to the last one in it, so its rounding is infinite (fp16: 65 520); within the fp32 sum's error of that
+        # border it may be either.
+        f = torch.finfo(dtype)
+        border, err = (2 - f.eps / 2) * 2.0 ** math.floor(math.log2(f.max)), (2 * c + D + terms) * U * mg
+        beyond = got.isinf().cpu() & (eg.abs() + err >= border) & (got.cpu() * eg.sign() > 0)
+        assert bool((beyond | (eg.abs() - err < border)).all())
+        close(torch.where(beyond.to(DEV), 0, got), torch.where(beyond, 0, eg), torch.where(beyond, 0, mg), 2 * c + D + terms, "d_gate")
+        close(runs[0][1], ev, mv, c, "d_value")
+        close(runs[0][2], es, ms, c, "d_state")
+        assert all(torch.equal(p, q) for p, q in zip(*runs))
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 16), (1, 64, 16), (64, 1, 16), (1, 1, 1), (1, 64, 1), (64, 1, 1)])
+def test_gated_scan_repeated_gate_outside_the_range_of_a_term(shape):
+    """Zero gates: d_gate[t] = d_h[t] h[t-1] = d_h[t] value[t-1].  Terms of 2^-26, below fp16, add up to what it holds; terms of
+    +-2^17, beyond it, cancel."""
+    from nerf_amd import ops
+    gate = torch.zeros(shape, dtype=torch.float16, device=DEV, requires_grad=True)
+    full = (64, 64, shape[2])
+    for size, grad, sign in ((2.0 ** -13, 2.0 ** -13, False), (512.0, 256.0, True)):
+        value = torch.full((64, 64, 16), size, dtype=torch.float16, device=DEV)
+        d_h = torch.full((64, 64, 16), grad, dtype=torch.float16, device=DEV)
+        if sign:
+            d_h[1::2, ::2] *= -1
+            d_h[::2, 1::2] *= -1                                           # + - + - along both axes, as many of each
+            d_h[:, -1] = 0
+        terms = d_h.double() * torch.cat([torch.zeros(64, 1, 16, device=DEV).half(), value[:, :-1]], 1).double()
+        if shape[2] == 1:
+            terms = terms.sum(2, keepdim=True)
+        assert terms.shape == full
+        for ax in range(2):
+            if shape[ax] == 1:
+                terms = terms.sum(ax, keepdim=True)
+        got = torch.autograd.grad(ops.gated_scan(gate, value)[0], gate, d_h)[0]
+        assert torch.equal(got, terms.half())
+
+
+def test_repeated_gates_in_a_captured_graph():
+    """the sum over samples and sequences takes two launches here; replayed on new inputs with eager work in between"""
+    from nerf_amd import ops
+    def run(t):
+        h, last = ops.gated_scan(t[0], t[1], state=t[2])
+        return list(torch.autograd.grad((h, last), t[:3], (t[3], t[4])))
+    cases = [[t.to(DEV) for t in scan_case(3, 900, 24, (1, 1, 24), torch.bfloat16, True, seed)] for seed in range(3)]
+    static = [t.clone() for t in cases[0]]
+    for t in (*cases, static):
+        for leaf in t[:3]:
+            leaf.requires_grad_(True)
+    want = [run(t) for t in cases]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(static)
+    for i in (1, 2, 0, 2):
+        with torch.no_grad():
+            for a, b in zip(static, cases[i]):
+                a.copy_(b)
+        graph.replay()
+        run(cases[1])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
 
 
 # ---- layers of the largest sizes that the documentation allows -------------------------------------------------------
