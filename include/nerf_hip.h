@@ -401,7 +401,7 @@ int nerf_embed_bwd(int64_t n, const void *ids, int id_bytes, int64_t rows, int64
  *   y[i] = act(weight[g(i)] x[i] + bias[g(i)]), act = ReLU when relu (keeps a NaN), zeros for rows of no group.
  * order, offsets and tile_base from nerf_group_rows or nerf_group_offsets (order 0 .. n-1) for the same n and n_groups; rows
  * are read and written where they are (row order[p] of x [n, K], y [n, N]).  order must not name a row twice
- * (nerf_group_rows never does).
+ * (nerf_group_rows never does).  Tables that hold anything else give wrong values, but no access outside the tensors.
  * The backward calls take dZ [n, N], the gradient in front of the activation:
  *   nerf_relu_bwd:            d_z[i] = d_y[i] where y[i] is not <= 0, else 0 (contiguous [n, N]; needed after a ReLU only)
  *   nerf_grouped_bwd_data:    d_x[i] = weight[g(i)]^T d_z[i] [n, K], zeros for rows of no group

@@ -219,6 +219,7 @@ struct Tables {
         } else {
             total = r.tile_base[r.n_groups + 1];
         }
+        total = grp::checked_tiles(total, grp::max_tiles(r.n, r.n_groups));
     }
     __device__ __forceinline__ Tile tile(const Rows& r, int64_t at, int tiles_o, int bn) const {
         const int G = r.n_groups;
@@ -227,7 +228,7 @@ struct Tables {
         t.o0 = (int)(at % tiles_o) * bn;
         int first, begin, end;
         if (G < 63) {
-            t.group = __popcll(__ballot(lane <= G && base <= i)) - 1;
+            t.group = max((int)__popcll(__ballot(lane <= G && base <= i)) - 1, 0);
             first = __builtin_amdgcn_readlane(base, t.group);
             begin = __builtin_amdgcn_readlane(off, t.group);
             end = __builtin_amdgcn_readlane(off, min(t.group + 1, G));
@@ -237,9 +238,9 @@ struct Tables {
             begin = r.offsets[t.group];
             end = r.offsets[min(t.group + 1, G)];
         }
-        t.pos0 = begin + (int64_t)(i - first) * TILE_ROWS;
-        const int64_t left = (t.group < G ? (int64_t)end : r.n) - t.pos0;
-        t.count = (int)(left < TILE_ROWS ? left : TILE_ROWS);
+        const grp::Span span = grp::checked_span(begin + ((int64_t)i - first) * TILE_ROWS, t.group < G ? (int64_t)end : r.n, r.n);
+        t.pos0 = span.pos;
+        t.count = span.count;
         return t;
     }
 };
@@ -547,7 +548,7 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
         const T *pa[NA], *pb[NB];
         auto copy_step = [&]() {
             if (c_k == 0) {
-                const int g = __builtin_amdgcn_readfirstlane(lds_int((unsigned)(uintptr_t)(lds_ptr)&d_grp[c_item]));
+                const int g = min(__builtin_amdgcn_readfirstlane(lds_int((unsigned)(uintptr_t)(lds_ptr)&d_grp[c_item])), G - 1);
                 const int o0 = __builtin_amdgcn_readfirstlane(lds_int((unsigned)(uintptr_t)(lds_ptr)&d_o0[c_item]));
 #pragma unroll
                 for (int i = 0; i < NA; ++i) {
@@ -959,7 +960,7 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
 
     // the blocks of one chunk next to each other, on one XCD where there are eight chunks or more: they read the same rows
     const int G = p.rows.n_groups, K = p.K, N = p.N;
-    const int tiles = p.rows.tile_base[G];                                  // the rows of no group stay out
+    const int tiles = grp::checked_tiles(p.rows.tile_base[G], grp::max_tiles(p.rows.n, G));      // the rows of no group stay out
     const int blocks = p.tiles_n * p.tiles_k;
     const int64_t chunks = (tiles + p.chunk - 1) / p.chunk;
     const int64_t per_xcd = (chunks * blocks + 7) / 8, local = blockIdx.x >> 3;
@@ -1007,7 +1008,8 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
     };
     const bool bias = p.db && k0 == 0;
     auto flush = [&](int g) {
-        const int b0 = p.rows.tile_base[g], b1 = p.rows.tile_base[g + 1];
+        // within [0, tiles], so that a single chunk, which has no workspace, finishes every group
+        const int b0 = grp::checked_tiles(p.rows.tile_base[g], tiles), b1 = grp::checked_tiles(p.rows.tile_base[g + 1], tiles);
         const bool whole = b0 >= t0 && b1 <= t1;
         const int64_t slot = 2 * (int64_t)c + (b0 >= t0 ? 1 : 0);
 #pragma unroll
@@ -1055,10 +1057,9 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
             }
             tile_grp[i] = t < t1 ? lo : -1;                                 // of the tile behind the last one here too
             if (i < here) {
-                const int64_t pos = p.rows.offsets[lo] + (int64_t)(t - p.rows.tile_base[lo]) * TILE_ROWS;
-                const int64_t left = p.rows.offsets[lo + 1] - pos;
-                tile_pos[i] = (int)pos;
-                tile_cnt[i] = (int)(left < TILE_ROWS ? left : TILE_ROWS);
+                const grp::Span span = grp::checked_span(p.rows.offsets[lo] + ((int64_t)t - p.rows.tile_base[lo]) * TILE_ROWS, p.rows.offsets[lo + 1], p.rows.n);
+                tile_pos[i] = (int)span.pos;
+                tile_cnt[i] = span.count;
             }
         }
         __syncthreads();
@@ -1155,7 +1156,7 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
 
     // the blocks of one chunk next to each other, on one XCD where there are eight chunks or more: they read the same rows
     const int G = p.rows.n_groups;
-    const int tiles = p.rows.tile_base[G];                                  // the rows of no group stay out
+    const int tiles = grp::checked_tiles(p.rows.tile_base[G], grp::max_tiles(p.rows.n, G));      // the rows of no group stay out
     const int blocks = p.tiles_n * p.tiles_k;
     const int64_t work = (int64_t)((tiles + p.chunk - 1) / p.chunk) * blocks;
     const int64_t per_xcd = (work + 7) / 8;
@@ -1173,10 +1174,9 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
             if (p.rows.tile_base[mid] <= t) lo = mid;
             else hi = mid;
         }
-        const int64_t pos = p.rows.offsets[lo] + (int64_t)(t - p.rows.tile_base[lo]) * TILE_ROWS;
-        const int64_t left = p.rows.offsets[lo + 1] - pos;
-        tile_pos[i] = (int)pos;
-        tile_cnt[i] = (int)(left < TILE_ROWS ? left : TILE_ROWS);
+        const grp::Span span = grp::checked_span(p.rows.offsets[lo] + ((int64_t)t - p.rows.tile_base[lo]) * TILE_ROWS, p.rows.offsets[lo + 1], p.rows.n);
+        tile_pos[i] = (int)span.pos;
+        tile_cnt[i] = span.count;
         tile_grp[i] = lo;
     }
     __syncthreads();
@@ -1226,7 +1226,8 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
     };
     const bool bias = p.db && k0 == 0 && k_off == 0;
     auto flush = [&](int g) {
-        const int b0 = p.rows.tile_base[g], b1 = p.rows.tile_base[g + 1];
+        // within [0, tiles], so that a single chunk, which has no workspace, finishes every group
+        const int b0 = grp::checked_tiles(p.rows.tile_base[g], tiles), b1 = grp::checked_tiles(p.rows.tile_base[g + 1], tiles);
         const bool whole = b0 >= t0 && b1 <= t1;
         const int64_t slot = 2 * (int64_t)c + (b0 >= t0 ? 1 : 0);
 #pragma unroll
@@ -1301,7 +1302,8 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
 template <typename T>
 __global__ __launch_bounds__(THREADS) void wgrad_join_kernel(WgradArgs p) {
     const int g = blockIdx.y;
-    const int b0 = p.rows.tile_base[g], b1 = p.rows.tile_base[g + 1];
+    const int64_t most = grp::max_tiles(p.rows.n, p.rows.n_groups);
+    const int b0 = grp::checked_tiles(p.rows.tile_base[g], most), b1 = grp::checked_tiles(p.rows.tile_base[g + 1], most);
     const int c0 = b0 / p.chunk, c1 = b1 > b0 ? (b1 - 1) / p.chunk : c0;
     if (b1 > b0 && c0 == c1) return;
     const int64_t NK = (int64_t)p.N * p.K, all = p.db ? NK + p.N : NK;
@@ -1355,7 +1357,6 @@ __global__ __launch_bounds__(THREADS) void relu_bwd_kernel(int64_t n, int N, con
 static inline bool sizes_ok(int64_t n, int64_t n_groups, int K, int N) {
     return n >= 0 && n <= grp::MAX_ROWS && n_groups >= 1 && n_groups <= 65535 && K >= 1 && K <= 65536 && N >= 1 && N <= 65536;
 }
-static inline int64_t max_tiles(int64_t n, int64_t n_groups) { return n / TILE_ROWS + n_groups + 1; }
 
 // Operands whose rows are not whole pieces are copied to rows that are, and streamed, where that pays; a copy and its launch
 // cost 5 us and up.  Measured, register form against copy and streaming form:
@@ -1413,7 +1414,7 @@ static WgradPlan wgrad_plan(int64_t n, int64_t n_groups, int K, int N, bool wide
     w.bx = wide && precision != NERF_PREC_FP32 && K > 128 ? 256 : w.bd;
     w.tiles_n = (N + w.bd - 1) / w.bd;
     w.tiles_k = (K + w.bx - 1) / w.bx;
-    const int64_t tiles = max_tiles(n, n_groups), blocks = (int64_t)w.tiles_n * w.tiles_k;
+    const int64_t tiles = grp::max_tiles(n, n_groups), blocks = (int64_t)w.tiles_n * w.tiles_k;
     int64_t chunks = (wide ? 256 : 512) / blocks;
     if (chunks < 1) chunks = 1;
     int64_t chunk = (tiles + chunks - 1) / chunks;
@@ -1433,7 +1434,7 @@ template <bool WT>
 static int launch_linear(const LinArgs& args, int precision, bool wide, void* stream) {
     LinArgs p = args;
     hipStream_t st = (hipStream_t)stream;
-    const int64_t tiles = max_tiles(p.rows.n, p.rows.n_groups);
+    const int64_t tiles = grp::max_tiles(p.rows.n, p.rows.n_groups);
     if (wide) {
         // Output tile: the width with the least work on the busiest compute unit, ceil(items / 256) tiles of BN + an
         // overhead for reading the rows once more per tile (which weighs more where the products are fast).

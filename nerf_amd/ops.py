@@ -803,13 +803,33 @@ class RowGroups:
 
     ``offsets`` [n_groups + 1] int32: positions offsets[g] .. offsets[g+1] - 1 hold the rows of group g.  ``order`` [n] int32:
     the row at each position (every row once).  Rows behind offsets[n_groups] belong to no group.
-    All on the GPU; nothing is read back to the host.  Treat the tensors as read-only.
+    ``tile_base`` [n_groups + 2] int32: the 128-row tiles in front of each group, and of the rows of no group.
+    All on the GPU; nothing is read back to the host.  Treat the tensors as read-only: what else is written into them gives wrong
+    results, though never an access outside the operands.  The fields cannot be replaced.
     """
     __slots__ = ("order", "offsets", "tile_base", "n_rows", "n_groups")
 
     def __init__(self, order, offsets, tile_base, n_rows, n_groups):
-        self.order, self.offsets, self.tile_base = order, offsets, tile_base
-        self.n_rows, self.n_groups = n_rows, n_groups
+        n_rows, n_groups = operator.index(n_rows), operator.index(n_groups)
+        _group_sizes(n_rows, n_groups)
+        for t, name, size in ((order, "order", n_rows), (offsets, "offsets", n_groups + 1), (tile_base, "tile_base", n_groups + 2)):
+            t = _gpu_ids(t, name)
+            if t.dtype != torch.int32:
+                raise TypeError(f"{name} must be int32, got {t.dtype}")
+            if t.dim() != 1 or t.numel() != size:
+                raise ValueError(f"{name} must be [{size}], got {tuple(t.shape)}")
+            if t.device != order.device:
+                raise RuntimeError(f"{name} is on {t.device}, order on {order.device}")
+        _fill_row_groups(self, order.contiguous(), offsets.contiguous(), tile_base.contiguous(), n_rows, n_groups)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"RowGroups.{name} cannot be replaced")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"RowGroups.{name} cannot be removed")
+
+    def __reduce__(self):
+        return RowGroups, tuple(getattr(self, name) for name in self.__slots__)
 
 
 _MAX_GROUPED_ROWS = 2 ** 31 - 1 - 128
@@ -819,8 +839,20 @@ _MAX_GROUPS = 2 ** 24
 def _group_sizes(n: int, n_groups: int) -> None:
     if not 1 <= n_groups <= _MAX_GROUPS:
         raise ValueError(f"the number of groups must be between 1 and {_MAX_GROUPS}, got {n_groups}")
-    if n > _MAX_GROUPED_ROWS:
-        raise ValueError(f"at most {_MAX_GROUPED_ROWS} rows, got {n}")
+    if not 0 <= n <= _MAX_GROUPED_ROWS:
+        raise ValueError(f"between 0 and {_MAX_GROUPED_ROWS} rows, got {n}")
+
+
+_set_order, _set_offsets, _set_tile_base, _set_n_rows, _set_n_groups = (getattr(RowGroups, name).__set__ for name in RowGroups.__slots__)
+
+
+def _fill_row_groups(groups, order, offsets, tile_base, n_rows, n_groups) -> RowGroups:
+    _set_order(groups, order)
+    _set_offsets(groups, offsets)
+    _set_tile_base(groups, tile_base)
+    _set_n_rows(groups, n_rows)
+    _set_n_groups(groups, n_groups)
+    return groups
 
 
 def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
@@ -839,7 +871,7 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
     work = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     _call("nerf_group_rows", "group_rows", dev, n, n, ids.data_ptr(), ids.element_size(), n_groups, order.data_ptr(), offsets.data_ptr(),
           base.data_ptr(), work.data_ptr(), nbytes)
-    return RowGroups(order, offsets, base, n, n_groups)
+    return _fill_row_groups(RowGroups.__new__(RowGroups), order, offsets, base, n, n_groups)
 
 
 def row_groups(offsets: torch.Tensor, n_rows: int) -> RowGroups:
@@ -850,15 +882,13 @@ def row_groups(offsets: torch.Tensor, n_rows: int) -> RowGroups:
     if offsets.dim() != 1 or offsets.numel() < 2:
         raise ValueError(f"offsets must be 1-D with one entry more than there are groups, got {tuple(offsets.shape)}")
     n_rows, n_groups, dev = operator.index(n_rows), offsets.numel() - 1, offsets.device
-    if n_rows < 0:
-        raise ValueError(f"n_rows must not be negative, got {n_rows}")
     _group_sizes(n_rows, n_groups)
     given = offsets.clamp(0, n_rows).to(torch.int32)
     new = torch.zeros if n_rows == 0 else torch.empty
     clean = new((n_groups + 1,), dtype=torch.int32, device=dev)
     base = new((n_groups + 2,), dtype=torch.int32, device=dev)
     _call("nerf_group_offsets", "group_offsets", dev, n_rows, n_rows, n_groups, given.data_ptr(), clean.data_ptr(), base.data_ptr())
-    return RowGroups(torch.arange(n_rows, dtype=torch.int32, device=dev), clean, base, n_rows, n_groups)
+    return _fill_row_groups(RowGroups.__new__(RowGroups), torch.arange(n_rows, dtype=torch.int32, device=dev), clean, base, n_rows, n_groups)
 
 
 def _embed_fwd(ids, table, scale):

@@ -145,6 +145,88 @@ def test_repeated_gates_in_a_captured_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
 
 
+# ---- what a group table may hold ---------------------------------------------------------------------------------------
+
+def test_row_groups_checks_its_fields_and_keeps_them():
+    import copy
+    import pickle
+    from nerf_amd import ops
+    good = ops.group_rows(torch.tensor([1, 0, 7, 1, 1], device=DEV), 2)
+    order, offsets, base = good.order, good.offsets, good.tile_base
+    for err, args in ((TypeError, (order.long(), offsets, base, 5, 2)), (TypeError, (order, offsets.float(), base, 5, 2)),
+                      (TypeError, (order, offsets, [0, 1, 2, 3], 5, 2)), (ValueError, (order[:4], offsets, base, 5, 2)),
+                      (ValueError, (order, offsets, base, 6, 2)), (ValueError, (order, offsets, base, 5, 1)), (ValueError, (order, offsets, base[1:], 5, 2)),
+                      (ValueError, (order[None], offsets, base, 5, 2)), (ValueError, (order, offsets, base, -1, 2)), (ValueError, (order, offsets, base, 5, 0)),
+                      (TypeError, (order, offsets, base, 5.0, 2)), (RuntimeError, (order, offsets.cpu(), base, 5, 2)), (RuntimeError, (order.cpu(), offsets, base, 5, 2))):
+        with pytest.raises(err):
+            ops.RowGroups(*args)
+    for name in ("order", "offsets", "tile_base", "n_rows", "n_groups", "other"):
+        with pytest.raises(AttributeError):
+            setattr(good, name, order)
+        with pytest.raises(AttributeError):
+            delattr(good, name)
+    x, w = torch.randn(5, 8, device=DEV), torch.randn(2, 3, 8, device=DEV)
+    want = ops.grouped_linear(x, w, good)
+    wide = torch.stack([order, order], 1)[:, 0]                            # not contiguous
+    for other in (ops.RowGroups(wide, offsets, base, 5, 2), copy.copy(good), copy.deepcopy(good), pickle.loads(pickle.dumps(good))):
+        assert torch.equal(ops.grouped_linear(x, w, other), want) and (other.n_rows, other.n_groups) == (5, 2)
+
+
+def bad_tables(n, G, g):
+    """tables of the right size that no grouping gives: of other rows, out of order, out of range"""
+    from nerf_amd import ops
+    most = n // 128 + G + 1
+    other = ops.group_rows(torch.randint(0, G, (n,), generator=g).to(DEV) // 2, G)
+    good = ops.group_rows(torch.randint(0, G, (n,), generator=g).to(DEV), G)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    full = lambda size, v: torch.full((size,), v, **i32)
+    wild = lambda size: torch.randint(-2 ** 31, 2 ** 31, (size,), generator=g).to(torch.int32).to(DEV)
+    yield "boundaries of other rows", good.order, other.offsets, good.tile_base
+    yield "tiles of other rows", good.order, good.offsets, other.tile_base
+    yield "boundaries backwards", good.order, good.offsets.flip(0), good.tile_base
+    yield "tiles backwards", good.order, good.offsets, good.tile_base.flip(0)
+    yield "positions behind the rows", good.order, good.offsets + n, good.tile_base
+    yield "tiles behind the last", good.order, good.offsets, good.tile_base + most
+    yield "twice the tiles", good.order, good.offsets, good.tile_base * 2
+    yield "nothing below zero", good.order, full(G + 1, -1), full(G + 2, -1)
+    yield "all at the top", good.order, full(G + 1, 2 ** 31 - 1), full(G + 2, 2 ** 31 - 1)
+    yield "all at the bottom", good.order, full(G + 1, -2 ** 31), full(G + 2, -2 ** 31)
+    yield "rows that are none", wild(n), good.offsets, good.tile_base
+    yield "anything", wild(n), wild(G + 1), wild(G + 2)
+    yield "tiles in any order", good.order, good.offsets, torch.randint(0, most + 1, (G + 2,), generator=g).to(torch.int32).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,G,K,N", [(1000, 8, 256, 256), (500, 70, 63, 40), (40000, 3, 64, 128), (40000, 3, 67, 40), (3000, 80, 128, 64), (300, 2, 64, 64)])
+def test_grouped_linear_stays_inside_its_tensors_whatever_the_tables_hold(n, G, K, N, dtype):
+    """the C entry points on outputs and workspaces that lie between guards; every kernel ends, nothing outside is written.  (What
+    the kernels do with such tables is bounded in groups.hpp: checked_tiles, checked_span.)"""
+    from nerf_amd import ops
+    from nerf_amd._C import check, lib
+    g = gen(n + K)
+    code, size = ops._ELEM[dtype], torch.finfo(dtype).bits // 8
+    x, w, b, d_y = (torch.randn(s, generator=g).to(dtype).to(DEV) for s in ((n, K), (G, N, K), (G, N), (n, N)))
+    guard, st = 1 << 16, torch.cuda.current_stream().cuda_stream
+    room = lib.nerf_grouped_bwd_weights_workspace_bytes(n, G, K, N, code)
+    areas = {name: torch.empty(bytes_ + 2 * guard, dtype=torch.uint8, device=DEV)
+             for name, bytes_ in (("y", n * N * size), ("dx", n * K * size), ("dw", G * N * K * size), ("db", G * N * size), ("work", room))}
+    at = {name: a.data_ptr() + guard for name, a in areas.items()}
+    nf, nb = (lib.nerf_grouped_workspace_bytes(n, G, K, N, way, code) for way in (0, 1))
+    small = torch.empty(max(nf, nb, 256), dtype=torch.uint8, device=DEV)
+    for what, order, offsets, base in bad_tables(n, G, g):
+        print(what, n, G, K, N, dtype, flush=True)
+        for a in areas.values():
+            a.fill_(0x5a)
+        t = ops.RowGroups(order, offsets, base, n, G)
+        p = (n, G, t.order.data_ptr(), t.offsets.data_ptr(), t.tile_base.data_ptr(), K, N)
+        check(lib.nerf_grouped_fwd(*p, x.data_ptr(), K, w.data_ptr(), b.data_ptr(), 1, code, at["y"], small.data_ptr(), nf, st), "fwd")
+        check(lib.nerf_grouped_bwd_data(*p, d_y.data_ptr(), N, w.data_ptr(), code, at["dx"], small.data_ptr(), nb, st), "bwd_data")
+        check(lib.nerf_grouped_bwd_weights(*p, d_y.data_ptr(), N, x.data_ptr(), K, code, at["dw"], at["db"], at["work"], room, st), "bwd_weights")
+        torch.cuda.synchronize()
+        for name, a in areas.items():
+            assert a[:guard].eq(0x5a).all() and a[-guard:].eq(0x5a).all(), (what, name)
+
+
 # ---- layers of the largest sizes that the documentation allows -------------------------------------------------------
 
 def test_grouped_linear_gradient_of_the_largest_layer():
