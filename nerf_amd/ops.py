@@ -973,16 +973,19 @@ class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, relu):
         y, x, weight = _grouped_fwd(x, weight, bias, groups, relu)
-        ctx.save_for_backward(x, weight, y if relu else None)
-        ctx.groups = groups
+        # the tables are saved like any input, so that writing into them before the backward is an error; tables made in inference
+        # mode cannot be saved, nor written into outside of it
+        tables = (groups.order, groups.offsets, groups.tile_base)
+        ctx.tables = tables if any(t.is_inference() for t in tables) else None
+        ctx.save_for_backward(x, weight, y if relu else None, *(tables if ctx.tables is None else ()))
         return y
 
     @staticmethod
     @_first_order
     def backward(ctx, d_y):
-        x, weight, y = ctx.saved_tensors
-        groups, dev = ctx.groups, d_y.device
-        n, (G, N, K), prec = groups.n_rows, weight.shape, _ELEM[d_y.dtype]
+        x, weight, y, *tables = ctx.saved_tensors
+        order, offsets, tile_base = tables or ctx.tables
+        n, (G, N, K), prec, dev = order.numel(), weight.shape, _ELEM[d_y.dtype], d_y.device
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = dw = db = None
         if n == 0:
@@ -993,7 +996,7 @@ class _GroupedLinear(torch.autograd.Function):
             dz = torch.empty((n, N), dtype=g.dtype, device=dev)
             _call("nerf_relu_bwd", "relu_bwd", dev, n, n, N, g.data_ptr(), ld, y.data_ptr(), prec, dz.data_ptr())
             g, ld = dz, N
-        at = (n, G, groups.order.data_ptr(), groups.offsets.data_ptr(), groups.tile_base.data_ptr(), K, N, g.data_ptr(), ld)
+        at = (n, G, order.data_ptr(), offsets.data_ptr(), tile_base.data_ptr(), K, N, g.data_ptr(), ld)
         if need_x:
             dx = torch.empty((n, K), dtype=g.dtype, device=dev)
             work, place, nbytes = _grouped_work(n, G, K, N, 1, prec, dev)

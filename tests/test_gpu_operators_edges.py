@@ -227,6 +227,46 @@ def test_grouped_linear_stays_inside_its_tensors_whatever_the_tables_hold(n, G, 
             assert a[:guard].eq(0x5a).all() and a[-guard:].eq(0x5a).all(), (what, name)
 
 
+# ---- tables written into between forward and backward ------------------------------------------------------------------
+
+def test_grouped_linear_refuses_a_backward_of_other_groups():
+    """as torch does for any tensor that a backward needs"""
+    from nerf_amd import ops
+    x, w = torch.randn(300, 16, device=DEV), torch.randn(4, 8, 16, device=DEV)
+    ids = torch.randint(-1, 4, (300,), device=DEV)
+    for field in ("order", "offsets", "tile_base"):
+        for relu in (False, True):
+            for leaf in (0, 1):
+                groups = ops.group_rows(ids, 4)
+                ops_in = [x.clone(), w.clone()]
+                ops_in[leaf].requires_grad_(True)
+                y = ops.grouped_linear(*ops_in, groups, relu=relu)
+                again = ops.grouped_linear(*ops_in, groups, relu=relu)
+                (want,) = torch.autograd.grad(y.sum(), ops_in[leaf])       # the same groups for several calls
+                y2 = ops.grouped_linear(*ops_in, groups, relu=relu)
+                getattr(groups, field).copy_(getattr(ops.group_rows(3 - ids, 4), field))
+                for late in (again, y2):
+                    with pytest.raises(RuntimeError, match="modified by an inplace"):
+                        late.sum().backward()
+                getattr(groups, field).copy_(getattr(ops.group_rows(ids, 4), field))
+                y3 = ops.grouped_linear(*ops_in, groups, relu=relu)        # written into before the forward: in order
+                assert torch.equal(torch.autograd.grad(y3.sum(), ops_in[leaf])[0], want)
+
+
+def test_groups_made_in_inference_mode_train():
+    from nerf_amd import ops
+    x, w, b = torch.randn(300, 16, device=DEV), torch.randn(4, 8, 16, device=DEV), torch.randn(4, 8, device=DEV)
+    ids = torch.randint(-1, 4, (300,), device=DEV)
+    with torch.inference_mode():
+        inside = ops.group_rows(ids, 4)
+    got = []
+    for groups in (inside, ops.group_rows(ids, 4)):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        y = ops.grouped_linear(leaves[0], leaves[1], groups, bias=leaves[2], relu=True)
+        got.append([y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))])
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
 # ---- layers of the largest sizes that the documentation allows -------------------------------------------------------
 
 def test_grouped_linear_gradient_of_the_largest_layer():
