@@ -338,3 +338,160 @@ def test_gated_scan_of_very_many_sequences(B, D, dtype):
         assert torch.equal(h.detach()[s, 0].float(), want) and torch.equal(last[s], want), lo
         assert torch.equal(d_value[s], d_h[s]), lo
         assert torch.equal(d_gate[s, 0], (d_h[s, 0].float() * state[s]).sum(1, keepdim=True).to(dtype)), lo
+
+
+# ---- weight gradients and products of many rows, exactly ---------------------------------------------------------------
+
+def exact_layer(offsets, n, K, N, dtype, seed=0):
+    """every output and gradient of a layer on whole numbers, bit for bit; offsets: the groups, rows in order"""
+    from nerf_amd import ops
+    g = gen(seed + n + K)
+    G = len(offsets) - 1
+    x, w, d_y = whole(g, -2, 2, n, K), whole(g, -1, 1, G, N, K), whole(g, -1, 1, n, N)
+    b = whole(g, -3, 3, G, N)
+    x[torch.rand(n, generator=g) < 0.5] *= -1
+    xs, ws, bs = (t.to(dtype).to(DEV).requires_grad_(True) for t in (x, w, b))
+    y = ops.grouped_linear(xs, ws, ops.row_groups(torch.tensor(offsets, device=DEV), n), bias=bs)
+    dx, dw, db = torch.autograd.grad(y, (xs, ws, bs), d_y.to(dtype).to(DEV))
+    y, dx, dw, db = (t.detach().cpu() for t in (y, dx, dw, db))
+    assert 2 * n < 2 ** 24 and 2 * K < 2 ** 24 and N < 2 ** 24             # every partial sum is exact in fp32
+    for e in range(G):
+        r = slice(offsets[e], offsets[e + 1])
+        assert torch.equal(y[r], (x[r] @ w[e].T + b[e]).to(dtype)), (e, "y")
+        assert torch.equal(dx[r], (d_y[r] @ w[e]).to(dtype)), (e, "d_x")
+        assert torch.equal(dw[e], (d_y[r].T @ x[r]).to(dtype)), (e, "d_weight")
+        assert torch.equal(db[e], d_y[r].sum(0).to(dtype)), (e, "d_bias")
+    assert y[offsets[-1]:].eq(0).all() and dx[offsets[-1]:].eq(0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(40, 24), (64, 64), (67, 40), (131, 250), (256, 256), (40, 1000)])
+def test_grouped_linear_every_row_counts(K, N, dtype):
+    """groups cut over many workgroups, one that lies inside a single one, empty ones and one of a single row"""
+    exact_layer([0, 45000, 45000, 45090, 45091, 59000, 59000], 60000, K, N, dtype)
+
+
+@pytest.mark.parametrize("K,N,dtype", [(512, 1024, torch.bfloat16), (1024, 512, torch.float16), (256, 256, torch.float32), (255, 257, torch.bfloat16)])
+def test_grouped_linear_long_runs_of_tiles_per_workgroup(K, N, dtype):
+    """more tiles per workgroup than it keeps row numbers of (24 in the weight gradient, 8 or 12 in the products): groups end one
+    tile before, at and behind the places where the numbers are read anew, on ragged tiles and whole ones"""
+    tiles = [23, 1, 1, 22, 1, 24, 48, 1, 95, 24, 25, 200, 2, 24]
+    offsets = [0]
+    for i, t in enumerate(tiles):
+        offsets.append(offsets[-1] + t * 128 - (0, 5, 127, 64)[i % 4])
+    offsets.append(195000)
+    exact_layer(offsets, 200003, K, N, dtype)
+
+
+# ---- as many groups and table rows as there may be -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("n", [1, 100, 2048, 2049, 300001])
+def test_group_rows_of_the_most_groups(n):
+    """ids of 25 bits: four digits in one workgroup, three in blocks"""
+    from nerf_amd import ops
+    G = 2 ** 24
+    ids = torch.randint(-1, G + 1, (n,), generator=gen(n))
+    ids[n // 2:] = ids[n // 2:] % 1000 + G - 1000
+    key = torch.where((ids >= 0) & (ids < G), ids, G)
+    key, order = torch.sort(key, stable=True)
+    offsets = torch.searchsorted(key, torch.arange(G + 1))
+    for dtype in (torch.int32, torch.int64):
+        got = ops.group_rows(ids.to(dtype).to(DEV), G)
+        assert torch.equal(got.order.cpu().long(), order) and torch.equal(got.offsets.cpu().long(), offsets)
+        ends = torch.cat([offsets, torch.tensor([n])])
+        tiles = torch.cat([torch.zeros(1, dtype=torch.int64), ((ends[1:] - ends[:-1] + 127) // 128).cumsum(0)])
+        assert torch.equal(got.tile_base.cpu().long(), tiles)
+
+
+@pytest.mark.parametrize("n,dim", [(5000, 3), (300, 9), (100000, 16)])
+def test_embed_rows_of_the_longest_table(n, dim):
+    from nerf_amd import ops
+    rows = 2 ** 24
+    g = gen(n)
+    ids = torch.randint(0, rows, (n,), generator=g)
+    ids[::3] = rows - 1 - ids[::3] % 5
+    ids[0], ids[n // 2] = -1, rows
+    table = torch.randint(-8, 9, (rows, dim), generator=torch.Generator(DEV).manual_seed(0), device=DEV).bfloat16().requires_grad_(True)
+    d_out = whole(g, -1, 1, n, dim).bfloat16().to(DEV)
+    ids = ids.to(DEV)
+    ok = (ids >= 0) & (ids < rows)
+    out = ops.embed_rows(ids, table, 0.5)
+    assert torch.equal(out.detach(), torch.where(ok[:, None], 0.5 * table.detach()[ids.clamp(0, rows - 1)], torch.zeros((), device=DEV).bfloat16()))
+    grad = torch.autograd.grad(out, table, d_out)[0]
+    want = torch.zeros(rows, dim, device=DEV, dtype=torch.float64).index_add_(0, ids[ok], 0.5 * d_out[ok].double())
+    assert torch.equal(grad, want.bfloat16())
+
+
+# ---- states carried over long distances, exactly -------------------------------------------------------------------------
+
+def long_scan(B, T, D, shared, dtype, seed=0):
+    """Gates of +-1 with a factor of 2 or 1/2 now and then (in turn, so that products stay within 1 and 2) and whole values:
+    h[t] = P[t] (state + sum_{s <= t} value[s] / P[s]) with P the running product of the gates, exactly"""
+    g = gen(seed + T + D)
+    C = 1 if shared else D
+    sign = torch.randint(0, 2, (B, T, C), generator=g) * 2 - 1
+    step = torch.rand(B, T, C, generator=g) < 20.0 / T
+    scale = torch.where(step, torch.where(step.cumsum(1) % 2 == 1, 2.0, 0.5), 1.0)
+    gate = (sign * scale).double()
+    some = 200.0 / T                                                      # few enough that the sums stay small
+    value, state, d_h, d_last = (torch.where(torch.rand(s, generator=g) < max(some, 1.0 if len(s) == 2 else 0.0),
+                                             torch.randint(0, 2, s, generator=g) * 2 - 1, 0).double()
+                                 for s in ((B, T, D), (B, D), (B, T, D), (B, D)))
+    P = gate.cumprod(1)
+    assert P.abs().max() <= 2 and P.abs().min() >= 1
+    total = state[:, None] + (value / P).cumsum(1)
+    h = P * total
+    before = torch.cat([state[:, None], h[:, :-1]], 1)
+    # G[t] P[t] = sum_{s >= t} d_h[s] P[s] + d_last P[T-1]
+    G = ((d_h * P).flip(1).cumsum(1).flip(1) + (d_last * P[:, -1])[:, None]) / P
+    d_gate = G * before
+    if shared:
+        d_gate = d_gate.sum(2, keepdim=True)
+    d_state = gate[:, 0] * G[:, 0]
+    # terms are whole, halves at the least (quarters in products), and no partial sum reaches 2^24 of them
+    assert 4 * (value.abs().sum(1).max() + d_h.abs().sum(1).max() + 2).item() < 2 ** 22
+    assert 4 * (G * before).abs().sum(2).max().item() < 2 ** 24
+    return gate, value, state, d_h, d_last, h, d_gate, G, d_state
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,D", [(1, 1000, 16), (1, 20000, 8), (2, 9000, 3), (2, 5000, 13), (1, 40001, 256), (2, 12000, 64), (1, 20000, 64), (1, 2500, 130), (9, 700, 67),
+                                   (1, 300000, 1)])
+def test_gated_scan_carries_the_state_to_the_far_end(B, T, D, dtype):
+    from nerf_amd import ops
+    from nerf_amd._C import lib
+    code = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[dtype]
+    tiles = lib.nerf_scan_states_floats(B, T, D, code) // (B * D) + 1
+    if (B, T) == (1, 40001):
+        assert tiles > 512                                                # two tiles a segment: more than 256 segments
+    for shared in (True, False):
+        for reverse in (False, True):
+            gate, value, state, d_h, d_last, h, d_gate, d_value, d_state = long_scan(B, T, D, shared, dtype)
+            along = (lambda t: t.flip(1)) if reverse else (lambda t: t)
+            ga, va = (along(t).to(dtype).to(DEV).requires_grad_(True) for t in (gate, value))
+            sa = state.float().to(DEV).requires_grad_(True)
+            got_h, last = ops.gated_scan(ga, va, state=sa, reverse=reverse)
+            grads = torch.autograd.grad((got_h, last), (ga, va, sa), (along(d_h).to(dtype).to(DEV), d_last.float().to(DEV)))
+            assert torch.equal(last.detach().cpu().double(), h[:, -1]), "last"
+            assert torch.equal(got_h.detach().cpu(), along(h).to(dtype)), "h"
+            assert torch.equal(grads[1].cpu(), along(d_value).to(dtype)), "d_value"
+            assert torch.equal(grads[2].cpu().double(), d_state), "d_state"
+            assert torch.equal(grads[0].cpu(), along(d_gate).to(dtype)), "d_gate"
+
+
+# ---- where the scan's range ends -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D,shared", [(4, True), (3, False), (64, True)])
+def test_gated_scan_products_of_gates_up_to_the_range_of_fp32(D, shared):
+    """100 gates in a row whose product is 2^+-120: every state is a power of two and exact, forward and backward"""
+    from nerf_amd import ops
+    for up in (1, -1):
+        gate = torch.ones(1, 100, 1 if shared else D, device=DEV)
+        gate[:, 10:70] = 2.0 ** (2 * up)                                   # 60 samples
+        gate.requires_grad_(True)
+        state = torch.full((1, D), 2.0 ** (-60 * up), device=DEV, requires_grad=True)
+        h, last = ops.gated_scan(gate, torch.zeros(1, 100, D, device=DEV), state=state)
+        want = state.detach()[0, 0].item() * gate.detach()[0, :, 0].double().cumprod(0)
+        assert torch.equal(h.detach()[0].double(), want[:, None].expand(100, D)) and last.detach().eq(2.0 ** (60 * up)).all()
+        d_state = torch.autograd.grad(last, state, torch.full((1, D), 2.0 ** (-60 * up), device=DEV))[0]
+        assert d_state.eq(2.0 ** (60 * up)).all()
