@@ -182,7 +182,7 @@ __device__ __forceinline__ float relu_or_not(float v, float least, unsigned bits
 
 struct Rows {
     int64_t n;
-    int n_groups;
+    int n_groups, most_tiles;
     const int32_t *order, *offsets, *tile_base;
 };
 
@@ -195,6 +195,7 @@ __device__ __forceinline__ int row_at(const Rows& r, int64_t pos) {
 struct LinArgs {
     Rows rows;
     int C, O, tiles_o;           // contraction length, outputs, output tiles
+    int grid_row;                // register form: workgroups per XCD in one row of the grid
     int64_t a_ld;
     int64_t w_ld, w_gs;          // elements between rows and between groups of w
     int w_rows;                  // rows of w where they are the contraction index (C is a whole number of pieces)
@@ -219,7 +220,7 @@ struct Tables {
         } else {
             total = r.tile_base[r.n_groups + 1];
         }
-        total = grp::checked_tiles(total, grp::max_tiles(r.n, r.n_groups));
+        total = grp::checked_tiles(total, r.most_tiles);
     }
     __device__ __forceinline__ Tile tile(const Rows& r, int64_t at, int tiles_o, int bn) const {
         const int G = r.n_groups;
@@ -731,7 +732,7 @@ __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
     // consecutive tiles on one XCD (workgroups go round the eight XCDs), output tiles of the same rows next to each other
     const Tables tables(p.rows, lane);
     const int64_t work = (int64_t)tables.total * p.tiles_o;
-    const int64_t per_xcd = (work + 7) / 8, local = (blockIdx.x >> 3) + (int64_t)blockIdx.y * (gridDim.x >> 3);
+    const int64_t per_xcd = (work + 7) / 8, local = (blockIdx.x >> 3) + (int64_t)blockIdx.y * p.grid_row;
     const int64_t at = (blockIdx.x & 7) * per_xcd + local;
     if (local >= per_xcd || at >= work) return;
     const Tile t = tables.tile(p.rows, at, p.tiles_o, BN);
@@ -960,7 +961,7 @@ __global__ __launch_bounds__(ST_THREADS) void wgrad_stream_kernel(WgradArgs p) {
 
     // the blocks of one chunk next to each other, on one XCD where there are eight chunks or more: they read the same rows
     const int G = p.rows.n_groups, K = p.K, N = p.N;
-    const int tiles = grp::checked_tiles(p.rows.tile_base[G], grp::max_tiles(p.rows.n, G));      // the rows of no group stay out
+    const int tiles = grp::checked_tiles(p.rows.tile_base[G], p.rows.most_tiles);      // the rows of no group stay out
     const int blocks = p.tiles_n * p.tiles_k;
     const int64_t chunks = (tiles + p.chunk - 1) / p.chunk;
     const int64_t per_xcd = (chunks * blocks + 7) / 8, local = blockIdx.x >> 3;
@@ -1156,7 +1157,7 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
 
     // the blocks of one chunk next to each other, on one XCD where there are eight chunks or more: they read the same rows
     const int G = p.rows.n_groups;
-    const int tiles = grp::checked_tiles(p.rows.tile_base[G], grp::max_tiles(p.rows.n, G));      // the rows of no group stay out
+    const int tiles = grp::checked_tiles(p.rows.tile_base[G], p.rows.most_tiles);      // the rows of no group stay out
     const int blocks = p.tiles_n * p.tiles_k;
     const int64_t work = (int64_t)((tiles + p.chunk - 1) / p.chunk) * blocks;
     const int64_t per_xcd = (work + 7) / 8;
@@ -1300,26 +1301,26 @@ __global__ __launch_bounds__(THREADS, 2) void wgrad_kernel(WgradArgs p) {
 
 // Groups whose tiles lie in several chunks: the sum of their pieces in order; groups without rows: zeros.
 template <typename T>
-__global__ __launch_bounds__(THREADS) void wgrad_join_kernel(WgradArgs p) {
+__global__ __launch_bounds__(THREADS) void wgrad_join_kernel(WgradArgs p, int64_t first) {
     const int g = blockIdx.y;
-    const int64_t most = grp::max_tiles(p.rows.n, p.rows.n_groups);
-    const int b0 = grp::checked_tiles(p.rows.tile_base[g], most), b1 = grp::checked_tiles(p.rows.tile_base[g + 1], most);
-    const int c0 = b0 / p.chunk, c1 = b1 > b0 ? (b1 - 1) / p.chunk : c0;
+    const int b0 = grp::checked_tiles(p.rows.tile_base[g], p.rows.most_tiles), b1 = grp::checked_tiles(p.rows.tile_base[g + 1], p.rows.most_tiles);
+    const unsigned chunk = (unsigned)p.chunk;                               // most workgroups end here: no signs to divide with
+    const int c0 = (int)((unsigned)b0 / chunk), c1 = b1 > b0 ? (int)((unsigned)(b1 - 1) / chunk) : c0;
     if (b1 > b0 && c0 == c1) return;
-    const int64_t NK = (int64_t)p.N * p.K, all = p.db ? NK + p.N : NK;
-    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < all; i += (int64_t)gridDim.x * THREADS) {
-        const bool is_w = i < NK;
-        const float* part = is_w ? p.part_w + i : p.part_b + (i - NK);
-        const int64_t ld = is_w ? NK : p.N;
-        float sum = 0.0f;
-        if (b1 > b0) {
-            sum = part[(2 * (int64_t)c0 + 1) * ld];
+    const int64_t NK = (int64_t)p.N * p.K;
+    const int64_t i = first + (int64_t)blockIdx.x * THREADS + threadIdx.x;
+    const bool is_w = i < NK;
+    if (!is_w && !(p.db && i < NK + p.N)) return;
+    const float* part = is_w ? p.part_w + i : p.part_b + (i - NK);
+    const int64_t ld = is_w ? NK : p.N;
+    float sum = 0.0f;
+    if (b1 > b0) {
+        sum = part[(2 * (int64_t)c0 + 1) * ld];
 #pragma unroll 8
-            for (int c = c0 + 1; c <= c1; ++c) sum += part[2 * (int64_t)c * ld];
-        }
-        if (is_w) ((T*)p.dw)[g * NK + i] = (T)sum;
-        else ((T*)p.db)[(int64_t)g * p.N + (i - NK)] = (T)sum;
+        for (int c = c0 + 1; c <= c1; ++c) sum += part[2 * (int64_t)c * ld];
     }
+    if (is_w) ((T*)p.dw)[g * NK + i] = (T)sum;
+    else ((T*)p.db)[(int64_t)g * p.N + (i - NK)] = (T)sum;
 }
 
 // Rows that are not whole pieces, copied to rows that are, for the streaming forms: with zeros behind the last column, or
@@ -1467,6 +1468,7 @@ static int launch_linear(const LinArgs& args, int precision, bool wide, void* st
     const int64_t work = xcd_grid(tiles * p.tiles_o), row = work < MAX_GRID ? work : MAX_GRID;
     NERF_REQUIRE((work + row - 1) / row < 65536, NERF_E_SHAPE);
     const dim3 grid((unsigned)row, (unsigned)((work + row - 1) / row));
+    p.grid_row = (int)(row / 8);
 #define NERF_CALL(T)                                                                                                           \
     do {                                                                                                                       \
         if (bn == 128) hipLaunchKernelGGL((linear_kernel<T, WT, 128>), grid, dim3(THREADS), 0, st, p);                         \
@@ -1503,7 +1505,7 @@ extern "C" int nerf_grouped_fwd(int64_t n, int64_t n_groups, const int32_t* orde
                  nerf_aligned(bias, (uintptr_t)es) && nerf_aligned(workspace, 256), NERF_E_ALIGN);
     NERF_REQUIRE(workspace_bytes >= nerf_grouped_workspace_bytes(n, n_groups, K, N, 0, precision), NERF_E_WORKSPACE);
     gl::LinArgs p = {};
-    p.rows = {n, (int)n_groups, order, offsets, tile_base};
+    p.rows = {n, (int)n_groups, (int)grp::max_tiles(n, n_groups), order, offsets, tile_base};
     p.C = K; p.O = N; p.a = x; p.a_ld = x_ld; p.w = weight; p.w_ld = K; p.w_gs = (int64_t)N * K; p.bias = bias; p.relu = relu ? 1 : 0; p.out = y;
     const bool whole = K % E == 0 && x_ld % E == 0 && nerf_aligned(x, 16) && nerf_aligned(weight, 16) && N >= E;
     if (pad.fwd) {
@@ -1548,7 +1550,7 @@ extern "C" int nerf_grouped_bwd_data(int64_t n, int64_t n_groups, const int32_t*
                  nerf_aligned(workspace, 256), NERF_E_ALIGN);
     NERF_REQUIRE(workspace_bytes >= nerf_grouped_workspace_bytes(n, n_groups, K, N, 1, precision), NERF_E_WORKSPACE);
     gl::LinArgs p = {};
-    p.rows = {n, (int)n_groups, order, offsets, tile_base};
+    p.rows = {n, (int)n_groups, (int)grp::max_tiles(n, n_groups), order, offsets, tile_base};
     p.C = N; p.O = K; p.a = d_z; p.a_ld = d_z_ld; p.w = weight; p.w_ld = K; p.w_gs = (int64_t)N * K; p.w_rows = N; p.out = d_x;
     bool a_whole = N % E == 0 && d_z_ld % E == 0 && nerf_aligned(d_z, 16), w_whole = K % E == 0 && nerf_aligned(weight, 16);
     if (pad.data && (a_whole || N % E) && (w_whole || K % E)) {
@@ -1622,7 +1624,7 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
     const bool wide = !small && d_whole && x_whole;
     const gl::WgradPlan w = gl::wgrad_plan(n, n_groups, K, N, wide, precision);
     gl::WgradArgs p = {};
-    p.rows = {n, (int)n_groups, order, offsets, tile_base};
+    p.rows = {n, (int)n_groups, (int)grp::max_tiles(n, n_groups), order, offsets, tile_base};
     p.K = K; p.N = N; p.Kp = pad.Kp; p.Np = pad.Np; p.tiles_k = w.tiles_k; p.tiles_n = w.tiles_n; p.chunk = w.chunk;
     p.x_ld = x_ld; p.dy_ld = d_z_ld; p.x = x; p.dy = d_z; p.dw = d_weight; p.db = d_bias;
     p.part_w = (float*)((char*)workspace + w.part_w);
@@ -1632,7 +1634,6 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
     NERF_REQUIRE(grid <= 2 * gl::MAX_GRID - 8, NERF_E_SHAPE);               // 512 threads each
     hipStream_t st = (hipStream_t)stream;
     const int64_t join_blocks = ((int64_t)N * K + N + gl::THREADS - 1) / gl::THREADS;
-    const dim3 join((unsigned)(join_blocks < gl::MAX_GRID ? join_blocks : gl::MAX_GRID), (unsigned)n_groups);
 #define NERF_WG(T, BT) hipLaunchKernelGGL((gl::wgrad_kernel<T, BT>), dim3((unsigned)grid), dim3(gl::THREADS), 0, st, p)
 #define NERF_WS(T, BX) hipLaunchKernelGGL((gl::wgrad_stream_kernel<T, BX>), dim3((unsigned)grid), dim3(gl::ST_THREADS), 0, st, p)
 #define NERF_CALL(T)                                                                                   \
@@ -1644,7 +1645,10 @@ extern "C" int nerf_grouped_bwd_weights(int64_t n, int64_t n_groups, const int32
         else if (wide) NERF_WS(T, 128);                                                                \
         else if (w.bd == 128) NERF_WG(T, 128);                                                         \
         else NERF_WG(T, 64);                                                                           \
-        hipLaunchKernelGGL(gl::wgrad_join_kernel<T>, join, dim3(gl::THREADS), 0, st, p);               \
+        for (int64_t b = 0; b < join_blocks; b += gl::MAX_GRID) {                                      \
+            const dim3 join((unsigned)(join_blocks - b < gl::MAX_GRID ? join_blocks - b : gl::MAX_GRID), (unsigned)n_groups); \
+            hipLaunchKernelGGL(gl::wgrad_join_kernel<T>, join, dim3(gl::THREADS), 0, st, p, b * gl::THREADS); \
+        }                                                                                              \
     } while (0)
     NERF_ELEM_DISPATCH(precision, NERF_CALL);
 #undef NERF_CALL

@@ -20,17 +20,15 @@ int launch_group_rows(int64_t n, const void* ids, int id_bytes, int64_t n_groups
 // nerf_group_rows or nerf_group_offsets wrote give wrong sums, never an access outside the tensors or a loop without end.
 
 // tiles of n rows in n_groups groups and of the rows of no group, at most
-__host__ __device__ __forceinline__ int64_t max_tiles(int64_t n, int64_t n_groups) { return n / TILE_ROWS + n_groups + 1; }
-__host__ __device__ __forceinline__ int checked_tiles(int tiles, int64_t most) {
-    return tiles < 0 ? 0 : tiles < most ? tiles : (int)most;
-}
+static inline int64_t max_tiles(int64_t n, int64_t n_groups) { return n / TILE_ROWS + n_groups + 1; }
+__device__ __forceinline__ int checked_tiles(int tiles, int most) { return min(max(tiles, 0), most); }
 
 // Rows of a tile that begins at position `pos` and ends at `end` or 128 rows later: at least one, all in [0, n) (n >= 1)
 struct Span {
     int64_t pos;
     int count;
 };
-__host__ __device__ __forceinline__ Span checked_span(int64_t pos, int64_t end, int64_t n) {
+__device__ __forceinline__ Span checked_span(int64_t pos, int64_t end, int64_t n) {
     pos = pos < 0 ? 0 : pos < n ? pos : n - 1;
     const int64_t left = (end < n ? end : n) - pos;
     return {pos, left < 1 ? 1 : left < TILE_ROWS ? (int)left : TILE_ROWS};
