@@ -13,6 +13,9 @@
 // The ragged ends of a workgroup's lane groups meet in LDS, those of the workgroups in the workspace, where a second
 // kernel adds them up in order of position and writes zeros for the rows that nothing reads.  No atomics: the result
 // does not depend on timing, and an id that holds all positions is spread over all workgroups like any other.
+// A term of the sum passes few fp32 additions however many there are: at most 64 in its lane group, G in LDS (G = 256 / LPR),
+// n / (64 G^2) or 1024 / G and then G more over the workgroups.  524 288 terms of one row, fp32: 115 to 211 additions at most, error 7e-8 of the
+// sum of magnitudes.
 #include "elems.hpp"
 #include "groups.hpp"
 
@@ -104,6 +107,8 @@ __device__ __forceinline__ void add_part(float (&acc)[VEC], const float* p) {
     }
 }
 
+// Four workgroups to a compute unit: 16-bit tensors spill one register for it, and are no slower (524 288 x 128 fp16, the whole
+// gradient: 101 us, 103 with three and no spill).
 template <typename T, int VEC>
 __global__ __launch_bounds__(THREADS, 4) void bwd_sum_kernel(BwdArgs a, const T* __restrict__ d_out, int64_t ld, T* __restrict__ d_table) {
     constexpr int BATCH = 8;

@@ -14,10 +14,11 @@
 // Anything else goes through registers, one workgroup per tile (linear_kernel, wgrad_kernel), or is copied to whole pieces
 // first (pad_plan).
 //
-// Bounds: 256 -> 256 features move 1 KiB per row for 128 kflop, memory at 16 bits (floor 39 us for 196 608 rows; 57 forward,
-// 59 data gradient, 65 weight gradient) and the fp32 matrix instructions at 32 (65 536 rows: 56 us; 102, 110, 113).  1024 ->
-// 1024 features are bound by the copies into LDS, 29 bytes per ns and compute unit (65 536 rows fp16, 64 uneven groups: 220 to
-// 239 us; one group 170 us, 0.81 PFLOP/s, where a large library product reaches 1.06).
+// Bounds: 256 -> 256 features move 1 KiB per row for 128 kflop, memory at 16 bits (196 608 rows, inputs from memory: forward
+// 70 us, data gradient 66, weight gradient 67, over a floor of 39, 39 and 28; inputs partly in the last-level cache 56, 54 and 57)
+// and the fp32 matrix instructions at 32 (65 536 rows: 91, 93 and 103 us over 56, matrix pipes 55 % busy).  1024 -> 1024 features
+// are bound by the copies into LDS, 33 to 37 bytes per ns and compute unit (65 536 rows fp16: forward 165 to 180 us with one group,
+// 0.76 to 0.83 PFLOP/s where a large library product reaches 1.06; 190 to 204 with 64 uneven ones; matrix pipes 38 % busy).
 //
 // A 16-byte piece holds the values of consecutive contraction indices of one row; operands whose contraction index is the
 // row (W in dX, both in dW) are read with ds_read_b64_tr_b16, which hands a lane four rows of its column, or in fp32 with
@@ -262,7 +263,7 @@ struct Tables {
 // row, and one exchange between the wave's halves (v_permlane32_swap) makes them eight, a 16-byte store.
 constexpr int ST_THREADS = 512;
 // items whose rows and bias are in LDS at a time; 64 outputs leave room for two workgroups in a compute unit's LDS
-// (65 536 rows 256 -> 256 fp32: 102 us with two, 111 with one)
+// (65 536 rows 256 -> 256 fp32, forward in short bursts of calls: 102 us with two, 111 with one)
 template <int BN> constexpr int st_items() { return BN == 64 ? 8 : 12; }
 
 // Output number of place o.  The last piece of a row ends where the row does, so it may repeat outputs of the one before, and
@@ -715,7 +716,7 @@ __global__ __launch_bounds__(ST_THREADS) void stream_kernel(LinArgs p) {
 
 // ---- through registers: any row length, any alignment ------------------------------------------------------------
 // The same product, one workgroup of four waves per tile of 128 rows x BN outputs; a step is requested before the products of
-// the one before it (65 536 rows, 67 -> 256 bf16: forward 24 us, data gradient 39; in whole pieces, 64 -> 256, 19 and 14).
+// the one before it (65 536 rows, 67 -> 256 bf16: forward 24 us, 28 with a bias; in whole pieces, 64 -> 256, 18).
 template <typename T, bool WT, int BN>
 __global__ __launch_bounds__(THREADS, 2) void linear_kernel(LinArgs p) {
     constexpr int E = piece<T>(), BK = step_len<T>();
@@ -1338,9 +1339,10 @@ __global__ __launch_bounds__(THREADS) void pad_kernel(int64_t rows, int cols, co
     }
 }
 
-// dZ = dY where the ReLU let something through.  Memory bound: 196 608 x 256 bf16 in 51 us, 5.9 TB/s.  Written out once, because
-// the gate inside the two products costs more: their tiles are bound by what they copy into LDS, and the gate is a third
-// operand (in the same shape, data gradient 125 us gated and 59 not, weight gradient 116 and 66).
+// dZ = dY where the ReLU let something through.  Memory bound: 196 608 x 256 bf16 in 53 us, 5.7 TB/s; a layer of that size
+// trains in 251 us with its ReLU and 190 without.  Written out once, because the gate inside the two products cost more when it
+// was there: their tiles are bound by what they copy into LDS, and the gate is a third operand (data gradient 125 us gated and 59
+// not, weight gradient 116 and 66, in short bursts of calls).
 template <typename T>
 __global__ __launch_bounds__(THREADS) void relu_bwd_kernel(int64_t n, int N, const T* dy, int64_t ld, const T* y, T* dz) {
     constexpr int E = piece<T>();

@@ -21,6 +21,10 @@
 // When the sequences alone do not fill the chip, a sequence is cut into segments: a first pass over a and v (or g) leaves
 // each segment's map, a small kernel composes them, and the main pass starts every segment from its state.  That reads
 // the inputs twice; the second time they come from the last-level cache as far as they fit.
+//
+// A gate that repeats over sequences or samples (one learned gate per channel, say) has a gradient that is a sum over them: the
+// terms are written in fp32 and added up in a fixed order by sum_kernel (4096 x 192 x 64 bf16, gate [1, 192, 64]: backward 128 us
+// for the terms and 36 for their sum).
 #include "elems.hpp"
 
 namespace nerf {
@@ -326,8 +330,9 @@ __global__ __launch_bounds__(THREADS) void fwd_kernel(Args a) {
 template <typename T, int V, bool SHARED, bool AGG, typename G = T>
 __global__ __launch_bounds__(THREADS, 2) void bwd_kernel(Args a) {
     constexpr int VA = SHARED ? 1 : V, L = max_len<V>();
-    // A tile is requested ahead, except where three fp32 tensors per channel would leave one wave per SIMD (or spill):
-    // 2 x 262 144 x 64 fp32, gate per channel: 225 us ahead, 203 not; 4096 x 192 x 64 bf16, one gate: 102 ahead, 152 not.
+    // A tile is requested ahead, except where three fp32 tensors per channel would leave one wave per SIMD: 2 x 262 144 x 64 fp32,
+    // gate per channel: 225 us ahead, 203 not; 4096 x 192 x 64 bf16, one gate: 102 ahead, 152 not.  16 bits with a gate per channel
+    // takes all 256 registers and spills five, and is faster for it: 4096 x 192 x 64 bf16 119 us ahead, 159 not.
     constexpr bool AHEAD = AGG || SHARED || V != 4;
     __shared__ float sm[WAVES * 64 * (V + VA)];
     const Geo& g = a.g;

@@ -422,6 +422,33 @@ def test_embed_rows_of_the_longest_table(n, dim):
     assert torch.equal(grad, want.bfloat16())
 
 
+# ---- long sums of the table's gradient in fp32 -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", [128, 20, 3])
+def test_embed_rows_gradient_of_half_a_million_terms(dim):
+    """A term passes at most 64 additions in its lane group, G in LDS (G = 256 threads / lanes of a row), n / (span G) + 1 over
+    workgroups of span = 64 G positions or less and G more, and the scale: far fewer than the terms of the sum."""
+    from nerf_amd import ops
+    n = 524288
+    g = gen(dim)
+    d_out = torch.randn(n, dim, generator=g) + 0.25                       # a sum that grows, with terms of either sign
+    leaf = torch.zeros(3, dim, device=DEV, requires_grad=True)
+    ids = torch.ones(n, dtype=torch.int64)
+    ids[::1000] = 2
+    grad = torch.autograd.grad(ops.embed_rows(ids.to(DEV), leaf, 2.0), leaf, d_out.to(DEV))[0]
+    lanes = 4
+    while lanes < 64 and lanes * (4 if dim >= 4 else 1) < dim:
+        lanes *= 2
+    groups = 256 // lanes
+    per = min(64, max(8, (n // (groups * 1024) + 7) // 8 * 8))
+    most = per + groups + (n // (groups * per) + groups) // groups + 1 + groups + 1
+    exact, mag, _ = R.embed_rows_grad(ids, 3, d_out, 2.0)
+    err = (grad.cpu().double() - exact).abs()[1:] / mag[1:]
+    print(f"dim {dim}: {most} roundings at most, worst error {err.max().item():.2e} of the magnitude, {((grad.cpu().double() - exact).abs() / exact.abs())[1].max().item():.2e} of the value")
+    close(grad, exact, mag, most)
+    assert grad[0].eq(0).all()
+
+
 # ---- states carried over long distances, exactly -------------------------------------------------------------------------
 
 def long_scan(B, T, D, shared, dtype, seed=0):
