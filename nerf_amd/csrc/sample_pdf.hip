@@ -223,6 +223,17 @@ __global__ __launch_bounds__(256) void sample_merge_kernel(int64_t n_rays, int S
     store_sorted<E>(v, zout + ray * n, n, lane);
 }
 
+// Rays of one launch: a wave each, and a direction of a grid holds fewer than 2^32 threads (the runtime cuts off what passes
+// them, without an error).  FN(first ray, rays, workgroups) for each run of rays.
+constexpr int64_t LAUNCH_RAYS = (int64_t)1 << 24;
+template <typename F>
+static inline void for_runs_of_rays(int64_t n_rays, F fn) {
+    for (int64_t r = 0; r < n_rays; r += LAUNCH_RAYS) {
+        const int64_t m = n_rays - r < LAUNCH_RAYS ? n_rays - r : LAUNCH_RAYS;
+        fn(r, m, (unsigned)((m + 3) / 4));
+    }
+}
+
 static inline int elems_per_lane(int n) {
     int e = 1;
     while (64 * e < n) e <<= 1;
@@ -240,10 +251,12 @@ extern "C" int nerf_sample_pdf(int64_t n_rays, int n_bins, const float* bins, in
     NERF_REQUIRE(bins && weights && samples, NERF_E_NULL);
     const int lds_stride = (n_bins + 3) & ~3;
     const size_t lds = (size_t)4 * 2 * lds_stride * sizeof(float);
-    const int64_t blocks = (n_rays + 3) / 4;
-    NERF_REQUIRE(blocks <= 0x7fffffff, NERF_E_SHAPE);
-    hipLaunchKernelGGL(nerf::sample_pdf_kernel, dim3((unsigned)blocks), dim3(256), lds, (hipStream_t)stream,
-                       n_rays, n_bins, bins, bins_ld, weights, w_ld, n_samples, u, samples, inds, lds_stride);
+    nerf::for_runs_of_rays(n_rays, [&](int64_t r, int64_t m, unsigned blocks) {
+        const int64_t at = r * n_samples;
+        hipLaunchKernelGGL(nerf::sample_pdf_kernel, dim3(blocks), dim3(256), lds, (hipStream_t)stream, m, n_bins, bins + r * bins_ld,
+                           bins_ld, weights + r * w_ld, w_ld, n_samples, u ? u + at : nullptr, samples + at, inds ? inds + at : nullptr,
+                           lds_stride);
+    });
     return nerf_launch_status();
 }
 
@@ -252,11 +265,12 @@ extern "C" int nerf_sort_rows(int64_t n_rows, int n_a, const float* a, int n_b, 
     NERF_REQUIRE(n_rows >= 0 && n_a >= 1 && n_b >= 0 && n_a + n_b <= 1024, NERF_E_SHAPE);
     if (n_rows == 0) return NERF_OK;
     NERF_REQUIRE(a && out && (b || n_b == 0), NERF_E_NULL);
-    const int64_t blocks = (n_rows + 3) / 4;
-    NERF_REQUIRE(blocks <= 0x7fffffff, NERF_E_SHAPE);
-    const dim3 grid((unsigned)blocks), block(256);
     hipStream_t st = (hipStream_t)stream;
-#define NERF_SORT(E) hipLaunchKernelGGL(nerf::sort_rows_kernel<E>, grid, block, 0, st, n_rows, n_a, a, n_b, b, out)
+#define NERF_SORT(E)                                                                                                  \
+    nerf::for_runs_of_rays(n_rows, [&](int64_t r, int64_t m, unsigned blocks) {                                       \
+        hipLaunchKernelGGL(nerf::sort_rows_kernel<E>, dim3(blocks), dim3(256), 0, st, m, n_a, a + r * n_a, n_b,       \
+                           n_b ? b + r * n_b : b, out + r * (n_a + n_b));                                             \
+    })
     switch (nerf::elems_per_lane(n_a + n_b)) {
         case 1: NERF_SORT(1); break;
         case 2: NERF_SORT(2); break;
@@ -275,13 +289,14 @@ extern "C" int nerf_sample_merge(int64_t n_rays, int Sc, const float* z_coarse, 
     NERF_REQUIRE(z_coarse && w_coarse && z_out, NERF_E_NULL);
     const int lds_stride = (Sc + 3) & ~3, n_pad = (Sc + n_fine + 3) & ~3;
     const size_t lds = (size_t)4 * 2 * (lds_stride + n_pad) * sizeof(float);        // at most 64 KiB
-    const int64_t blocks = (n_rays + 3) / 4;
-    NERF_REQUIRE(blocks <= 0x7fffffff, NERF_E_SHAPE);
-    const dim3 grid((unsigned)blocks), block(256);
     hipStream_t st = (hipStream_t)stream;
-#define NERF_SM(E)                                                                                        \
-    hipLaunchKernelGGL(nerf::sample_merge_kernel<E>, grid, block, lds, st, n_rays, Sc, z_coarse, w_coarse, \
-                       n_fine, u, z_out, z_fine_out, lds_stride, n_pad)
+#define NERF_SM(E)                                                                                                        \
+    nerf::for_runs_of_rays(n_rays, [&](int64_t r, int64_t m, unsigned blocks) {                                           \
+        const int64_t at = r * n_fine;                                                                                    \
+        hipLaunchKernelGGL(nerf::sample_merge_kernel<E>, dim3(blocks), dim3(256), lds, st, m, Sc, z_coarse + r * Sc,       \
+                           w_coarse + r * Sc, n_fine, u ? u + at : nullptr, z_out + r * (Sc + n_fine),                     \
+                           z_fine_out ? z_fine_out + at : nullptr, lds_stride, n_pad);                                     \
+    })
     switch (nerf::elems_per_lane(Sc + n_fine)) {
         case 1: NERF_SM(1); break;
         case 2: NERF_SM(2); break;
